@@ -78,7 +78,7 @@ def draw(rng):
     H = rng.choice((16, 32, 64)) if shared else HK * rng.choice((1, 3, 4, 8, 16))
     case = {"kind": kind, "S": 1, "spread": rng.choice((0.0, 1.0, 4.0, 10.0)), "e4m3": rng.random() < 0.4,
             "shared": shared, "sink": rng.random() < 0.4, "track": False, "H": H, "HK": HK, "D": D,
-            "page": rng.choice((8, 16, 32, 64, 128, 256))}
+            "page": rng.choice((16, 16, 32, 64, 128, 256))}
     row = HK * D * (1 if case["e4m3"] else 2) * (1 if shared else 2)
     if kind == "attend":
         case["S"] = rng.choice((1, 1, 1, 2, 4, 7))
