@@ -362,6 +362,70 @@ int wz_sparse_attn(const void* q_bf16, const void* kv_bf16, const float* attn_si
                    int64_t D, int64_t N, int64_t topk, float softmax_scale, void* workspace,
                    int64_t workspace_bytes, hipStream_t stream);
 
+/* A paged key-value cache (no counterpart in the reference, whose cache is one
+ * contiguous row per sequence, architecture.py:596-600): slot t of sequence b lies in
+ * row t % page_size of page table[b, t / page_size].  Every array is dense
+ * [pages, kv_heads, page_size(, head_dim)], so a head's rows of a page are contiguous.
+ * K and V are separate (head_dim 64, 128, 256) or one row that serves as both, as
+ * sparse_attn's latents do (v NULL; head_dim 128, 256, 512).  dtype WZ_KV_E4M3 holds
+ * e4m3 codes with one float32 scale for each row (act_quant's rule over the row:
+ * max(amax, 1e-4) / 448).  weights and positions make the cache a tracked one: the
+ * attention weight a slot has been given so far, and the token position it holds.
+ * page_size is a power of two from 16 to 1024; k, v 16-byte aligned.  Pages whose id
+ * lies outside [0, pages) hold nothing: they are not read, written or moved.
+ * A tracked cache's pages belong to one sequence each; others may share pages that
+ * are only read. */
+#define WZ_KV_BF16 0
+#define WZ_KV_E4M3 1
+typedef struct wz_paged_kv {
+  void* k;
+  void* v;            /* NULL: V = K */
+  float* k_scale;     /* WZ_KV_E4M3 only */
+  float* v_scale;     /* WZ_KV_E4M3 with a v only */
+  float* weights;     /* NULL: not tracked */
+  int32_t* positions; /* with weights */
+  int64_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;      /* WZ_KV_* */
+} wz_paged_kv;
+
+/* New tokens into their pages: row i of k (and v) [B, S, kv_heads, head_dim] bf16 of
+ * sequence b to slot start[b] + i, for i < count[b] (NULL: S).  k_strides, v_strides: the
+ * elements between sequences, tokens and heads (host, multiples of 8; rows dense and
+ * 16-byte aligned).  A tracked slot starts with weight 0 and position
+ * position[b] + i (NULL: its slot).  Slots outside the table are dropped. */
+int wz_paged_kv_write(const wz_paged_kv* cache, const void* k_bf16, const int64_t* k_strides, const void* v_bf16,
+                      const int64_t* v_strides, const int32_t* table, int64_t table_width, const int32_t* start,
+                      const int32_t* count, const int32_t* position, int64_t B, int64_t S, hipStream_t stream);
+
+/* Attention of S new tokens a sequence (1..16, already written, causal among themselves)
+ * over every cached token: row (i, h) of sequence b sees the slots below
+ * lens[b] - (S - 1 - i); o = sum_j p_j v_j / (sum_j p_j + exp(sink[h] - m)), p_j =
+ * exp(q . k_j scale - m), m the maximum; a row that sees nothing gets 0.  q [B, S, H,
+ * head_dim] bf16 (q_strides as above), H a multiple of kv_heads, query head h reading KV
+ * head h / (H / kv_heads); attn_sink [H] float32 or NULL; o dense bf16.  accumulate adds to
+ * each slot's weight the attention that the rows of its KV head give it, in a fixed
+ * order (a tracked cache, one call at a time).  lens beyond the table are cut to it. */
+int64_t wz_paged_attn_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t S, int64_t H, int64_t table_width,
+                                      int accumulate);
+int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q_strides, const float* attn_sink,
+                  const int32_t* table, int64_t table_width, const int32_t* lens, void* o_bf16, int64_t B, int64_t S,
+                  int64_t H, float softmax_scale, int accumulate, void* workspace, int64_t workspace_bytes,
+                  hipStream_t stream);
+
+/* Cuts every sequence of a tracked cache to `keep` slots, in place: for each KV head the
+ * slots with positions below `first`, the `recent` newest positions and then those of the
+ * highest weight stay (NaN counts as the lowest, equal weights go by the lower slot);
+ * the i-th dropped slot below `keep` takes over the i-th kept slot from `keep` on, with
+ * its K, V, scales, weight and position.  new_lens[b] = min(lens[b], keep) (may be lens
+ * itself); sequences within the budget are left as they are.  first + recent <= keep. */
+int64_t wz_paged_evict_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t table_width, int64_t keep);
+int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, int64_t table_width, const int32_t* lens,
+                   int32_t* new_lens, int64_t B, int64_t keep, int64_t first, int64_t recent, void* workspace,
+                   int64_t workspace_bytes, hipStream_t stream);
+
 /* The FP8 wire format of a pipeline-stage boundary — _pack_t / _unpack_t
  * (serving/chain.py:208-222): per row scale = bf16(clamp(amax/448, 1e-8, bf16 max)),
  * q = e4m3(clamp(x/scale, +-448)); unpack y = bf16(q * scale).  x, y [M, D] bf16,

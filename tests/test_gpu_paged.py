@@ -1,0 +1,573 @@
+"""The paged cache (wanferenz_amd.paged.PagedKV) against 64-bit statements of its operators.
+
+Tolerances of the attention, per element, from what is rounded: the output to bf16, half a step
+2^-8 |o|; every p_j (times an e4m3 row's scale) to bf16 before the product with V, 2^-8 sum p_j |v_j|;
+and 32-bit arithmetic: a score of D products is off by at most (D + 8) 2^-24 sum |q k| scale (plus its
+maximum's own 2^-23), which moves a p_j by twice that relatively, with 2^-20 for the exponentials,
+their sum and the joined parts.  A slot's accumulated weight has the last part only.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as op
+from wanferenz_amd.paged import PagedKV
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+
+
+def make(gpu, seed, lens, *, HK, D, page, dtype=torch.bfloat16, shared=False, track=False, spare=2, width=None,
+         fill=None, kv_scale=1.0):
+    """A cache whose sequences hold random rows; every other slot of the pools holds ``fill`` (NaN)."""
+    rng = np.random.default_rng(seed)
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    width = max(need + [1]) if width is None else width
+    P = sum(need) + spare
+    order = rng.permutation(P)
+    table = np.full((len(lens), width), -1, dtype=np.int32)
+    at = 0
+    for b, c in enumerate(need):
+        table[b, :c] = order[at:at + c]
+        at += c
+    sides = ["k"] if shared else ["k", "v"]
+    q = dtype == E4M3
+    pools, vals = {}, {}
+    live = np.zeros((P, page), dtype=bool)
+    for b, n in enumerate(lens):
+        for t in range(n):
+            live[table[b, t // page], t % page] = True
+    lv = torch.from_numpy(live)[:, None, :].expand(P, HK, page)
+    for s in sides:
+        x = (torch.randn(P, HK, page, D, generator=g) * kv_scale).to(torch.bfloat16)
+        if q:
+            sc = x.float().abs().amax(-1).clamp(min=1e-4) * (1.0 / 448.0)
+            code = (x.float() / sc[..., None]).clamp(-448, 448).to(E4M3)
+            vals[s] = code.double().numpy() * sc.double().numpy()[..., None]
+            raw = code.view(torch.uint8).clone()
+            raw[~lv] = 0x7F  # NaN
+            pools[s] = raw.view(E4M3)
+            pools[s + "_scale"] = torch.where(lv, sc, torch.tensor(float("nan")))
+        else:
+            vals[s] = x.double().numpy()
+            pools[s] = torch.where(lv[..., None], x, torch.tensor(float("nan"), dtype=torch.bfloat16))
+    if track:
+        pools["weights"] = torch.rand(P, HK, page, generator=g)
+        pools["positions"] = torch.from_numpy(rng.permutation(P * HK * page).astype(np.int32)).view(P, HK, page)
+    dev = {n: t.to(gpu).contiguous() for n, t in pools.items()}
+    cache = PagedKV(dev.pop("k"), dev.pop("v", None), **dev)
+    return cache, vals, torch.from_numpy(table).to(gpu), table
+
+
+def queries(gpu, seed, B, S, H, D, scale=1.0, strided=False):
+    g = torch.Generator().manual_seed(seed + 1000)
+    q = (torch.randn(B, S, H, D, generator=g) * scale).to(torch.bfloat16)
+    if not strided:
+        return q.to(gpu), q.double().numpy()
+    rows = torch.full((B, S, (H + 2) * D), float("nan"), dtype=torch.bfloat16)
+    rows[..., D:(H + 1) * D] = q.view(B, S, H * D)
+    return rows.to(gpu)[..., D:(H + 1) * D].view(B, S, H, D), q.double().numpy()
+
+
+def bounds(o, mag, reach, D):
+    e32 = 2 * (D + 10) * 2.0 ** -24 * max(reach, 1.0) + 2.0 ** -20
+    return 2.0 ** -8 * (np.abs(o) + mag) * 1.01 + e32 * mag + 1e-30, e32
+
+
+def check(got, ref, D):
+    o, mag, _, reach = ref
+    tol, _ = bounds(o, mag, reach, D)
+    err = np.abs(got.double().cpu().numpy() - o)
+    assert np.isfinite(err).all(), "not finite"
+    assert (err <= tol).all(), (float((err / tol).max()), np.unravel_index((err / tol).argmax(), err.shape))
+
+
+LAYOUTS = [  # HK, g, D, shared
+    (2, 4, 128, False), (8, 1, 128, False), (1, 16, 64, False), (2, 3, 64, False), (2, 5, 256, False),
+    (1, 8, 128, True), (1, 20, 256, True), (1, 16, 512, True), (1, 64, 512, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("HK,g,D,shared", LAYOUTS)
+def test_attend_layouts(gpu, HK, g, D, shared, dtype):
+    """Head layouts and widths, one token, ragged lengths among them 0 and 1, NaN in every slot
+    that no sequence holds."""
+    lens = [0, 1, 16, 17, 33, 64, 130, 700]
+    cache, vals, tab, table = make(gpu, D + HK + g, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared)
+    q, qd = queries(gpu, g, len(lens), 1, HK * g, D, strided=True)
+    o = cache.attend(q, tab, torch.tensor(lens, dtype=torch.int32, device=gpu), D ** -0.5)
+    check(o, op.attend(vals, qd, table, lens, D ** -0.5), D)
+    assert (o[0] == 0).all()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 1024])
+@pytest.mark.parametrize("S", [1, 2, 4, 16])
+def test_attend_pages_and_new_tokens(gpu, S, page):
+    """Pages smaller and larger than a tile, several new tokens (rows of one, two and four tiles, and
+    more than one group), lengths at and off the tiles' and granules' borders, a sink."""
+    lens = [S, 0, 1, 31, 32, 128, 129, 257, 1000]
+    HK, g, D = 2, 8, 64
+    cache, vals, tab, table = make(gpu, S + page, lens, HK=HK, D=D, page=page)
+    q, qd = queries(gpu, S, len(lens), S, HK * g, D, scale=1.5)
+    sink = torch.linspace(-3, 4, HK * g)
+    o = cache.attend(q, tab, torch.tensor(lens, dtype=torch.int32, device=gpu), D ** -0.5, attn_sink=sink.to(gpu))
+    check(o, op.attend(vals, qd, table, lens, D ** -0.5, sink.double().numpy()), D)
+
+
+@pytest.mark.parametrize("S,g,D,shared", [(1, 4, 128, False), (4, 8, 128, False), (3, 16, 256, False), (2, 64, 512, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_attend_long(gpu, S, g, D, shared, dtype):
+    """One long sequence over many workgroups, next to short ones."""
+    lens = [4099, 5, 900] if D < 512 else [1500, 40]
+    cache, vals, tab, table = make(gpu, S, lens, HK=1, D=D, page=64, dtype=dtype, shared=shared)
+    q, qd = queries(gpu, S, len(lens), S, g, D, scale=2.0)
+    o = cache.attend(q, tab, torch.tensor(lens, dtype=torch.int32, device=gpu), D ** -0.5)
+    check(o, op.attend(vals, qd, table, lens, D ** -0.5), D)
+
+
+def test_attend_running_maximum_moves(gpu):
+    """Rows that grow along the sequence, so that the maximum moves far at many tiles."""
+    lens, D = [900, 333], 128
+    cache, vals, tab, table = make(gpu, 5, lens, HK=1, D=D, page=32)
+    grow = torch.ones(cache.pages, 1, 32, 1)
+    for b, n in enumerate(lens):
+        for p in range(-(-n // 32)):
+            grow[table[b, p]] = 2.0 ** (p // 4)
+    k = (torch.from_numpy(vals["k"]) * grow).to(torch.bfloat16)
+    cache.k.copy_(torch.where(torch.isnan(cache.k.cpu()), cache.k.cpu(), k).to(gpu))
+    vals["k"] = k.double().numpy()
+    q, qd = queries(gpu, 6, 2, 1, 4, D)
+    o = cache.attend(q, tab, torch.tensor(lens, dtype=torch.int32, device=gpu), 0.3)
+    check(o, op.attend(vals, qd, table, lens, 0.3), D)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("page", [16, 64])
+def test_attend_missing_pages_and_long_lengths(gpu, page, dtype):
+    """Table entries below 0 and past the pool, at the start, inside and at the end; lengths beyond
+    the table; negative ones."""
+    lens = [page * 4, page * 4, page * 4 - 3, page * 2]
+    HK, D = 2, 128
+    cache, vals, tab, table = make(gpu, 9, lens, HK=HK, D=D, page=page, dtype=dtype)
+    table[0, 0], table[0, 2], table[1, 3], table[1, 1] = -1, cache.pages, 2 ** 31 - 1, -(2 ** 31)
+    table[3, :] = -1
+    asked = [page * 9, page * 4, page * 4 - 3, page * 2]
+    q, qd = queries(gpu, 3, 4, 2, HK * 2, D)
+    o = cache.attend(q, torch.from_numpy(table).to(gpu), torch.tensor(asked, dtype=torch.int32, device=gpu), D ** -0.5)
+    check(o, op.attend(vals, qd, table, asked, D ** -0.5), D)
+    assert (o[3] == 0).all()
+    o = cache.attend(q, tab, torch.tensor([-5, -1, 0, -2 ** 31], dtype=torch.int32, device=gpu), D ** -0.5)
+    assert (o == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_attend_row_takes_nothing_from_tokens_it_does_not_see(gpu, dtype):
+    """The newest tokens hold NaN (K of one, V of another): the rows before them stay finite."""
+    lens, S, HK, D = [200, 33], 4, 2, 64
+    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype)
+    q, qd = queries(gpu, 4, 2, S, 4, D)
+    ref = op.attend(vals, qd, table, lens, D ** -0.5)
+    for b, n in enumerate(lens):
+        for t, pool in ((n - 1, cache.k), (n - 2, cache.v)):
+            row = pool[table[b, t // 16], :, t % 16]
+            row.view(torch.uint8 if dtype == E4M3 else torch.int16).fill_(0x7F if dtype == E4M3 else 0x7FC0)
+    o = cache.attend(q, tab, torch.tensor(lens, dtype=torch.int32, device=gpu), D ** -0.5)
+    check(o[:, :2], tuple(x[:, :2] if i < 2 else x for i, x in enumerate(ref)), D)
+    assert torch.isnan(o[:, 2:]).all()
+
+
+def test_attend_infinite_values_and_scores(gpu):
+    """An infinite value reaches its column only, as the formula has it; a row whose every score is
+    -inf takes nothing; a NaN query row stays alone."""
+    lens, HK, D = [77], 1, 128
+    cache, vals, tab, table = make(gpu, 14, lens, HK=HK, D=D, page=32)
+    q, qd = queries(gpu, 5, 1, 1, 4, D)
+    cache.v[table[0, 2], 0, 76 % 32, 3] = float("inf")
+    vals["v"][table[0, 2], 0, 76 % 32, 3] = np.inf
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    o = cache.attend(q, tab, n, D ** -0.5)
+    assert torch.isposinf(o[..., 3]).all()
+    keep = [c for c in range(D) if c != 3]
+    ref = op.attend(vals, qd, table, lens, D ** -0.5)
+    check(o[..., keep], tuple(x[..., keep] if i < 2 else x for i, x in enumerate(ref)), D)
+    q2 = q.clone()
+    q2[0, 0, 1] = float("nan")
+    o2 = cache.attend(q2, tab, n, D ** -0.5)
+    assert torch.isnan(o2[0, 0, 1]).all()
+    for h in (0, 2, 3):
+        assert torch.equal(o2[0, 0, h], o[0, 0, h])
+    # every visible key far along one axis, the query against it: all scores -inf
+    cache.v.zero_()
+    cache.k.zero_()
+    cache.k[..., 0] = float("inf")
+    q3 = torch.zeros_like(q)
+    q3[..., 0] = -1.0
+    cache.v[...] = 1.0
+    assert (cache.attend(q3, tab, n, D ** -0.5) == 0).all()
+    q3[...] = -1.0
+    cache.k.fill_(float("inf"))
+    assert (cache.attend(q3, tab, n, D ** -0.5) == 0).all()
+    sink = torch.zeros(4, device=gpu)
+    assert (cache.attend(q3, tab, n, D ** -0.5, attn_sink=sink) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("S,HK,g,D,shared,page", [(1, 2, 4, 128, False, 16), (3, 2, 16, 64, False, 32), (1, 1, 64, 512, True, 64)])
+def test_accumulated_weights(gpu, S, HK, g, D, shared, page, dtype):
+    """Every slot's weight grows by what the rows of its head gave it, twice over; no other does."""
+    lens = [1, 0, 100, 517, 2]
+    cache, vals, tab, table = make(gpu, 21, lens, HK=HK, D=D, page=page, dtype=dtype, shared=shared, track=True)
+    q, qd = queries(gpu, 22, len(lens), S, HK * g, D, scale=1.5)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    sink = torch.linspace(-1, 2, HK * g)
+    for _ in range(2):
+        before = cache.weights.cpu().double().numpy()
+        o = cache.attend(q, tab, n, D ** -0.5, attn_sink=sink.to(gpu), accumulate=True)
+        ref = op.attend(vals, qd, table, lens, D ** -0.5, sink.double().numpy())
+        check(o, ref, D)
+        _, e32 = bounds(ref[0], ref[1], ref[3], D)
+        after = cache.weights.cpu().double().numpy()
+        assert (np.abs(after - before - ref[2]) <= e32 * ref[2] + 2.0 ** -23 * (np.abs(after) + 1e-30)).all()
+        assert (after[ref[2] == 0] == before[ref[2] == 0]).all()
+    first = cache.weights.clone()
+    cache.weights.zero_()
+    cache.attend(q, tab, n, D ** -0.5, accumulate=True)
+    again = cache.weights.clone()
+    cache.weights.zero_()
+    cache.attend(q, tab, n, D ** -0.5, accumulate=True)
+    assert torch.equal(again, cache.weights) and not torch.equal(first, again)
+
+
+def test_attend_pool_past_32_bits(gpu):
+    """Pages whose rows lie past 4 GiB of each pool."""
+    HK, D, page, P = 8, 128, 64, 36000
+    k = torch.empty(P, HK, page, D, dtype=torch.bfloat16, device=gpu)
+    v = torch.empty_like(k)
+    ids = torch.tensor([P - 1, 3, P - 2, 17000, P - 7], device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    small_k = torch.randn(5, HK, page, D, device=gpu, generator=g).to(torch.bfloat16)
+    small_v = torch.randn(5, HK, page, D, device=gpu, generator=g).to(torch.bfloat16)
+    k[ids], v[ids] = small_k, small_v
+    n = torch.tensor([5 * page - 9], dtype=torch.int32, device=gpu)
+    q, _ = queries(gpu, 2, 1, 1, 32, D)
+    o = PagedKV(k, v).attend(q, ids.to(torch.int32)[None], n, D ** -0.5)
+    few = torch.arange(5, dtype=torch.int32, device=gpu)[None]
+    assert torch.equal(o, PagedKV(small_k, small_v).attend(q, few, n, D ** -0.5))
+    new = torch.randn(1, 2, HK, D, device=gpu, generator=g).to(torch.bfloat16)
+    PagedKV(k, v).write(new, new, ids.to(torch.int32)[None], n)
+    assert torch.equal(k[P - 7, :, 55:57], new[0].transpose(0, 1)) and torch.equal(v[P - 7, :, 55:57], new[0].transpose(0, 1))
+    assert torch.equal(k[P - 7, :, :55], small_k[4, :, :55]) and torch.equal(k[P - 7, :, 57:], small_k[4, :, 57:])
+
+
+# ---------------------------------------------------------------- write -------
+
+
+def quantise(x):
+    s = x.float().abs().amax(-1).clamp(min=1e-4) * (1.0 / 448.0)
+    return (x.float() / s[..., None]).clamp(-448, 448).to(E4M3), s
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("HK,D,shared,page", [(2, 64, False, 16), (3, 128, False, 64), (1, 256, False, 32), (2, 128, True, 16),
+                                             (1, 256, True, 128), (1, 512, True, 64)])
+@pytest.mark.parametrize("S", [1, 37])
+def test_write(gpu, S, HK, D, shared, page, dtype):
+    """Rows land in their slots bit for bit (e4m3: codes and scales of the row), a padded batch's spare
+    rows and slots without a page are dropped, and no other slot changes."""
+    B, width = 6, 5
+    cache = PagedKV.empty(B * width + 2, page, HK, D, dtype=dtype, shared=shared, track=True, device=gpu)
+    rng = np.random.default_rng(S + D)
+    table = rng.permutation(cache.pages)[:B * width].reshape(B, width).astype(np.int32)
+    table[3, 1], table[4, 0] = -1, cache.pages
+    start = np.array([0, 5, page - 1, page - 3, 2, width * page - 2], dtype=np.int32)
+    count = np.array([S, max(0, S - 3), S, S, 0, S], dtype=np.int32)
+    position = np.array([0, 100, 7, 2 ** 30, 1, 50], dtype=np.int32)
+    g = torch.Generator().manual_seed(D)
+    rows = torch.randn(B, S, 2 * HK * D + 8, generator=g).to(torch.bfloat16)
+    rows[0, 0] = 0
+    rows[1, :, :3] = 3e38
+    dev = rows.to(gpu)
+    k, v = dev[..., :HK * D].view(B, S, HK, D), dev[..., HK * D:2 * HK * D].view(B, S, HK, D)
+    cache.weights.fill_(3.0)
+    cache.positions.fill_(-7)
+    to = lambda a: torch.from_numpy(a).to(gpu)  # noqa: E731
+    for use_count, use_pos in ((True, True), (False, False)):
+        want = {n: getattr(cache, n).cpu().clone() for n in ("k", "v", "k_scale", "v_scale", "weights", "positions")
+                if getattr(cache, n) is not None}
+        for b in range(B):
+            for i in range(int(count[b]) if use_count else S):
+                (pid, r), = op.slot_places(table[b], cache.pages, page, [int(start[b]) + i])
+                if pid < 0:
+                    continue
+                for name, x in (("k", rows[b, i, :HK * D]),) + (() if shared else (("v", rows[b, i, HK * D:2 * HK * D]),)):
+                    x = x.view(HK, D)
+                    if dtype == E4M3:
+                        code, s = quantise(x)
+                        want[name].view(torch.uint8)[pid, :, r] = code.view(torch.uint8)
+                        want[name + "_scale"][pid, :, r] = s
+                    else:
+                        want[name][pid, :, r] = x
+                want["weights"][pid, :, r] = 0.0
+                want["positions"][pid, :, r] = int(position[b] if use_pos else start[b]) + i
+        cache.write(k, None if shared else v, to(table), to(start), count=to(count) if use_count else None,
+                    position=to(position) if use_pos else None)
+        for name, x in want.items():
+            got = getattr(cache, name).cpu()
+            if dtype == E4M3 and name in ("k", "v"):
+                x, got = x.view(torch.uint8), got.view(torch.uint8)
+            assert torch.equal(got, x), name
+        start[:] = [9, 0, 1, 0, 3, 1]
+
+
+def test_write_unaligned_rows(gpu):
+    """Rows that do not begin on 16 bytes, and strides that are no multiple of eight."""
+    cache = PagedKV.empty(4, 16, 2, 64, device=gpu)
+    base = torch.randn(3 * (2 * 64 + 3) + 1, device=gpu).to(torch.bfloat16)[1:]
+    k = base.view(1, 3, 2 * 64 + 3)[..., :128].unflatten(-1, (2, 64))
+    table = torch.tensor([[2]], dtype=torch.int32, device=gpu)
+    cache.write(k, k, table, torch.tensor([4], dtype=torch.int32, device=gpu))
+    assert torch.equal(cache.k[2, :, 4:7], k[0].transpose(0, 1)) and torch.equal(cache.v[2, :, 4:7], k[0].transpose(0, 1))
+
+
+# ---------------------------------------------------------------- evict -------
+
+
+def arrays(cache):
+    return {n: (t.view(torch.uint8) if t.dtype == E4M3 else t.view(torch.int16) if t.dtype == torch.bfloat16 else
+                t.view(torch.int32) if n.endswith("_scale") else t).cpu().numpy().copy()
+            for n in ("k", "v", "k_scale", "v_scale", "weights", "positions") if (t := getattr(cache, n)) is not None}
+
+
+@pytest.mark.parametrize("dtype,HK,D,shared,page", [(torch.bfloat16, 2, 64, False, 16), (E4M3, 2, 128, False, 32),
+                                                   (torch.bfloat16, 1, 512, True, 64), (E4M3, 1, 256, True, 16)])
+@pytest.mark.parametrize("keep,first,recent", [(0, 0, 0), (1, 0, 1), (50, 4, 10), (64, 0, 0), (200, 200, 0), (1000, 3, 300),
+                                              (1000, 0, 1000)])
+def test_evict(gpu, dtype, HK, D, shared, page, keep, first, recent):
+    """The slots that stay, and where they lie, against the sorted order: ragged lengths around the budget,
+    many equal weights, infinities and NaN among them, positions in any order."""
+    lens = [0, 1, keep, keep + 1, keep + 7, 2 * keep + 3, 1300]
+    cache, _, tab, table = make(gpu, 3 + keep, lens, HK=HK, D=D, page=page, dtype=dtype, shared=shared, track=True)
+    g = torch.Generator().manual_seed(keep)
+    w = torch.randint(0, 6, cache.weights.shape, generator=g).float() / 4
+    w[torch.rand(w.shape, generator=g) < 0.05] = float("nan")
+    w[torch.rand(w.shape, generator=g) < 0.02] = float("inf")
+    w[torch.rand(w.shape, generator=g) < 0.02] = -0.0
+    w[torch.rand(w.shape, generator=g) < 0.02] = -1.5
+    cache.weights.copy_(w)
+    for b, n in enumerate(lens):  # a sequence's positions are its own tokens, in any order
+        for h in range(HK):
+            p = torch.randperm(n + 5, generator=g)[:n].to(torch.int32)
+            for t in range(n):
+                cache.positions[table[b, t // page], h, t % page] = int(p[t]) if n < 400 else 3 * t
+    want = arrays(cache)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    ref = op.evict(want, table, lens, keep, first, recent)
+    got = cache.evict(tab, n, keep, first=first, recent=recent)
+    assert np.array_equal(got.cpu().numpy(), ref) and n.tolist() == lens
+    for name, x in arrays(cache).items():
+        assert np.array_equal(x, want[name], equal_nan=name == "weights"), name
+
+
+def test_evict_in_place_and_missing_pages(gpu):
+    """lens as its own output; pages that the table lacks lose first and are not moved."""
+    lens, page, keep = [160, 90, 30], 16, 64
+    cache, _, tab, table = make(gpu, 31, lens, HK=2, D=64, page=page, track=True)
+    table[0, 1], table[0, 9], table[1, 2] = -1, cache.pages + 5, -3
+    want = arrays(cache)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    ref = op.evict(want, table, lens, keep, 2, 8)
+    out = cache.evict(torch.from_numpy(table).to(gpu), n, keep, first=2, recent=8, out=n)
+    assert out is n and np.array_equal(n.cpu().numpy(), ref)
+    for name, x in arrays(cache).items():
+        assert np.array_equal(x, want[name]), name
+
+
+@pytest.mark.parametrize("n,keep", [(5000, 4096), (20000, 1500), (70001, 8192)])
+def test_evict_long(gpu, n, keep):
+    """Lengths of many rounds of a workgroup, against torch's stable sort."""
+    page, HK = 64, 2
+    cache = PagedKV.empty(-(-n // page) + 1, page, HK, 64, track=True, device=gpu)
+    g = torch.Generator().manual_seed(n)
+    table = torch.randperm(cache.pages, generator=g)[:-(-n // page)].to(torch.int32)[None].to(gpu)
+    cache.weights.copy_(torch.randn(cache.weights.shape, generator=g).mul(8).round().div(8).exp())
+    slot = torch.arange(table.shape[1] * page, dtype=torch.int32, device=gpu).view(-1, page)
+    cache.positions[table[0].long()] = slot[:, None, :].expand(-1, HK, page).contiguous()
+    cache.k[..., 0] = cache.positions.to(torch.bfloat16)
+    cache.k.view(torch.int16)[..., 1] = (cache.positions & 0x7FFF).to(torch.int16)
+    flat = lambda x: x[table[0].long()].transpose(0, 1).reshape(HK, -1)  # noqa: E731
+    w, p = flat(cache.weights), flat(cache.positions)
+    first, recent = 4, 512
+    safe = (p < first) | (p >= n - recent)
+    key = torch.where(safe, torch.tensor(float("inf"), device=gpu), w)
+    key[:, n:] = -1
+    order = torch.sort(key, dim=1, descending=True, stable=True).indices
+    kept = torch.zeros_like(safe).scatter_(1, order[:, :keep], True)
+    out = cache.evict(table, torch.tensor([n], dtype=torch.int32, device=gpu), keep, first=first, recent=recent)
+    assert out.tolist() == [keep]
+    after = flat(cache.positions)
+    for h in range(HK):
+        want = torch.arange(table.shape[1] * page, dtype=torch.int32, device=gpu)
+        holes, movers = torch.nonzero(~kept[h, :keep])[:, 0], torch.nonzero(kept[h, keep:])[:, 0] + keep
+        want[holes] = movers.to(torch.int32)
+        assert torch.equal(after[h], want)
+    assert torch.equal(flat(cache.weights), torch.gather(w, 1, after.long()))
+    low = cache.k.view(torch.int16)[..., 1]
+    assert torch.equal(flat(low), (after & 0x7FFF).to(torch.int16))
+
+
+# ---------------------------------------------------------------- together ----
+
+
+@pytest.mark.parametrize("dtype,S", [(torch.bfloat16, 1), (E4M3, 3)])
+def test_decode_under_a_budget(gpu, dtype, S):
+    """A prompt's write, then steps of write, attend and evict as a serving loop makes them, against
+    a cache that the plain statements keep (its choice of what stays is made from the same weights)."""
+    B, HK, g, D, page, keep = 3, 2, 4, 64, 16, 48
+    width = 6
+    cache = PagedKV.empty(B * width, page, HK, D, dtype=dtype, track=True, device=gpu)
+    rng = np.random.default_rng(1)
+    table = rng.permutation(B * width).reshape(B, width).astype(np.int32)
+    tab = torch.from_numpy(table).to(gpu)
+    plain = {"k": np.zeros((B * width, HK, page, D)), "v": np.zeros((B * width, HK, page, D)),
+             "weights": np.zeros((B * width, HK, page)), "positions": np.zeros((B * width, HK, page), dtype=np.int64)}
+    gen = torch.Generator().manual_seed(2)
+    lens, pos = np.zeros(B, dtype=np.int32), np.zeros(B, dtype=np.int32)
+    n = torch.zeros(B, dtype=torch.int32, device=gpu)
+    p = torch.zeros(B, dtype=torch.int32, device=gpu)
+    for step in range(14):
+        s = 30 if step == 0 else S
+        count = np.array([30, 7, 0], dtype=np.int32) if step == 0 else np.full(B, s, dtype=np.int32)
+        k = torch.randn(B, s, HK, D, generator=gen).to(torch.bfloat16)
+        v = torch.randn(B, s, HK, D, generator=gen).to(torch.bfloat16)
+        c = torch.from_numpy(count).to(gpu)
+        cache.write(k.to(gpu), v.to(gpu), tab, n, count=c, position=p)
+        for b in range(B):
+            for i in range(count[b]):
+                (pid, r), = op.slot_places(table[b], B * width, page, [int(lens[b]) + i])
+                for name, x in (("k", k), ("v", v)):
+                    x = x[b, i]
+                    if dtype == E4M3:
+                        code, sc = quantise(x)
+                        x = code.double() * sc.double()[:, None]
+                    plain[name][pid, :, r] = x.double().numpy()
+                plain["weights"][pid, :, r], plain["positions"][pid, :, r] = 0.0, pos[b] + i
+        lens, pos = lens + count, pos + count
+        n, p = n + c, p + c
+        if step == 0:
+            continue
+        q, qd = queries(gpu, step, B, S, HK * g, D, scale=2.0)
+        o = cache.attend(q, tab, n, D ** -0.5, accumulate=True)
+        ref = op.attend(plain, qd, table, lens, D ** -0.5)
+        check(o, ref, D)
+        plain["weights"] += ref[2]
+        got = cache.weights.cpu().numpy()
+        assert np.abs(got - plain["weights"]).max() < 1e-4
+        plain["weights"] = got.astype(np.float64)  # what stays is chosen from the cache's own sums
+        n = cache.evict(tab, n, keep, first=2, recent=8)
+        lens = op.evict(plain, table, lens, keep, 2, 8)
+        assert np.array_equal(n.cpu().numpy(), lens)
+        assert np.array_equal(cache.positions.cpu().numpy(), plain["positions"])
+
+
+def test_captured_loop_replays(gpu):
+    """Write, attend and evict captured as one graph and replayed, with eager work on the same cache and
+    other streams between the replays: every replay equals the eager result."""
+    HK, g, D, page, keep = 2, 4, 128, 16, 96
+    lens = [96, 50, 0]
+    cache, _, tab, _ = make(gpu, 41, lens, HK=HK, D=D, page=page, track=True, width=8, spare=40)
+    tab = torch.arange(24, dtype=torch.int32, device=gpu).view(3, 8)
+    for t in (cache.k, cache.v):
+        t.copy_(torch.randn(t.shape, device=gpu))
+    q, _ = queries(gpu, 1, 3, 1, HK * g, D)
+    k = torch.randn(3, 1, HK, D, device=gpu).to(torch.bfloat16)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    start = torch.empty_like(n)
+
+    def step():
+        cache.write(k, k, tab, n, position=p)
+        m = n + 1
+        o = cache.attend(q, tab, m, D ** -0.5, accumulate=True)
+        n.copy_(cache.evict(tab, m, keep, first=2, recent=4))
+        p.add_(1)
+        return o
+
+    held = (cache.k, cache.v, cache.weights, cache.positions, n)
+    p = n.clone()
+    held += (p,)
+    saved = [t.clone() for t in held]
+    want = []
+    for i in range(5):
+        k.fill_(0.1 * i)
+        want.append((step().clone(), *[t.clone() for t in held]))
+    for t, x in zip(held, saved):
+        t.copy_(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = step()
+    for t, x in zip(held, saved):
+        t.copy_(x)
+    other = torch.cuda.Stream()
+    for i in range(5):
+        k.fill_(0.1 * i)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, x in zip((o, *held), want[i]):
+            assert torch.equal(a, x)
+        with torch.cuda.stream(other):  # eager work of the same kind between the replays
+            e = cache.attend(q, tab, n, D ** -0.5)
+        torch.cuda.synchronize()
+        assert torch.equal(e, cache.attend(q, tab, n, D ** -0.5))
+
+
+def test_two_streams_at_once(gpu):
+    """Two calls in flight on two streams, each with its own workspace."""
+    HK, D = 4, 128
+    cache, vals, tab, table = make(gpu, 51, [3000, 2000, 900], HK=HK, D=D, page=64)
+    n = torch.tensor([3000, 2000, 900], dtype=torch.int32, device=gpu)
+    q1, _ = queries(gpu, 1, 3, 1, 16, D)
+    q2, _ = queries(gpu, 2, 3, 1, 16, D)
+    a, b = cache.attend(q1, tab, n, D ** -0.5), cache.attend(q2, tab, n, D ** -0.5)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        with torch.cuda.stream(s1):
+            x = cache.attend(q1, tab, n, D ** -0.5)
+        with torch.cuda.stream(s2):
+            y = cache.attend(q2, tab, n, D ** -0.5)
+        torch.cuda.synchronize()
+        assert torch.equal(x, a) and torch.equal(y, b)
+
+
+def test_workspace_and_outputs_of_the_caller(gpu):
+    """A given workspace and out are used; two graphs that share a workspace replay one after the other."""
+    HK, D = 2, 128
+    cache, _, tab, _ = make(gpu, 61, [700, 45], HK=HK, D=D, page=32, track=True)
+    n = torch.tensor([700, 45], dtype=torch.int32, device=gpu)
+    q, _ = queries(gpu, 1, 2, 1, 8, D)
+    want = cache.attend(q, tab, n, D ** -0.5)
+    ws = torch.empty(cache.attend_workspace_bytes(2, 1, 8, tab.shape[1]), dtype=torch.uint8, device=gpu)
+    out = torch.empty_like(want)
+    assert cache.attend(q, tab, n, D ** -0.5, out=out, workspace=ws) is out and torch.equal(out, want)
+    q2 = q.flip(2).contiguous()
+    want2 = cache.attend(q2, tab, n, D ** -0.5)
+    graphs, outs = [], []
+    for x in (q, q2):
+        graphs.append(torch.cuda.CUDAGraph())
+        outs.append(torch.empty_like(out))
+        with torch.cuda.graph(graphs[-1]):
+            cache.attend(x, tab, n, D ** -0.5, out=outs[-1], workspace=ws)
+    for _ in range(3):
+        for t in outs:
+            t.zero_()
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)

@@ -59,6 +59,11 @@ SIGNATURES = {
     "wz_fp8_wire_pack": (_I, [_P, _P, _P, _I64, _I64, _P]),
     "wz_sparse_attn_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "wz_sparse_attn": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P, _I64, _P]),
+    "wz_paged_kv_write": (_I, [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _I64, _P]),
+    "wz_paged_attn_workspace_bytes": (_I64, [_P, _I64, _I64, _I64, _I64, _I]),
+    "wz_paged_attn": (_I, [_P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _F, _I, _P, _I64, _P]),
+    "wz_paged_evict_workspace_bytes": (_I64, [_P, _I64, _I64, _I64]),
+    "wz_paged_evict": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P]),
     "wz_fp8_wire_unpack": (_I, [_P, _P, _P, _I64, _I64, _P]),
     "wz_synth_fill": (_I, [_P, _I64, ctypes.c_uint64, _I64, _I, ctypes.c_double, ctypes.c_double, _P]),
     "wz_prof_begin": (_I, [_I]),
@@ -72,6 +77,8 @@ WZ_SCALE_UE8M0 = 1
 WZ_SCALE_UE8M0_F32 = 2
 WZ_WSCALE_F32 = 0
 WZ_WSCALE_E8M0 = 1
+WZ_KV_BF16 = 0
+WZ_KV_E4M3 = 1
 WZ_SCORE_SOFTMAX = 0
 WZ_SCORE_SIGMOID = 1
 WZ_SCORE_SQRTSOFTPLUS = 2

@@ -1,0 +1,685 @@
+// Attention of a few new tokens over a paged cache: the kernel, compiled for bf16 and e4m3
+// rows by the two sources that include it.
+//
+// One KV head's rows of queries (the S tokens' heads that share it, R = S H / kv_heads of them)
+// are taken in groups of 16 RT; a group of a sequence is a unit, and its n cached tokens are
+// `granules` of 32 NW.  All units' granules in a row are cut into one equal share per workgroup, so
+// the chip is filled whatever the lengths: a unit inside one share is finished there, a cut one
+// leaves (m, l, O) partials that paged_attn_join_kernel merges.  A workgroup's share holds at most
+// two cut units, its first and its last, which own its partial slots 2w and 2w + 1.
+//
+// Inside a share every wave works by itself on each NW-th tile of 32 tokens, with its own ring of
+// NS tiles in LDS that the loads fill directly (no registers, no barriers):
+//   * S^T = K Q^T and O^T += V^T P^T with V_MFMA_F32_16X16X32; lane (row n, group g) of S^T
+//     holds tokens 4g + i and 16 + 4g + i, which are the k slots of its P operand, so P never
+//     leaves the lane and the softmax statistics are one register a row tile;
+//   * y = q . k scale log2(e), p = 2^(y - m), m moved only when a tile's maximum exceeds it by more
+//     than 8 (the final quotient does not depend on m); p is rounded to bf16 for the product with V
+//     (the sums keep it in 32 bits), which adds as much error as the output's own rounding;
+//   * the waves' (m, l, O) meet in LDS when the unit's part is done.
+// Reading the cache bounds it: 4 R / element-size flops a byte is far below the matrix units' rate
+// for the usual group sizes.
+#pragma once
+
+#include <algorithm>
+
+#include "paged.h"
+
+namespace wz {
+
+typedef short pv4s __attribute__((ext_vector_type(4)));
+typedef short pv8s __attribute__((ext_vector_type(8)));
+typedef __bf16 pv8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 pv2bf __attribute__((ext_vector_type(2)));
+typedef int pv2i __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) pv4s lds_pv4s;
+typedef __attribute__((address_space(3))) pv2i lds_pv2i;
+
+constexpr int kPagedTile = 32;           // tokens of a wave's tile
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kPagedLazy = 8.0f;       // the running maximum moves when a tile exceeds it by more
+constexpr int kPagedMaxS = 16;
+
+struct PagedAttnArgs {
+  PagedView c;
+  const uint16_t* q;
+  int64_t qb, qs, qh;  // elements between sequences, tokens, heads
+  const float* sink;
+  const int32_t* table;
+  const int32_t* lens;
+  uint16_t* o;
+  float* part;    // 2 W slots of (m, l)[16 RT] and O[16 RT][D]
+  float* ml;      // accumulate: per unit and row the final maximum and 1 / sum
+  float* scores;  // accumulate: y [B, heads, R, capacity]
+  int width, B, S, H, W;
+  int64_t capacity;  // slots of the table, width * page
+  float scale2;      // softmax scale * log2(e)
+};
+
+// Tokens of a sequence, and its granules.
+__device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
+  return int(min(int64_t(max(a.lens[b], 0)), a.capacity));
+}
+
+// Where the units' granules begin: upb units a sequence, each of ceil(n / G).  Every lane of a wave
+// gets the result; B sequences are summed 64 at a time.
+template <int G>
+__device__ __forceinline__ int64_t paged_total(const PagedAttnArgs& a, int upb) {
+  const int lane = threadIdx.x & 63;
+  int64_t sum = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int g = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
+    for (int o = 1; o < 64; o <<= 1) g += __shfl_xor(g, o, 64);
+    sum += g;
+  }
+  return sum * upb;
+}
+
+// The sequence that holds granule x (0 <= x < total) and the granules before it.
+template <int G>
+__device__ __forceinline__ void paged_find(const PagedAttnArgs& a, int upb, int64_t x, int* seq, int64_t* before) {
+  const int lane = threadIdx.x & 63;
+  int64_t sum = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int g = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
+    int inc = g;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += y;
+    }
+    const int64_t end = (sum + inc) * upb;  // granules up to and with this lane's sequence
+    const uint64_t past = __ballot(end > x);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      *seq = b0 + l;
+      *before = (sum + __shfl(inc - g, l, 64)) * upb;
+      return;
+    }
+    sum += __shfl(inc, 63, 64);
+  }
+  *seq = a.B - 1;  // not reached: x < total
+  *before = sum * upb;
+}
+
+// Workgroups with a share (one granule at least each), the first granule of workgroup w's, and the
+// workgroup that holds granule x.
+__device__ __forceinline__ int paged_workers(int64_t total, int W) { return int(min(total, int64_t(W))); }
+__device__ __forceinline__ int64_t paged_share(int64_t total, int W, int w) { return total * w / W; }
+__device__ __forceinline__ int paged_owner(int64_t total, int W, int64_t x) { return int(((x + 1) * W - 1) / total); }
+
+// LDS image of a tile: rows of RB bytes, 16-byte chunk c of row r at slot c ^ swz(r).  The
+// fragments' 16-byte reads of one chunk of 16 rows are served in passes that mix rows 0-3 and 12-15
+// with rows 4-11 of the neighbouring chunk; the transpose reads take two adjacent chunks of 8 rows.
+template <int RB>
+struct PagedRow {
+  static constexpr int CH = RB / 16;     // chunks a row
+  static constexpr int RPI = 1024 / RB;  // rows a load
+  static __device__ __forceinline__ int swz(int row) {
+    const int hi = (row >> 3) & 1;
+    if constexpr (RB >= 256) return ((row ^ (hi << 2)) & 7) << 1 | hi;
+    if constexpr (RB == 128) return ((((row >> 1) & 3) ^ (hi << 1)) << 1) | hi;
+    const int q = (row >> 2) & 3;
+    return (q << 1 ^ 3 * (q >> 1)) & 3;  // 0, 2, 3, 1
+  }
+};
+
+// 1 KB straight into LDS, 16 bytes a lane, from a wave-uniform base and a lane's offset.  The
+// compiler does not look into the block for hazards, so it waits itself for what the hardware does
+// not check: an SGPR that a vector instruction wrote (a readlane) is readable by a load after five
+// states, m0 after one.
+__device__ __forceinline__ int64_t paged_uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(x)), hi = __builtin_amdgcn_readfirstlane(uint32_t(x >> 32));
+  return int64_t(uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ void paged_load16(const uint8_t* base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(voff), "s"(base) : "memory", "m0");
+}
+// 4 bytes a lane.
+__device__ __forceinline__ void paged_load4(const float* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(p) : "memory", "m0");
+}
+
+__device__ __forceinline__ v4f paged_mfma(pv8s a, pv8s b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pv8bf, a), __builtin_bit_cast(pv8bf, b), c, 0, 0, 0);
+}
+
+// 8 e4m3 codes as bf16 (exact).
+__device__ __forceinline__ pv8s paged_widen(int lo, int hi) {
+  union {
+    pv2bf p[4];
+    pv8s v;
+  } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return u.v;
+}
+
+// Sizes of one compiled kernel.
+template <int D, bool FP8, bool SHARED, int RT>
+struct PagedCfg {
+  static constexpr int ESZ = FP8 ? 1 : 2;
+  static constexpr int RB = D * ESZ;
+  static constexpr int TILE = kPagedTile * RB;                    // one side of a tile
+  static constexpr int STAGE = TILE * (SHARED ? 1 : 2);
+  static constexpr int SCALES = FP8 ? 256 : 0;                    // a tile's K and V scales
+  static constexpr int NW = STAGE >= 32768 ? 2 : 4;               // waves
+  static constexpr int WAVE = NW == 2 ? 65536 : 32768;            // ring bytes a wave
+  static constexpr int NS = WAVE / STAGE > 4 ? 4 : WAVE / STAGE;  // tiles in the ring
+  static constexpr int LOADS = STAGE / 1024 + (FP8 ? 1 : 0);      // loads a tile
+  static constexpr int G = kPagedTile * NW;                       // tokens of a granule
+  static constexpr int ROWS = 16 * RT;
+  static constexpr int MERGE = ROWS * D * 4;                      // a wave's O in LDS
+  static constexpr int RING = NS * (STAGE + SCALES) > MERGE ? NS * (STAGE + SCALES) : MERGE;
+  static constexpr int SMALL = NW * ROWS * 8 + NW * NS * 4;       // (m, l) of the waves, valid masks
+  static constexpr int LDS = NW * RING + SMALL;
+  static constexpr int64_t SLOT = int64_t(ROWS) * (D + 2);        // floats of a partial
+  static_assert(NS >= 2 && (NS - 1) * LOADS < 64, "the waits count the loads in flight");
+};
+
+template <int D, bool FP8, bool SHARED, int RT>
+__global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void paged_attn_kernel(PagedAttnArgs a) {
+  using C = PagedCfg<D, FP8, SHARED, RT>;
+  using L = PagedRow<C::RB>;
+  constexpr int NW = C::NW, NS = C::NS, RB = C::RB, ROWS = C::ROWS;
+  constexpr int KC = D / 32, NT = D / 16;
+  extern __shared__ __align__(1024) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nl = lane & 15, g = lane >> 4;
+  uint8_t* const ring = lds + wave * C::RING;
+  uint8_t* const scales = ring + NS * C::STAGE;  // e4m3: 256 bytes a tile
+  float* const s_m = reinterpret_cast<float*>(lds + NW * C::RING);  // [wave][row]
+  float* const s_l = s_m + NW * ROWS;
+  uint32_t* const s_valid = reinterpret_cast<uint32_t*>(s_l + NW * ROWS) + wave * NS;
+  const uint32_t ring_lds = lds_addr(ring), scales_lds = lds_addr(scales);
+
+  const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
+  const int w = blockIdx.x;
+  const int64_t total = paged_uniform(paged_total<C::G>(a, upb));
+  const int W = paged_workers(total, a.W);
+  if (w >= W) return;
+  int64_t x = paged_uniform(paged_share(total, W, w));
+  const int64_t x_end = paged_uniform(paged_share(total, W, w + 1));
+  int b;
+  int64_t before;
+  paged_find<C::G>(a, upb, x, &b, &before);
+  b = __builtin_amdgcn_readfirstlane(b);
+  before = paged_uniform(before);
+  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+  const int ps = a.c.shift, page = a.c.page;
+  const int ish = page >= kPagedTile ? 0 : 1;  // page ids a tile: 1 or 2
+
+  for (bool first_piece = true; x < x_end; first_piece = false) {
+    int gran = (n + C::G - 1) / C::G;
+    while (x >= before + int64_t(gran) * upb) {  // the next sequence that holds anything
+      before += int64_t(gran) * upb;
+      ++b;
+      n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+      gran = (n + C::G - 1) / C::G;
+    }
+    const int u = __builtin_amdgcn_readfirstlane(int((x - before) / gran));  // unit of the sequence
+    const int64_t ubeg = before + int64_t(u) * gran;
+    const int g0 = int(x - ubeg), g1 = int(min(x_end - ubeg, int64_t(gran)));
+    const bool whole = g0 == 0 && g1 == gran;
+    const int hk = __builtin_amdgcn_readfirstlane(u / RG), rg = u - hk * RG;
+    const int t0 = g0 * C::G, t1 = min(g1 * C::G, n);
+    // the last S - 1 tokens are seen by some rows only: they are added one by one below
+    const int tm = min(t1, max(n - a.S + 1, t0));
+    const int32_t* const trow = a.table + int64_t(b) * a.width;
+
+    // Q fragments: lane (row nl, group g); e4m3 rows are read 16 codes at a time, so there the
+    // chunks 2p and 2p + 1 hold d 64p + 16g .. +8 and +8 .. +16
+    pv8s qf[RT][KC];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = min(rg * ROWS + 16 * rt + nl, R - 1);
+      const uint16_t* const qrow = a.q + b * a.qb + (r / grp) * a.qs + (hk * grp + r % grp) * a.qh;
+#pragma unroll
+      for (int cc = 0; cc < KC; ++cc) {
+        const int d = FP8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g;
+        qf[rt][cc] = *reinterpret_cast<const pv8s*>(qrow + d);
+      }
+    }
+    v4f acc[RT][NT];  // acc[rt][nt][i] = O[row 16rt + nl][16nt + 4g + i]
+    float m_run[RT], l_run[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m_run[rt] = -INFINITY;
+      l_run[rt] = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[rt][nt] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- this wave's tiles: t0 + 32 (wave + NW k), k < nk ----
+    const int ntile = (tm - t0 + kPagedTile - 1) / kPagedTile;
+    const int nk = max(0, (ntile - wave + NW - 1) / NW);
+    // page ids of the next 64 >> ish tiles, lane e: tile base + (e >> ish), part e & ish
+    int ids = -1, ids_base = 0;
+    auto fetch_ids = [&](int k0) {
+      ids_base = k0;
+      const int k = k0 + (lane >> ish);
+      const int t = t0 + kPagedTile * (wave + NW * k) + ((lane & ish) << 4);
+      int id = -1;
+      if (k < nk && t < tm) id = trow[t >> ps];
+      ids = uint32_t(id) < uint32_t(a.c.pages) ? id : -1;
+    };
+    auto issue = [&](int k, int stage) {
+      if (((k - ids_base) << ish) >= 64) fetch_ids(k);
+      const int t = t0 + kPagedTile * (wave + NW * k);
+      const int e = (k - ids_base) << ish;
+      int id[2];
+      id[0] = __builtin_amdgcn_readlane(ids, e);
+      id[1] = ish ? __builtin_amdgcn_readlane(ids, e + 1) : id[0];
+      uint32_t valid = tm - t >= 32 ? 0xFFFFFFFFu : (1u << (tm - t)) - 1u;
+      if (id[0] < 0) valid &= ish ? 0xFFFF0000u : 0u;
+      if (id[1] < 0) valid &= ish ? 0x0000FFFFu : 0u;
+      if (lane == 0) s_valid[stage] = valid;
+      const int off = ish ? 0 : t & (page - 1);
+      int64_t row[2];  // of the tile's halves
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        row[i] = (int64_t(max(id[i], 0)) * a.c.heads + hk) * page + off + (ish ? 0 : 16 * i);
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(ring_lds + stage * C::STAGE);
+      const int rin = lane / L::CH, slot = lane % L::CH;
+#pragma unroll
+      for (int side = 0; side < (SHARED ? 1 : 2); ++side) {
+        const uint8_t* const pool = side ? a.c.v : a.c.k;
+#pragma unroll
+        for (int j = 0; j < kPagedTile / L::RPI; ++j) {
+          constexpr int HALF = 16 / L::RPI > 0 ? 16 / L::RPI : 1;  // loads of half a tile
+          const int half = j / HALF, r = (j % HALF) * L::RPI;
+          const uint32_t voff = uint32_t(rin * RB + ((slot ^ L::swz(r + rin)) << 4));
+          paged_load16(pool + (row[half] + r) * RB, voff, dst + side * C::TILE + j * 1024);
+        }
+      }
+      if constexpr (FP8) {
+        const int tok = lane & 31;
+        const int64_t at = tok < 16 ? row[0] + tok : row[1] + tok - 16;
+        paged_load4((lane < 32 ? a.c.ks : a.c.vs) + at,
+                    __builtin_amdgcn_readfirstlane(scales_lds + stage * C::SCALES));
+      }
+    };
+    if (nk > 0) fetch_ids(0);
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // Q too: no wait for it is left inside the loop
+#pragma unroll
+    for (int k = 0; k < NS - 1; ++k)
+      if (k < nk) issue(k, k);
+
+    int stage = 0;
+#pragma unroll 1
+    for (int k = 0; k < nk; ++k) {
+      if (k + NS - 1 < nk) {
+        __builtin_amdgcn_s_waitcnt(lgkmcnt_only(0));  // the tile before has been read out of its stage
+        issue(k + NS - 1, stage == 0 ? NS - 1 : stage - 1);
+        __builtin_amdgcn_s_waitcnt(vmcnt_only((NS - 1) * C::LOADS));
+      } else {
+        __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+      }
+      asm volatile("" ::: "memory");
+      uint8_t* const kt = ring + stage * C::STAGE;
+      uint8_t* const vt = SHARED ? kt : kt + C::TILE;
+      const uint32_t valid = __builtin_amdgcn_readfirstlane(s_valid[stage]);
+      if (valid != 0xFFFFFFFFu) {
+        // rows that hold nothing become zeros, whatever bits their memory has
+        for (int i = lane; i < kPagedTile * L::CH; i += 64)
+          if (!((valid >> (i / L::CH)) & 1)) {
+            *reinterpret_cast<v4i*>(kt + i * 16) = v4i{0, 0, 0, 0};
+            if (!SHARED) *reinterpret_cast<v4i*>(vt + i * 16) = v4i{0, 0, 0, 0};
+          }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      // ---- S^T: sacc[rt][tt][i] = q . k of row nl, token 16tt + 4g + i ----
+      v4f sacc[RT][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sacc[rt][0] = sacc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const uint8_t* const krow = kt + (16 * tt + nl) * RB;
+        const int sw = L::swz(nl);
+        if constexpr (!FP8) {
+#pragma unroll
+          for (int cc = 0; cc < KC; ++cc) {
+            const pv8s kf = *reinterpret_cast<const pv8s*>(krow + (((4 * cc + g) ^ sw) << 4));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) sacc[rt][tt] = paged_mfma(kf, qf[rt][cc], sacc[rt][tt]);
+          }
+        } else {
+#pragma unroll
+          for (int cp = 0; cp < KC / 2; ++cp) {
+            const v4i kc = *reinterpret_cast<const v4i*>(krow + (((4 * cp + g) ^ sw) << 4));
+            const pv8s k0 = paged_widen(kc[0], kc[1]), k1 = paged_widen(kc[2], kc[3]);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              sacc[rt][tt] = paged_mfma(k0, qf[rt][2 * cp], sacc[rt][tt]);
+              sacc[rt][tt] = paged_mfma(k1, qf[rt][2 * cp + 1], sacc[rt][tt]);
+            }
+          }
+        }
+      }
+      v4f ksc[2], vsc[2];
+      if constexpr (FP8) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          ksc[tt] = *reinterpret_cast<const v4f*>(scales + stage * C::SCALES + 4 * (16 * tt + 4 * g));
+          vsc[tt] = *reinterpret_cast<const v4f*>(scales + stage * C::SCALES + 128 + 4 * (16 * tt + 4 * g));
+        }
+      }
+      // ---- softmax ----
+      pv8s pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float y[8], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = sacc[rt][i >> 2][i & 3] * a.scale2;
+          if constexpr (FP8) y[i] = sacc[rt][i >> 2][i & 3] * ksc[i >> 2][i & 3] * a.scale2;
+        }
+        if (valid != 0xFFFFFFFFu) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (!((valid >> (16 * (i >> 2) + 4 * g + (i & 3))) & 1)) y[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, y[i]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (a.scores) {
+          const int r = rg * ROWS + 16 * rt + nl, t = t0 + kPagedTile * (wave + NW * k) + 4 * g;
+          if (r < R) {
+            float* const row = a.scores + ((int64_t(b) * a.c.heads + hk) * R + r) * a.capacity;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+              if (t + 16 * tt + 3 < tm) {
+                *reinterpret_cast<v4f*>(row + t + 16 * tt) = v4f{y[4 * tt], y[4 * tt + 1], y[4 * tt + 2], y[4 * tt + 3]};
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (t + 16 * tt + i < tm) row[t + 16 * tt + i] = y[4 * tt + i];
+              }
+            }
+          }
+        }
+        const bool bump = top > m_run[rt] + kPagedLazy;
+        if (__ballot(bump)) {
+          const float resc = !bump ? 1.0f : (m_run[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[rt] - top));
+          m_run[rt] = bump ? top : m_run[rt];
+          l_run[rt] *= resc;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[rt][nt] = acc[rt][nt] * resc;
+        }
+        const float m = m_run[rt] == -INFINITY ? 0.0f : m_run[rt];
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(y[i] - m);
+        l_run[rt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        if constexpr (FP8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] *= vsc[i >> 2][i & 3];
+          if (valid != 0xFFFFFFFFu) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (!((valid >> (16 * (i >> 2) + 4 * g + (i & 3))) & 1)) p[i] = 0.0f;
+          }
+        }
+        union {
+          uint32_t d[4];
+          pv8s v;
+        } pk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pk.d[i] = f32x2_to_bf16x2(p[2 * i], p[2 * i + 1]);
+        pf[rt] = pk.v;
+      }
+      // ---- O^T += V^T P^T: k slots 0-3 tokens 4g + i, 4-7 tokens 16 + 4g + i ----
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        pv8s vf;
+        if constexpr (!FP8) {
+          const int row = 4 * g + (nl >> 2);
+          const uint8_t* const p = vt + row * RB + (((2 * nt + ((nl >> 1) & 1)) ^ L::swz(row)) << 4) + (nl & 1) * 8;
+          const pv4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_pv4s*)p);
+          const pv4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_pv4s*)(p + 16 * RB));
+          vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          const int row = 4 * g + ((nl >> 1) & 3) + 16 * (nl >> 3);
+          const uint8_t* const p = vt + row * RB + ((nt ^ L::swz(row)) << 4) + (nl & 1) * 8;
+          const pv2i c8 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_pv2i*)p);
+          vf = paged_widen(c8[0], c8[1]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][nt] = paged_mfma(vf, pf[rt], acc[rt][nt]);
+      }
+      stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+
+    // ---- the tokens that only some rows see, by the first wave: a row takes nothing, not even a
+    // NaN, from a token it does not see ----
+    if (wave == 0) {
+      for (int t = tm; t < t1; ++t) {
+        const int64_t at = paged_row(a.c, trow, a.width, hk, t);
+        if (at < 0) continue;
+        const uint8_t* const kr = a.c.k + at * RB;
+        const uint8_t* const vr = (SHARED ? a.c.k : a.c.v) + at * RB;
+        const float ksc = FP8 ? a.c.ks[at] : 1.0f, vsc = FP8 ? a.c.vs[at] : 1.0f;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float dot = 0.0f;
+#pragma unroll
+          for (int cc = 0; cc < KC; ++cc) {
+            pv8s kf;
+            if constexpr (!FP8) {
+              kf = *reinterpret_cast<const pv8s*>(kr + (32 * cc + 8 * g) * 2);
+            } else {
+              const pv2i c8 = *reinterpret_cast<const pv2i*>(kr + 64 * (cc >> 1) + 16 * g + 8 * (cc & 1));
+              kf = paged_widen(c8[0], c8[1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dot = fmaf(bf16_to_f32(uint16_t(kf[i])), bf16_to_f32(uint16_t(qf[rt][cc][i])), dot);
+          }
+          dot += __shfl_xor(dot, 16, 64);
+          dot += __shfl_xor(dot, 32, 64);
+          const int r = rg * ROWS + 16 * rt + nl;
+          const bool sees = r < R && t < n - (a.S - 1 - r / grp);
+          const float y = FP8 ? dot * ksc * a.scale2 : dot * a.scale2;
+          if (a.scores && r < R && g == 0)
+            a.scores[((int64_t(b) * a.c.heads + hk) * R + r) * a.capacity + t] = y;
+          if (sees) {
+            const float m_new = fmaxf(m_run[rt], y);
+            const float m = m_new == -INFINITY ? 0.0f : m_new;
+            const float resc = m_run[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[rt] - m);
+            const float p = __builtin_amdgcn_exp2f(y - m);
+            m_run[rt] = m_new;
+            l_run[rt] = l_run[rt] * resc + (g == 0 ? p : 0.0f);
+            const float pv = p * vsc;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int d = 16 * nt + 4 * g + i;
+                float v;
+                if constexpr (!FP8)
+                  v = bf16_to_f32(reinterpret_cast<const uint16_t*>(vr)[d]);
+                else
+                  v = __builtin_amdgcn_cvt_f32_fp8(vr[d], 0);
+                acc[rt][nt][i] = fmaf(pv, v, acc[rt][nt][i] * resc);
+              }
+          }
+        }
+      }
+    }
+
+    // ---- the waves' parts meet ----
+    __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l_run[rt] += __shfl_xor(l_run[rt], 16, 64);
+      l_run[rt] += __shfl_xor(l_run[rt], 32, 64);
+      if (g == 0) {
+        s_m[wave * ROWS + 16 * rt + nl] = m_run[rt];
+        s_l[wave * ROWS + 16 * rt + nl] = l_run[rt];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = 16 * rt + nl;
+      float M = -INFINITY;
+      for (int i = 0; i < NW; ++i) M = fmaxf(M, s_m[i * ROWS + r]);
+      const float f = m_run[rt] == -INFINITY && M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[rt] - M);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        *reinterpret_cast<v4f*>(ring + r * (D * 4) + (((4 * nt + g) ^ nl) << 4)) = acc[rt][nt] * f;
+    }
+    __syncthreads();
+    // row r, four columns a thread
+    float* const part = a.part + (first_piece ? 2 * int64_t(w) : 2 * int64_t(w) + 1) * C::SLOT;
+    for (int i = tid; i < ROWS * (D / 4); i += 64 * NW) {
+      const int r = i / (D / 4), ch = i % (D / 4);
+      const int rr = rg * ROWS + r;
+      if (rr >= R) continue;
+      float M = -INFINITY, l = 0.0f;
+      for (int j = 0; j < NW; ++j) M = fmaxf(M, s_m[j * ROWS + r]);
+      for (int j = 0; j < NW; ++j) {
+        const float m = s_m[j * ROWS + r];
+        l += s_l[j * ROWS + r] * (m == -INFINITY && M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M));
+      }
+      v4f o = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < NW; ++j)
+        o += *reinterpret_cast<const v4f*>(lds + j * C::RING + r * (D * 4) + ((ch ^ (r & 15)) << 4));
+      if (whole) {
+        const int head = hk * grp + rr % grp, s = rr / grp;
+        float den = l, f = 1.0f, Mf = M;
+        if (a.sink) {
+          const float sk = a.sink[head] * kLog2e;
+          Mf = fmaxf(M, sk);
+          const float Me = Mf == -INFINITY ? 0.0f : Mf;
+          f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Me);
+          den = l * f + __builtin_amdgcn_exp2f(sk - Me);
+        }
+        const float inv = den == 0.0f ? 0.0f : f / den;
+        uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D + ch * 4;
+        *reinterpret_cast<uint2*>(orow) =
+            make_uint2(f32x2_to_bf16x2(o[0] * inv, o[1] * inv), f32x2_to_bf16x2(o[2] * inv, o[3] * inv));
+        if (a.ml && ch == 0) {
+          float* const e = a.ml + 2 * ((int64_t(b) * a.c.heads + hk) * R + rr);
+          e[0] = Mf == -INFINITY ? 0.0f : Mf;
+          e[1] = den == 0.0f ? 0.0f : 1.0f / den;
+        }
+      } else {
+        *reinterpret_cast<v4f*>(part + 2 * ROWS + r * D + ch * 4) = o;
+        if (ch == 0) {
+          part[r] = M;
+          part[ROWS + r] = l;
+        }
+      }
+    }
+    __syncthreads();
+    x = ubeg + g1;
+  }
+}
+
+// Merges a cut unit's partials, four rows a workgroup; a unit without tokens gets zeros.
+template <int D, int ROWS, int G>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
+  constexpr int64_t SLOT = int64_t(ROWS) * (D + 2);
+  const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
+  const int r4 = blockIdx.x % (ROWS / 4) * 4, unit = blockIdx.x / (ROWS / 4);
+  const int b = unit / upb, u = unit % upb, hk = u / RG, rg = u % RG;
+  if (rg * ROWS + r4 >= R) return;
+  const int n = paged_len(a, b), gran = (n + G - 1) / G;
+  const int64_t total = paged_total<G>(a, upb);
+  const int W = paged_workers(total, a.W);
+  int w0 = 0, w1 = -1;
+  int64_t ubeg = 0;
+  if (n > 0) {
+    const int lane = threadIdx.x & 63;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < b; b0 += 64) {
+      int gs = b0 + lane < b ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
+      for (int o = 1; o < 64; o <<= 1) gs += __shfl_xor(gs, o, 64);
+      before += gs;
+    }
+    ubeg = before * upb + int64_t(u) * gran;
+    w0 = paged_owner(total, W, ubeg);
+    w1 = paged_owner(total, W, ubeg + gran - 1);
+    if (w0 == w1) return;  // finished by its workgroup
+  }
+  const int64_t slot0 = n > 0 ? 2 * int64_t(w0) + (paged_share(total, W, w0) >= ubeg ? 0 : 1) : 0;
+  for (int i = threadIdx.x; i < 4 * (D / 4); i += 256) {
+    const int r = r4 + i / (D / 4), ch = i % (D / 4), rr = rg * ROWS + r;
+    if (rr >= R) continue;
+    const int head = hk * grp + rr % grp, s = rr / grp;
+    const float sk = a.sink ? a.sink[head] * kLog2e : -INFINITY;
+    float M = sk;
+    for (int w = w0; w <= w1; ++w) M = fmaxf(M, a.part[(w == w0 ? slot0 : 2 * int64_t(w)) * SLOT + r]);
+    const float Me = M == -INFINITY ? 0.0f : M;
+    float den = a.sink ? __builtin_amdgcn_exp2f(sk - Me) : 0.0f;
+    v4f o = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int w = w0; w <= w1; ++w) {
+      const float* const p = a.part + (w == w0 ? slot0 : 2 * int64_t(w)) * SLOT;
+      const float f = __builtin_amdgcn_exp2f(p[r] - Me);
+      den += f * p[ROWS + r];
+      o += *reinterpret_cast<const v4f*>(p + 2 * ROWS + r * D + ch * 4) * f;
+    }
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D + ch * 4;
+    *reinterpret_cast<uint2*>(orow) =
+        make_uint2(f32x2_to_bf16x2(o[0] * inv, o[1] * inv), f32x2_to_bf16x2(o[2] * inv, o[3] * inv));
+    if (a.ml && ch == 0) {
+      float* const e = a.ml + 2 * ((int64_t(b) * a.c.heads + hk) * R + rr);
+      e[0] = Me;
+      e[1] = inv;
+    }
+  }
+}
+
+// Row tiles of a unit: as many as hold the rows, up to what the registers hold.
+constexpr int paged_row_tiles(int D, int R) {
+  const int most = D <= 128 ? 4 : D == 256 ? 2 : 1;
+  const int want = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  return want < most ? want : most;
+}
+
+template <int D, bool FP8, bool SHARED, int RT>
+int paged_attn_launch_rt(PagedAttnArgs a, hipStream_t stream) {
+  using C = PagedCfg<D, FP8, SHARED, RT>;
+  static_assert(C::LDS <= 160 * 1024, "a workgroup's LDS");
+  static LdsGrant grant;
+  auto* const kernel = paged_attn_kernel<D, FP8, SHARED, RT>;
+  if (int rc = allow_lds("paged_attn", kernel, C::LDS, grant)) return rc;
+  WZ_LAUNCH("paged_attn", stream, kernel, dim3{unsigned(a.W)}, dim3(64 * C::NW), C::LDS, a);
+  if (int rc = check_launch("paged_attn")) return rc;
+  const int R = a.S * (a.H / a.c.heads);
+  const int64_t units = int64_t(a.B) * a.c.heads * ((R + C::ROWS - 1) / C::ROWS);
+  auto* const join = paged_attn_join_kernel<D, C::ROWS, C::G>;
+  WZ_LAUNCH("paged_attn_join", stream, join, dim3{unsigned(units * (C::ROWS / 4))}, dim3(256), 0, a);
+  return check_launch("paged_attn_join");
+}
+
+template <int D, bool FP8, bool SHARED>
+int paged_attn_launch_d(const PagedAttnArgs& a, hipStream_t stream) {
+  const int rt = paged_row_tiles(D, a.S * (a.H / a.c.heads));
+  if constexpr (D <= 128)
+    if (rt == 4) return paged_attn_launch_rt<D, FP8, SHARED, 4>(a, stream);
+  if constexpr (D <= 256)
+    if (rt == 2) return paged_attn_launch_rt<D, FP8, SHARED, 2>(a, stream);
+  return paged_attn_launch_rt<D, FP8, SHARED, 1>(a, stream);
+}
+
+template <bool FP8>
+int paged_attn_launch(int D, const PagedAttnArgs& a, hipStream_t stream) {
+  if (a.c.shared) {
+    if (D == 128) return paged_attn_launch_d<128, FP8, true>(a, stream);
+    if (D == 256) return paged_attn_launch_d<256, FP8, true>(a, stream);
+    return paged_attn_launch_d<512, FP8, true>(a, stream);
+  }
+  if (D == 64) return paged_attn_launch_d<64, FP8, false>(a, stream);
+  if (D == 128) return paged_attn_launch_d<128, FP8, false>(a, stream);
+  return paged_attn_launch_d<256, FP8, false>(a, stream);
+}
+
+int paged_attn_bf16(int D, const PagedAttnArgs& a, hipStream_t stream);
+int paged_attn_e4m3(int D, const PagedAttnArgs& a, hipStream_t stream);
+
+}  // namespace wz

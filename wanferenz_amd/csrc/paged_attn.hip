@@ -1,0 +1,112 @@
+// paged_attn: the kernels for bf16 rows, the weights' accumulation and the entry points.
+#include "paged_attn.h"
+
+namespace wz {
+
+int paged_attn_bf16(int D, const PagedAttnArgs& a, hipStream_t stream) { return paged_attn_launch<false>(D, a, stream); }
+
+// weights[slot] += sum over the KV head's rows that see the slot of 2^(y - m) / sum, rows in
+// ascending order.  A thread per slot; blockIdx.y = (sequence, head).
+__global__ __launch_bounds__(256) void paged_attn_weigh_kernel(PagedAttnArgs a) {
+  extern __shared__ float s_ml[];
+  const int bh = blockIdx.y, b = bh / a.c.heads, hk = bh % a.c.heads;
+  const int grp = a.H / a.c.heads, R = a.S * grp;
+  const int n = paged_len(a, b);
+  if (int(blockIdx.x) * 256 >= n) return;
+  for (int i = threadIdx.x; i < 2 * R; i += 256) s_ml[i] = a.ml[2 * int64_t(bh) * R + i];
+  __syncthreads();
+  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < n; t += int64_t(gridDim.x) * 256) {
+    const int64_t at = paged_row(a.c, a.table + int64_t(b) * a.width, a.width, hk, int(t));
+    if (at < 0) continue;
+    const float* const y = a.scores + int64_t(bh) * R * a.capacity + t;
+    float sum = 0.0f;
+    for (int r = 0; r < R; ++r)
+      if (t < n - (a.S - 1 - r / grp)) sum += __builtin_amdgcn_exp2f(y[r * a.capacity] - s_ml[2 * r]) * s_ml[2 * r + 1];
+    a.c.weights[at] += sum;
+  }
+}
+
+struct PagedAttnSizes {
+  int64_t part, ml, scores;  // floats
+};
+
+static PagedAttnSizes paged_attn_sizes(const wz_paged_kv* c, int64_t B, int64_t S, int64_t H, int64_t width,
+                                       bool accumulate) {
+  PagedAttnSizes z{};
+  const int64_t R = S * (H / c->kv_heads);
+  const int rows = 16 * paged_row_tiles(c->head_dim, int(R));
+  z.part = 2 * int64_t(cu_count()) * rows * (c->head_dim + 2);
+  if (accumulate) {
+    z.ml = (2 * B * c->kv_heads * R + 3) / 4 * 4;
+    z.scores = B * c->kv_heads * R * width * c->page_size;
+  }
+  return z;
+}
+
+}  // namespace wz
+
+extern "C" int64_t wz_paged_attn_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t S, int64_t H,
+                                                 int64_t table_width, int accumulate) {
+  using namespace wz;
+  if (!cache || cache->kv_heads <= 0 || B <= 0 || S <= 0 || S > kPagedMaxS || H <= 0 || H > 65536 || table_width <= 0)
+    return 0;
+  const PagedAttnSizes z = paged_attn_sizes(cache, B, S, H, table_width, accumulate != 0);
+  return (z.part + z.ml + z.scores) * int64_t(sizeof(float));
+}
+
+extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q_strides,
+                             const float* attn_sink, const int32_t* table, int64_t table_width, const int32_t* lens,
+                             void* o_bf16, int64_t B, int64_t S, int64_t H, float softmax_scale, int accumulate,
+                             void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  using namespace wz;
+  PagedAttnArgs a{};
+  if (int rc = paged_view("paged_attn", cache, table_width, &a.c)) return rc;
+  if (B < 0 || B > 65535 || S < 0 || S > kPagedMaxS)
+    return set_error(WZ_EINVAL, "paged_attn: bad shape B=%lld (up to 65535) S=%lld (up to %d)", (long long)B,
+                     (long long)S, kPagedMaxS);
+  if (H <= 0 || H > 65536 || H % a.c.heads)
+    return set_error(WZ_EINVAL, "paged_attn: %lld heads on %d KV heads", (long long)H, a.c.heads);
+  if (accumulate && !a.c.weights)
+    return set_error(WZ_EINVAL, "paged_attn: the cache is not tracked (weights and positions)");
+  if (B == 0 || S == 0) return WZ_OK;
+  if (!q_bf16 || !q_strides || !lens || !o_bf16 || (table_width > 0 && !table))
+    return set_error(WZ_EINVAL, "paged_attn: null pointer");
+  if ((reinterpret_cast<uintptr_t>(q_bf16) | reinterpret_cast<uintptr_t>(o_bf16) |
+       reinterpret_cast<uintptr_t>(workspace)) & 15 || ((q_strides[0] | q_strides[1] | q_strides[2]) & 7))
+    return set_error(WZ_EINVAL, "paged_attn: q rows, o and the workspace must be 16-byte aligned");
+  const int64_t R = S * (H / a.c.heads);
+  const int64_t units = B * a.c.heads * ((R + 15) / 16);
+  if (units * 16 > 0x7FFFFFFFLL || B * a.c.heads > 65535 * int64_t(accumulate ? 1 : 65535))
+    return set_error(WZ_EINVAL, "paged_attn: %lld sequences of %lld heads", (long long)B, (long long)H);
+  if (2 * R * int64_t(sizeof(float)) > 65536)
+    return set_error(WZ_EINVAL, "paged_attn: %lld query rows on a KV head", (long long)R);
+  const PagedAttnSizes z = paged_attn_sizes(cache, B, S, H, table_width, accumulate != 0);
+  const int64_t need = (z.part + z.ml + z.scores) * int64_t(sizeof(float));
+  if (!workspace || workspace_bytes < need)
+    return set_error(WZ_ESPACE, "paged_attn: workspace of %lld bytes, %lld needed",
+                     (long long)(workspace ? workspace_bytes : 0), (long long)need);
+  a.q = static_cast<const uint16_t*>(q_bf16);
+  a.qb = q_strides[0];
+  a.qs = q_strides[1];
+  a.qh = q_strides[2];
+  a.sink = attn_sink;
+  a.table = table;
+  a.lens = lens;
+  a.o = static_cast<uint16_t*>(o_bf16);
+  a.part = static_cast<float*>(workspace);
+  a.ml = accumulate ? a.part + z.part : nullptr;
+  a.scores = accumulate ? a.part + z.part + z.ml : nullptr;
+  a.width = int(table_width);
+  a.B = int(B);
+  a.S = int(S);
+  a.H = int(H);
+  a.W = cu_count();
+  a.capacity = table_width * a.c.page;
+  a.scale2 = softmax_scale * kLog2e;
+  const int rc = a.c.ks ? paged_attn_e4m3(cache->head_dim, a, stream) : paged_attn_bf16(cache->head_dim, a, stream);
+  if (rc != WZ_OK || !accumulate || a.capacity == 0) return rc;
+  const int64_t blocks = std::min<int64_t>((a.capacity + 255) / 256, 1024);
+  WZ_LAUNCH("paged_attn_weigh", stream, paged_attn_weigh_kernel, dim3(unsigned(blocks), unsigned(B * a.c.heads)),
+            dim3(256), 2 * R * sizeof(float), a);
+  return check_launch("paged_attn_weigh");
+}
