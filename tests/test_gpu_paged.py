@@ -345,11 +345,14 @@ def arrays(cache):
                                                    (torch.bfloat16, 1, 512, True, 64), (E4M3, 1, 256, True, 16)])
 @pytest.mark.parametrize("keep,first,recent", [(0, 0, 0), (1, 0, 1), (50, 4, 10), (64, 0, 0), (200, 200, 0), (1000, 3, 300),
                                               (1000, 0, 1000)])
-def test_evict(gpu, dtype, HK, D, shared, page, keep, first, recent):
+@pytest.mark.parametrize("slots", [0, 9000])
+def test_evict(gpu, dtype, HK, D, shared, page, keep, first, recent, slots):
     """The slots that stay, and where they lie, against the sorted order: ragged lengths around the budget,
-    many equal weights, infinities and NaN among them, positions in any order."""
+    many equal weights, infinities and NaN among them, positions in any order.  A table of 9000 slots has
+    several workgroups share a unit."""
     lens = [0, 1, keep, keep + 1, keep + 7, 2 * keep + 3, 1300]
-    cache, _, tab, table = make(gpu, 3 + keep, lens, HK=HK, D=D, page=page, dtype=dtype, shared=shared, track=True)
+    cache, _, tab, table = make(gpu, 3 + keep, lens, HK=HK, D=D, page=page, dtype=dtype, shared=shared, track=True,
+                                width=max(-(-max(lens) // page), -(-slots // page)))
     g = torch.Generator().manual_seed(keep)
     w = torch.randint(0, 6, cache.weights.shape, generator=g).float() / 4
     w[torch.rand(w.shape, generator=g) < 0.05] = float("nan")
@@ -371,10 +374,11 @@ def test_evict(gpu, dtype, HK, D, shared, page, keep, first, recent):
         assert np.array_equal(x, want[name], equal_nan=name == "weights"), name
 
 
-def test_evict_in_place_and_missing_pages(gpu):
+@pytest.mark.parametrize("slots", [0, 9000])
+def test_evict_in_place_and_missing_pages(gpu, slots):
     """lens as its own output; pages that the table lacks lose first and are not moved."""
     lens, page, keep = [160, 90, 30], 16, 64
-    cache, _, tab, table = make(gpu, 31, lens, HK=2, D=64, page=page, track=True)
+    cache, _, tab, table = make(gpu, 31, lens, HK=2, D=64, page=page, track=True, width=max(10, -(-slots // page)))
     table[0, 1], table[0, 9], table[1, 2] = -1, cache.pages + 5, -3
     want = arrays(cache)
     n = torch.tensor(lens, dtype=torch.int32, device=gpu)
@@ -385,7 +389,7 @@ def test_evict_in_place_and_missing_pages(gpu):
         assert np.array_equal(x, want[name]), name
 
 
-@pytest.mark.parametrize("n,keep", [(5000, 4096), (20000, 1500), (70001, 8192)])
+@pytest.mark.parametrize("n,keep", [(5000, 4096), (8200, 4000), (20000, 1500), (70001, 8192), (300000, 100000)])
 def test_evict_long(gpu, n, keep):
     """Lengths of many rounds of a workgroup, against torch's stable sort."""
     page, HK = 64, 2

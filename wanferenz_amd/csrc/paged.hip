@@ -89,7 +89,13 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedView c, WriteArgs
 
 // ---- evict ----
 
+constexpr int kEvictBins = 2048;         // keys are taken 11, 11 and 10 bits at a time
+constexpr int kEvictSmall = 8192;        // slots that one workgroup holds
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictChunk = 4096;        // slots of a workgroup where several share a unit
+constexpr int kEvictChunkThreads = 256;
+constexpr int64_t kEvictFused = 65536;   // bytes of K a unit's one workgroup moves itself
+constexpr int kNoPosition = -0x7FFFFFFF - 1;
 
 // A slot's place in the order of what stays, as an unsigned number: the float's bits, ordered
 // like the values (NaN lowest), a protected slot above them all.
@@ -101,129 +107,389 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
   return (k & 0x80000000u) ? ~k : k | 0x80000000u;
 }
 
-// One workgroup per (sequence, head): the keep-th largest key by four rounds of 8 bits, then one
-// pass in slot order that lists the holes below keep and the kept slots from keep on.
-__global__ __launch_bounds__(kEvictThreads) void paged_evict_select_kernel(
-    PagedView c, const int32_t* __restrict__ table, int width, const int32_t* __restrict__ lens,
-    int32_t* __restrict__ counts, int32_t* __restrict__ holes, int32_t* __restrict__ movers, int64_t moves_max,
-    int keep, int first, int recent) {
-  __shared__ int s_hist[256];
-  __shared__ int s_red[kEvictThreads / 64];
-  __shared__ int s_pick[2];
-  __shared__ int s_scan[3][kEvictThreads / 64];
-  const int u = blockIdx.x, b = u / c.heads, h = u % c.heads;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int32_t* const trow = table + int64_t(b) * width;
-  const int n = int(min(int64_t(max(lens[b], 0)), int64_t(width) << c.shift));
-  if (n <= keep) {
-    if (tid == 0) counts[u] = 0;
+// What the workgroups that share a unit tell each other.
+struct EvictUnit {
+  int32_t hist[3][kEvictBins];  // of the keys' three digits, each under the digits before
+  int32_t known[3][2];          // after each digit: the threshold's bits so far, and the keys still needed
+};
+
+struct EvictArgs {
+  PagedView c;
+  const int32_t* table;
+  const int32_t* lens;
+  int32_t* new_lens;
+  int32_t* counts;  // pairs of a unit (sequence, head)
+  int32_t* holes;   // [unit][moves]
+  int32_t* movers;
+  EvictUnit* unit;  // shared units only, as the rest
+  int32_t* newest;  // [unit][chunk]
+  int32_t* tally;   // [unit][chunk][4]
+  uint32_t* keys;   // [unit][capacity]
+  int64_t moves, capacity;
+  int width, keep, first, recent;
+};
+
+__device__ __forceinline__ int evict_len(const EvictArgs& a, int b) {
+  return int(min(int64_t(max(a.lens[b], 0)), a.capacity));
+}
+
+// Pair i of a unit: row `fro` over row `to`, 16 bytes a thread of lpr.
+__device__ __forceinline__ void evict_move(const EvictArgs& a, const int32_t* trow, int h, int hole, int mover, int ch,
+                                           int row_bytes) {
+  const PagedView& c = a.c;
+  const int64_t to = paged_row(c, trow, a.width, h, hole), fro = paged_row(c, trow, a.width, h, mover);
+  if (to < 0 || fro < 0) return;
+  const v4i k = load16(c.k + fro * row_bytes + ch * 16);
+  v4i v = v4i{0, 0, 0, 0};
+  if (!c.shared) v = load16(c.v + fro * row_bytes + ch * 16);
+  if (ch == 0) {
+    c.weights[to] = c.weights[fro];
+    c.positions[to] = c.positions[fro];
+    if (c.ks) c.ks[to] = c.ks[fro];
+    if (c.vs && !c.shared) c.vs[to] = c.vs[fro];
+  }
+  *reinterpret_cast<v4i*>(c.k + to * row_bytes + ch * 16) = k;
+  if (!c.shared) *reinterpret_cast<v4i*>(c.v + to * row_bytes + ch * 16) = v;
+}
+
+// A thread's R keys, of the slots t0 + 64 i: their positions and weights, all loads in flight together.
+template <int R>
+__device__ __forceinline__ void evict_load(const EvictArgs& a, const int32_t* trow, int h, int n, int t0, int64_t (&at)[R],
+                                           int (&p)[R], float (&w)[R]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) at[i] = t0 + 64 * i < n ? paged_row(a.c, trow, a.width, h, t0 + 64 * i) : -1;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    p[i] = at[i] >= 0 ? a.c.positions[at[i]] : kNoPosition;
+    w[i] = at[i] >= 0 ? a.c.weights[at[i]] : 0.0f;
+  }
+}
+
+__device__ __forceinline__ int wave_max(int x) {
+  for (int o = 1; o < 64; o <<= 1) x = max(x, __shfl_xor(x, o, 64));
+  return x;
+}
+__device__ __forceinline__ int wave_sum(int x) {
+  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+
+// The bin, from the top, in which the need-th key lies, and how many of its keys are needed.  Called
+// by a whole workgroup; the bins are not changed until everyone has read them.
+template <int THREADS>
+__device__ __forceinline__ void evict_pick(const int32_t* hist, int* bin, int* need) {
+  __shared__ int s_sum[THREADS / 64];
+  __shared__ int s_out[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, want = *need;
+  constexpr int P = kEvictBins / THREADS;
+  int c[P], sum = 0;
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    c[j] = hist[kEvictBins - 1 - (tid * P + j)];
+    sum += c[j];
+  }
+  int up = sum;  // inclusive over the workgroup
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(up, o, 64);
+    if (lane >= o) up += y;
+  }
+  if (lane == 63) s_sum[wave] = up;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) up += s_sum[i];
+  int before = up - sum;
+  // the keys are at least `want` in all, so one thread has the crossing (none wanted: the topmost bin)
+  if ((up >= want && before < want) || (want == 0 && tid == 0)) {
+    int j = 0;
+    while (j < P - 1 && before + c[j] < want) before += c[j++];
+    s_out[0] = kEvictBins - 1 - (tid * P + j);
+    s_out[1] = want - before;
+  }
+  __syncthreads();
+  *bin = s_out[0];
+  *need = s_out[1];
+}
+
+// Digit d (0, 1, 2) of a key, its place, and whether a key has the threshold's digits before it.
+__device__ __forceinline__ constexpr int evict_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+__device__ __forceinline__ int evict_digit(uint32_t k, int d) {
+  return int((k >> evict_shift(d)) & (d == 2 ? 1023u : 2047u));
+}
+__device__ __forceinline__ bool evict_under(uint32_t k, uint32_t prefix, int d) {
+  return d == 0 || (d == 1 ? (k ^ prefix) >> 21 == 0 : (k ^ prefix) >> 10 == 0);
+}
+
+// A wave's counts of its R rounds: kept slots above the threshold and ties, below keep and past it.
+template <int R>
+__device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, int n, int keep, uint32_t top, int (&sum)[4]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int t = t0 + 64 * i;
+    const bool in = t < n, low = t < keep, gt = in && key[i] > top, tie = in && key[i] == top;
+    sum[0] += __popcll(__ballot(gt && low));
+    sum[1] += __popcll(__ballot(tie && low));
+    sum[2] += __popcll(__ballot(gt && !low));
+    sum[3] += __popcll(__ballot(tie && !low));
+  }
+}
+
+// A wave's part of the lists.  `before`: evict_count's sums of the slots before the wave's, `all`: of
+// the unit.  Of the ties the lowest `need` stay, so those below keep go first.  -> the unit's pairs
+template <int R>
+__device__ __forceinline__ int evict_list(const EvictArgs& a, int u, const uint32_t (&key)[R], int t0, int n, uint32_t top,
+                                          int need, const int (&before)[4], const int (&all)[4]) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t below = (1ull << lane) - 1;
+  const int high = max(0, need - all[1]);  // ties past keep that stay
+  const int pairs = int(min(int64_t(all[2] + min(all[3], high)), a.moves));
+  int ties = before[1] + before[3];
+  int ih = min(t0 - lane, a.keep) - before[0] - min(before[1], need);  // dropped slots below keep
+  int im = before[2] + min(before[3], high);                          // kept slots past it
+  int32_t* const holes = a.holes + u * a.moves;
+  int32_t* const movers = a.movers + u * a.moves;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int t = t0 + 64 * i;
+    const uint64_t tie = __ballot(t < n && key[i] == top);
+    const bool kept = t < n && (key[i] > top || (key[i] == top && ties + __popcll(tie & below) < need));
+    ties += __popcll(tie);
+    const bool hole = t < n && !kept && t < a.keep, mover = kept && t >= a.keep;
+    const uint64_t bh = __ballot(hole), bm = __ballot(mover);
+    const int x = ih + __popcll(bh & below), y = im + __popcll(bm & below);
+    if (hole && x < pairs) holes[x] = t;
+    if (mover && y < pairs) movers[y] = t;
+    ih += __popcll(bh);
+    im += __popcll(bm);
+  }
+  return pairs;
+}
+
+// A unit (sequence, head) of up to kEvictSmall slots: the keep-th largest key by three digits, then the
+// holes below keep and the kept slots from keep on, in slot order.  Every wave has a range of
+// consecutive slots, 64 a round with the keys in registers, so the ranks need one exchange between the
+// waves.  MOVE: few pairs are moved here, which saves the second launch.
+template <bool MOVE>
+__global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictArgs a, int row_bytes) {
+  constexpr int R = kEvictSmall / kEvictThreads, NW = kEvictThreads / 64;
+  __shared__ int s_hist[3][kEvictBins];
+  __shared__ int s_wave[4][NW];
+  const int u = blockIdx.x, b = u / a.c.heads, h = u - b * a.c.heads;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t* const trow = a.table + int64_t(b) * a.width;
+  const int n = evict_len(a, b);
+  if (MOVE && h == 0 && tid == 0) a.new_lens[b] = min(a.lens[b], a.keep);
+  if (n <= a.keep) {
+    if (!MOVE && tid == 0) a.counts[u] = 0;
     return;
   }
-  int last = -0x7FFFFFFF - 1;
-  for (int t = tid; t < n; t += kEvictThreads) {
-    const int64_t at = paged_row(c, trow, width, h, t);
-    if (at >= 0) last = max(last, c.positions[at]);
-  }
-  for (int o = 1; o < 64; o <<= 1) last = max(last, __shfl_xor(last, o, 64));
-  if (lane == 0) s_red[wave] = last;
+  const int per = ((n + 63) / 64 + NW - 1) / NW;  // rounds of a wave, up to R
+  const int t0 = wave * per * 64 + lane;
+  const int end = min(n, (wave + 1) * per * 64);
+  int64_t at[R];
+  int p[R];
+  float w[R];
+  evict_load<R>(a, trow, h, end, t0, at, p, w);
+  for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
+  int last = kNoPosition;
+#pragma unroll
+  for (int i = 0; i < R; ++i) last = max(last, p[i]);
+  last = wave_max(last);
+  if (lane == 0) s_wave[0][wave] = last;
   __syncthreads();
-  for (int i = 0; i < kEvictThreads / 64; ++i) last = max(last, s_red[i]);
-  auto key_of = [&](int t) -> uint32_t {
-    const int64_t at = paged_row(c, trow, width, h, t);
-    if (at < 0) return 0u;
-    const int p = c.positions[at];
-    return evict_key(c.weights[at], p < first || int64_t(p) > int64_t(last) - recent);
-  };
-  uint32_t prefix = 0, mask = 0;
-  int need = keep;  // of the keys that match the prefix
-  for (int sh = 24; sh >= 0; sh -= 8) {
-    for (int i = tid; i < 256; i += kEvictThreads) s_hist[i] = 0;
+  last = wave_max(s_wave[0][lane & (NW - 1)]);
+  const int64_t old = int64_t(last) - a.recent;  // positions above it are protected
+  uint32_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) key[i] = at[i] < 0 ? 0u : evict_key(w[i], p[i] < a.first || int64_t(p[i]) > old);
+  uint32_t top = 0;
+  int need = a.keep;
+#pragma unroll
+  for (int d = 0; d < 3; ++d) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (t0 + 64 * i < end && evict_under(key[i], top, d)) atomicAdd(&s_hist[d][evict_digit(key[i], d)], 1);
     __syncthreads();
-    for (int t = tid; t < n; t += kEvictThreads) {
-      const uint32_t k = key_of(t);
-      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> sh) & 255], 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int left = need, d = 255;
-      while (d > 0 && s_hist[d] < left) left -= s_hist[d--];
-      s_pick[0] = d;
-      s_pick[1] = left;
-    }
-    __syncthreads();
-    prefix |= uint32_t(s_pick[0]) << sh;
-    mask |= 255u << sh;
-    need = s_pick[1];
-    __syncthreads();
+    int bin;
+    evict_pick<kEvictThreads>(s_hist[d], &bin, &need);
+    top |= uint32_t(bin) << evict_shift(d);
   }
-  // prefix: the keep-th largest key; `need` slots that have it stay, the lowest first
-  int ties = 0, nh = 0, nm = 0;
-  for (int t0 = 0; t0 < n; t0 += kEvictThreads) {
-    const int t = t0 + tid;
-    const uint32_t k = t < n ? key_of(t) : 0u;
-    const bool tie = t < n && k == prefix;
-    const uint64_t bt = __ballot(tie);
-    const uint64_t below = (1ull << lane) - 1;
-    if (lane == 0) s_scan[0][wave] = __popcll(bt);
-    __syncthreads();
-    int tb = ties + __popcll(bt & below);
-    for (int i = 0; i < kEvictThreads / 64; ++i) {
-      if (i < wave) tb += s_scan[0][i];
-      ties += s_scan[0][i];
+  int sum[4] = {0, 0, 0, 0};
+  evict_count<R>(key, t0, end, a.keep, top, sum);
+  if (lane == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s_wave[j][wave] = sum[j];
+  __syncthreads();
+  int before[4], all[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int x = lane < NW ? s_wave[j][lane] : 0;
+    all[j] = wave_sum(x);
+    before[j] = wave_sum(lane < wave ? x : 0);
+  }
+  const int pairs = evict_list<R>(a, u, key, t0, end, top, need, before, all);
+  if constexpr (MOVE) {
+    __threadfence_block();
+    __syncthreads();  // the lists, written and read by this workgroup
+    const int lpr = row_bytes / 16;
+    const int64_t list = u * a.moves;
+    for (int i = tid; i < pairs * lpr; i += kEvictThreads)
+      evict_move(a, trow, h, a.holes[list + i / lpr], a.movers[list + i / lpr], i % lpr, row_bytes);
+  } else if (tid == 0) {
+    a.counts[u] = pairs;
+  }
+}
+
+// The same for longer units, which one compute unit's instruction rate would bound (32767 slots of 16
+// units took it 87 us, 65535 of one 160): a workgroup per chunk of kEvictChunk slots, a launch for
+// each time that the workgroups have to meet.  STEP 0: the chunk's newest position, and the unit's
+// histograms cleared.  1: keys and the first digit's histogram.  2, 3: the second's and third's.
+// 4: the chunk's counts.  5: its part of the lists.
+template <int STEP>
+__global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(EvictArgs a) {
+  constexpr int R = kEvictChunk / kEvictChunkThreads, NW = kEvictChunkThreads / 64;
+  const int u = blockIdx.y, chunk = blockIdx.x, nb = gridDim.x, b = u / a.c.heads, h = u - b * a.c.heads;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t* const trow = a.table + int64_t(b) * a.width;
+  const int n = evict_len(a, b);
+  EvictUnit& st = a.unit[u];
+  int32_t* const newest = a.newest + int64_t(u) * nb;
+  int32_t* const tally = a.tally + int64_t(u) * nb * 4;
+  uint32_t* const keys = a.keys + u * a.capacity;
+  if constexpr (STEP == 0)
+    for (int i = chunk * kEvictChunkThreads + tid; i < 3 * kEvictBins; i += nb * kEvictChunkThreads)
+      (&st.hist[0][0])[i] = 0;
+  if (n <= a.keep) {
+    if (STEP == 5 && chunk == 0 && tid == 0) a.counts[u] = 0;
+    return;
+  }
+  const int chunks = (n + kEvictChunk - 1) / kEvictChunk;
+  if (chunk >= chunks) return;
+  const int t0 = chunk * kEvictChunk + wave * (64 * R) + lane;
+  const int end = min(n, t0 - lane + 64 * R);
+  __shared__ int s_wave[4][NW];
+  uint32_t key[R];
+  if constexpr (STEP <= 1) {
+    int64_t at[R];
+    int p[R];
+    float w[R];
+    evict_load<R>(a, trow, h, end, t0, at, p, w);
+    if constexpr (STEP == 0) {
+      int last = kNoPosition;
+#pragma unroll
+      for (int i = 0; i < R; ++i) last = max(last, p[i]);
+      last = wave_max(last);
+      if (lane == 0) s_wave[0][wave] = last;
+      __syncthreads();
+      if (tid == 0) newest[chunk] = max(max(s_wave[0][0], s_wave[0][1]), max(s_wave[0][2], s_wave[0][3]));
+      return;
     }
-    const bool kept = t < n && (k > prefix || (tie && tb < need));
-    const bool hole = t < n && !kept && t < keep, mover = kept && t >= keep;
-    const uint64_t bh = __ballot(hole), bm = __ballot(mover);
-    if (lane == 0) {
-      s_scan[1][wave] = __popcll(bh);
-      s_scan[2][wave] = __popcll(bm);
+    int last = kNoPosition;
+    for (int i = lane; i < chunks; i += 64) last = max(last, newest[i]);
+    const int64_t old = int64_t(wave_max(last)) - a.recent;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      key[i] = at[i] < 0 ? 0u : evict_key(w[i], p[i] < a.first || int64_t(p[i]) > old);
+      if (t0 + 64 * i < end) keys[t0 + 64 * i] = key[i];
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) key[i] = t0 + 64 * i < end ? keys[t0 + 64 * i] : 0u;
+  }
+  // the threshold's digits so far; the launch before wrote what is read here
+  uint32_t top = 0;
+  int need = a.keep;
+  if constexpr (STEP > 2) {
+    top = uint32_t(st.known[STEP - 3][0]);
+    need = st.known[STEP - 3][1];
+  }
+  if constexpr (STEP >= 2 && STEP <= 4) {
+    int bin;
+    evict_pick<kEvictChunkThreads>(st.hist[STEP - 2], &bin, &need);
+    top |= uint32_t(bin) << evict_shift(STEP - 2);
+    if (chunk == 0 && tid == 0) {
+      st.known[STEP - 2][0] = int32_t(top);
+      st.known[STEP - 2][1] = need;
+    }
+  }
+  if constexpr (STEP >= 1 && STEP <= 3) {
+    constexpr int d = STEP - 1;
+    __shared__ int s_hist[kEvictBins];
+    for (int i = tid; i < kEvictBins; i += kEvictChunkThreads) s_hist[i] = 0;
     __syncthreads();
-    int ih = nh + __popcll(bh & below), im = nm + __popcll(bm & below);
-    for (int i = 0; i < kEvictThreads / 64; ++i) {
-      if (i < wave) {
-        ih += s_scan[1][i];
-        im += s_scan[2][i];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (t0 + 64 * i < end && evict_under(key[i], top, d)) atomicAdd(&s_hist[evict_digit(key[i], d)], 1);
+    __syncthreads();
+    for (int i = tid; i < kEvictBins; i += kEvictChunkThreads)
+      if (s_hist[i]) atomicAdd(&st.hist[d][i], s_hist[i]);  // integers: the order does not matter
+  }
+  if constexpr (STEP >= 4) {
+    int sum[4] = {0, 0, 0, 0};
+    evict_count<R>(key, t0, end, a.keep, top, sum);
+    if (lane == 0)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s_wave[j][wave] = sum[j];
+    __syncthreads();
+    if constexpr (STEP == 4) {
+      if (tid < 4) tally[chunk * 4 + tid] = s_wave[tid][0] + s_wave[tid][1] + s_wave[tid][2] + s_wave[tid][3];
+    } else {
+      int before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
+      for (int i = lane; i < chunks; i += 64)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int x = tally[i * 4 + j];
+          all[j] += x;
+          before[j] += i < chunk ? x : 0;
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        all[j] = wave_sum(all[j]);
+        before[j] = wave_sum(before[j]);
+        for (int i = 0; i < wave; ++i) before[j] += s_wave[j][i];
       }
-      nh += s_scan[1][i];
-      nm += s_scan[2][i];
+      const int pairs = evict_list<R>(a, u, key, t0, end, top, need, before, all);
+      if (chunk == 0 && tid == 0) a.counts[u] = pairs;
     }
-    if (hole && ih < moves_max) holes[u * moves_max + ih] = t;
-    if (mover && im < moves_max) movers[u * moves_max + im] = t;
-    __syncthreads();
   }
-  if (tid == 0) counts[u] = min(nh, nm);
 }
 
 // The pairs' rows: D * element / 16 threads a row, K and V and what belongs to the slot.
-__global__ __launch_bounds__(256) void paged_evict_move_kernel(
-    PagedView c, const int32_t* __restrict__ table, int width, const int32_t* __restrict__ lens,
-    int32_t* __restrict__ new_lens, const int32_t* __restrict__ counts, const int32_t* __restrict__ holes,
-    const int32_t* __restrict__ movers, int64_t moves_max, int keep, int row_bytes) {
-  const int u = blockIdx.y, b = u / c.heads, h = u % c.heads;
-  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0)
-    new_lens[b] = min(lens[b], keep);
+__global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a, int row_bytes) {
+  const int u = blockIdx.y, b = u / a.c.heads, h = u - b * a.c.heads;
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.new_lens[b] = min(a.lens[b], a.keep);
   const int lpr = row_bytes / 16;
-  const int count = counts[u];
-  const int32_t* const trow = table + int64_t(b) * width;
+  const int count = a.counts[u];
+  const int32_t* const trow = a.table + int64_t(b) * a.width;
   for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < int64_t(count) * lpr; t += int64_t(gridDim.x) * 256) {
-    const int i = int(t / lpr), ch = int(t % lpr);
-    const int64_t to = paged_row(c, trow, width, h, holes[u * moves_max + i]);
-    const int64_t fro = paged_row(c, trow, width, h, movers[u * moves_max + i]);
-    if (to < 0 || fro < 0) continue;
-    *reinterpret_cast<v4i*>(c.k + to * row_bytes + ch * 16) = load16(c.k + fro * row_bytes + ch * 16);
-    if (!c.shared) *reinterpret_cast<v4i*>(c.v + to * row_bytes + ch * 16) = load16(c.v + fro * row_bytes + ch * 16);
-    if (ch == 0) {
-      c.weights[to] = c.weights[fro];
-      c.positions[to] = c.positions[fro];
-      if (c.ks) c.ks[to] = c.ks[fro];
-      if (c.vs && !c.shared) c.vs[to] = c.vs[fro];
-    }
+    const int64_t i = u * a.moves + t / lpr;
+    evict_move(a, trow, h, a.holes[i], a.movers[i], int(t % lpr), row_bytes);
   }
 }
 
 static int64_t evict_moves_max(const wz_paged_kv* c, int64_t width, int64_t keep) {
   return std::max<int64_t>(0, std::min(keep, width * c->page_size - keep));
+}
+
+// Bytes of the workspace's parts, in order: EvictUnit, newest, tally, keys (shared units only), counts,
+// holes, movers.
+struct EvictSizes {
+  int64_t units, chunks, unit, newest, tally, keys, counts, moves, total;
+};
+
+static EvictSizes evict_sizes(const wz_paged_kv* c, int64_t B, int64_t width, int64_t keep) {
+  EvictSizes z{};
+  const int64_t capacity = width * c->page_size;
+  z.units = B * c->kv_heads;
+  z.moves = evict_moves_max(c, width, keep);
+  if (capacity > kEvictSmall) {
+    z.chunks = (capacity + kEvictChunk - 1) / kEvictChunk;
+    z.unit = z.units * int64_t(sizeof(EvictUnit));
+    z.newest = 4 * z.units * z.chunks;
+    z.tally = 16 * z.units * z.chunks;
+    z.keys = 4 * z.units * capacity;
+  }
+  z.counts = 4 * z.units;
+  z.total = z.unit + z.newest + z.tally + z.keys + z.counts + 8 * z.units * z.moves;
+  return z;
 }
 
 }  // namespace wz
@@ -283,8 +549,7 @@ extern "C" int64_t wz_paged_evict_workspace_bytes(const wz_paged_kv* cache, int6
                                                   int64_t keep) {
   using namespace wz;
   if (!cache || B <= 0 || table_width < 0 || keep < 0 || cache->page_size <= 0 || cache->kv_heads <= 0) return 0;
-  const int64_t units = B * cache->kv_heads;
-  return (units + 2 * units * evict_moves_max(cache, table_width, keep)) * int64_t(sizeof(int32_t));
+  return evict_sizes(cache, B, table_width, keep).total;
 }
 
 extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, int64_t table_width, const int32_t* lens,
@@ -305,19 +570,63 @@ extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, in
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(WZ_ESPACE, "paged_evict: workspace of %lld bytes, %lld needed",
                      (long long)(workspace ? workspace_bytes : 0), (long long)need);
-  const int64_t units = B * c.heads, moves = evict_moves_max(cache, table_width, keep);
-  int32_t* const counts = static_cast<int32_t*>(workspace);
-  int32_t* const holes = counts + units;
-  int32_t* const movers = holes + units * moves;
-  const int width = int(table_width);
-  if (reinterpret_cast<uintptr_t>(workspace) & 3) return set_error(WZ_EINVAL, "paged_evict: workspace alignment");
-  WZ_LAUNCH("paged_evict_select", stream, paged_evict_select_kernel, dim3{unsigned(units)}, dim3(kEvictThreads), 0, c,
-            table, width, lens, counts, holes, movers, moves, int(keep), int(first), int(recent));
-  if (int rc = check_launch("paged_evict")) return rc;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return set_error(WZ_EINVAL, "paged_evict: the workspace must be 16-byte aligned");
+  const EvictSizes z = evict_sizes(cache, B, table_width, keep);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  auto take = [&](int64_t bytes) {
+    uint8_t* const p = ws;
+    ws += bytes;
+    return p;
+  };
+  EvictArgs a{};
+  a.c = c;
+  a.table = table;
+  a.lens = lens;
+  a.new_lens = new_lens;
+  a.unit = reinterpret_cast<EvictUnit*>(take(z.unit));
+  a.newest = reinterpret_cast<int32_t*>(take(z.newest));
+  a.tally = reinterpret_cast<int32_t*>(take(z.tally));
+  a.keys = reinterpret_cast<uint32_t*>(take(z.keys));
+  a.counts = reinterpret_cast<int32_t*>(take(z.counts));
+  a.holes = reinterpret_cast<int32_t*>(take(4 * z.units * z.moves));
+  a.movers = reinterpret_cast<int32_t*>(take(4 * z.units * z.moves));
+  a.moves = z.moves;
+  a.capacity = table_width * c.page;
+  a.width = int(table_width);
+  a.keep = int(keep);
+  a.first = int(first);
+  a.recent = int(recent);
   const int row_bytes = cache->head_dim * (c.ks ? 1 : 2);
-  const int64_t blocks = std::min<int64_t>(std::max<int64_t>(1, (moves * (row_bytes / 16) + 255) / 256),
-                                           std::max<int64_t>(1, 4096 / units));
-  WZ_LAUNCH("paged_evict_move", stream, paged_evict_move_kernel, dim3(unsigned(blocks), unsigned(units)), dim3(256), 0,
-            c, table, width, lens, new_lens, counts, holes, movers, moves, int(keep), row_bytes);
+  const unsigned units = unsigned(z.units);
+  if (z.chunks == 0) {
+    // Up to kEvictFused bytes of a unit are moved by the workgroup that chose them.  The lengths can
+    // then be written there too, unless other heads' workgroups still read them.
+    const bool move = z.moves * row_bytes <= kEvictFused && new_lens != lens;
+    if (move)
+      WZ_LAUNCH("paged_evict", stream, paged_evict_small_kernel<true>, dim3{units}, dim3(kEvictThreads), 0, a, row_bytes);
+    else
+      WZ_LAUNCH("paged_evict", stream, paged_evict_small_kernel<false>, dim3{units}, dim3(kEvictThreads), 0, a, row_bytes);
+    if (int rc = check_launch("paged_evict")) return rc;
+    if (move) return WZ_OK;
+  } else {
+#define WZ_EVICT(STEP)                                                                                               \
+  do {                                                                                                               \
+    WZ_LAUNCH("paged_evict", stream, paged_evict_chunk_kernel<STEP>, dim3(unsigned(z.chunks), units),                \
+              dim3(kEvictChunkThreads), 0, a);                                                                       \
+    if (int rc = check_launch("paged_evict")) return rc;                                                             \
+  } while (0)
+    WZ_EVICT(0);
+    WZ_EVICT(1);
+    WZ_EVICT(2);
+    WZ_EVICT(3);
+    WZ_EVICT(4);
+    WZ_EVICT(5);
+#undef WZ_EVICT
+  }
+  const int64_t blocks = std::min<int64_t>(std::max<int64_t>(1, (z.moves * (row_bytes / 16) + 255) / 256),
+                                           std::max<int64_t>(1, 4096 / z.units));
+  WZ_LAUNCH("paged_evict_move", stream, paged_evict_move_kernel, dim3(unsigned(blocks), units), dim3(256), 0, a,
+            row_bytes);
   return check_launch("paged_evict");
 }

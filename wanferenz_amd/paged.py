@@ -29,6 +29,8 @@ import torch
 from . import _native as N
 
 _E4M3 = torch.float8_e4m3fn
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _I64x3 = ctypes.c_int64 * 3
 
 
@@ -88,6 +90,9 @@ class PagedKV:
                       self.page_size, self.kv_heads, self.head_dim, N.WZ_KV_E4M3 if quantised else N.WZ_KV_BF16)
         self._desc = d
         self._ref = ctypes.byref(d)
+        lib = N.lib()
+        self._entry = {n: getattr(lib, n) for n in ("wz_paged_kv_write", "wz_paged_attn", "wz_paged_evict")}
+        self._sizes = {}
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, *, dtype=torch.bfloat16, shared=False, track=False,
@@ -107,19 +112,21 @@ class PagedKV:
                    v_scale=slots() if q and not shared else None, weights=slots() if track else None,
                    positions=slots(torch.int32) if track else None)
 
-    # ---- checks ----
+    # ---- checks (a decode step makes three calls for each layer: one pass over what can be wrong) ----
 
-    def _ints(self, what, name, t, shape):
-        if t.dtype != torch.int32 or t.shape != shape:
-            raise ValueError(f"{what}: {name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    def _ints(self, what, name, t, b):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != b:
+            raise ValueError(f"{what}: {name} must be int32 {[b]}, got {t.dtype} {list(t.shape)}")
         if t.device != self.device:
             raise ValueError(f"{what}: {name} is on {t.device}, the cache on {self.device}")
         return t if t.is_contiguous() else t.contiguous()
 
     def _table(self, what, t, b):
-        if t.dim() != 2:
-            raise ValueError(f"{what}: table must be [sequences, pages], got {list(t.shape)}")
-        return self._ints(what, "table", t, (b, t.shape[1]))
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != b:
+            raise ValueError(f"{what}: table must be int32 [{b}, pages], got {t.dtype} {list(t.shape)}")
+        if t.device != self.device:
+            raise ValueError(f"{what}: table is on {t.device}, the cache on {self.device}")
+        return t if t.is_contiguous() else t.contiguous()
 
     def _rows(self, what, name, t):
         """t as bf16 rows [.., .., .., D] that the kernels read in place: dense in their last dimension
@@ -129,23 +136,27 @@ class PagedKV:
         if t.device != self.device:
             raise ValueError(f"{what}: {name} is on {t.device}, the cache on {self.device}")
         sb, ss, sh, sd = t.stride()
-        if sd != 1 or (sb | ss | sh) & 7 or t.data_ptr() & 15:
-            t = t.contiguous()
-            sb, ss, sh, sd = t.stride()
-            if t.data_ptr() & 15 or (sb | ss | sh) & 7:  # a contiguous view may still begin between 16-byte units
-                t = t.clone(memory_format=torch.contiguous_format)
-                sb, ss, sh, sd = t.stride()
+        if sd != 1 or (sb | ss | sh | t.data_ptr() >> 1) & 7:
+            t = t.clone(memory_format=torch.contiguous_format)
+            sb, ss, sh, _ = t.stride()
         return t, _I64x3(sb, ss, sh)
 
     def _call(self, name, *args):
-        if torch.cuda.current_device() == self.device.index:
-            N.call(name, self._ref, *args, N.stream_handle(self.device))
+        index = self.device.index
+        if _current_device() == index:
+            rc = self._entry[name](self._ref, *args, _raw_stream(index))
         else:
-            with torch.cuda.device(self.device):
-                N.call(name, self._ref, *args, N.stream_handle(self.device))
+            with torch.cuda.device(index):
+                rc = self._entry[name](self._ref, *args, _raw_stream(index))
+        if rc:
+            N.check(rc, name)
 
-    def _space(self, what, workspace, need):
+    def _space(self, what, workspace, size, *shape):
+        """The caller's workspace, or a new one of size(*shape) bytes."""
         if workspace is None:
+            need = self._sizes.get(shape)
+            if need is None:
+                need = self._sizes[shape] = size(*shape)
             return torch.empty(need, dtype=torch.uint8, device=self.device)
         if workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
             raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor on {self.device}")
@@ -160,19 +171,20 @@ class PagedKV:
         weight 0 and the position ``position[b] + i`` (its slot number without ``position``: give it once a
         cache has been cut).  Slots that the table has no page for are dropped.  A slot must be written once
         in a call."""
-        if k.dim() != 4 or k.shape[2] != self.kv_heads or k.shape[3] != self.head_dim:
+        shape = k.shape
+        if len(shape) != 4 or shape[2] != self.kv_heads or shape[3] != self.head_dim:
             raise ValueError(f"PagedKV.write: k must be [b, s, {self.kv_heads}, {self.head_dim}], got {list(k.shape)}")
         if (v is None) != (self.v is None):
             raise ValueError("PagedKV.write: v is given where the cache has a v")
-        if v is not None and v.shape != k.shape:
+        if v is not None and v.shape != shape:
             raise ValueError(f"PagedKV.write: v {list(v.shape)} does not match k {list(k.shape)}")
-        b, s = k.shape[:2]
+        b, s = shape[0], shape[1]
         table = self._table("PagedKV.write", table, b)
-        start = self._ints("PagedKV.write", "start", start, (b,))
+        start = self._ints("PagedKV.write", "start", start, b)
         if count is not None:
-            count = self._ints("PagedKV.write", "count", count, (b,))
+            count = self._ints("PagedKV.write", "count", count, b)
         if position is not None:
-            position = self._ints("PagedKV.write", "position", position, (b,))
+            position = self._ints("PagedKV.write", "position", position, b)
         k, ks = self._rows("PagedKV.write", "k", k)
         v, vs = (None, None) if v is None else self._rows("PagedKV.write", "v", v)
         self._call("wz_paged_kv_write", k.data_ptr(), ks, N.ptr(v), vs, table.data_ptr(), table.shape[1],
@@ -192,7 +204,7 @@ class PagedKV:
             raise ValueError(f"PagedKV.attend: q must be [b, s, h, {self.head_dim}], got {list(q.shape)}")
         b, s, h, d = q.shape
         table = self._table("PagedKV.attend", table, b)
-        lens = self._ints("PagedKV.attend", "lens", lens, (b,))
+        lens = self._ints("PagedKV.attend", "lens", lens, b)
         sink = None
         if attn_sink is not None:
             if attn_sink.shape != (h,) or attn_sink.dtype != torch.float32 or attn_sink.device != self.device:
@@ -205,8 +217,8 @@ class PagedKV:
               or not out.is_contiguous()):
             raise ValueError(f"PagedKV.attend: out must be contiguous bf16 {[b, s, h, d]} on {self.device}")
         width = table.shape[1]
-        workspace = self._space("PagedKV.attend", workspace,
-                                0 if workspace is not None else self.attend_workspace_bytes(b, s, h, width, accumulate))
+        workspace = self._space("PagedKV.attend", workspace, self.attend_workspace_bytes, b, s, h, width,
+                                bool(accumulate))
         self._call("wz_paged_attn", q.data_ptr(), qs, N.ptr(sink), table.data_ptr(), width, lens.data_ptr(),
                    out.data_ptr(), b, s, h, float(softmax_scale), int(accumulate), workspace.data_ptr(),
                    workspace.numel())
@@ -229,14 +241,13 @@ class PagedKV:
             raise ValueError("PagedKV.evict: the cache is not tracked (weights and positions)")
         b = lens.shape[0] if lens.dim() == 1 else -1
         table = self._table("PagedKV.evict", table, b)
-        lens = self._ints("PagedKV.evict", "lens", lens, (b,))
+        lens = self._ints("PagedKV.evict", "lens", lens, b)
         if out is None:
             out = torch.empty(b, dtype=torch.int32, device=self.device)
-        elif self._ints("PagedKV.evict", "out", out, (b,)) is not out:
+        elif self._ints("PagedKV.evict", "out", out, b) is not out:
             raise ValueError("PagedKV.evict: out must be contiguous")
         width = table.shape[1]
-        need = 0 if workspace is not None else self.evict_workspace_bytes(b, width, keep)
-        workspace = self._space("PagedKV.evict", workspace, need)
+        workspace = self._space("PagedKV.evict", workspace, self.evict_workspace_bytes, b, width, keep)
         self._call("wz_paged_evict", table.data_ptr(), width, lens.data_ptr(), out.data_ptr(), b, keep, first, recent,
                    workspace.data_ptr(), workspace.numel())
         return out
