@@ -1,24 +1,24 @@
 // Attention of a few new tokens over a paged cache: the kernel, compiled for bf16 and e4m3
 // rows by the two sources that include it.
 //
-// One KV head's rows of queries (the S tokens' heads that share it, R = S H / kv_heads of them)
-// are taken in groups of 16 RT; a group of a sequence is a unit, and its n cached tokens are
-// `granules` of 32 NW.  All units' granules in a row are cut into one equal share per workgroup, so
-// the chip is filled whatever the lengths: a unit inside one share is finished there, a cut one
-// leaves (m, l, O) partials that paged_attn_join_kernel merges.  A workgroup's share holds at most
-// two cut units, its first and its last, which own its partial slots 2w and 2w + 1.
+// One KV head's rows of queries (the S tokens' heads that share it, R = S H / kv_heads of them) are
+// taken in groups of up to 64; a group of a sequence is a unit, and its n cached tokens are granules
+// of 32.  All units' granules in a row are cut into one equal share per worker, so the chip is filled
+// whatever the lengths: a unit inside one share is finished there, a cut one leaves (m, l, O) partials
+// that paged_attn_join_kernel merges.  A worker's share holds at most two cut units, its first and its
+// last, which own its partial slots 2w and 2w + 1.
 //
-// Inside a share every wave works by itself on each NW-th tile of 32 tokens, with its own ring of
-// NS tiles in LDS that the loads fill directly (no registers, no barriers):
+// A worker is one wave, or two that split 64 rows (RH = 2) and the loads.  One wave waits for nobody:
+// while it begins a unit or ends one, the compute unit's other workers keep loading.  Tiles of 32 tokens
+// go through a ring of NS in LDS that the loads fill directly, without registers:
 //   * S^T = K Q^T and O^T += V^T P^T with V_MFMA_F32_16X16X32; lane (row n, group g) of S^T
 //     holds tokens 4g + i and 16 + 4g + i, which are the k slots of its P operand, so P never
 //     leaves the lane and the softmax statistics are one register a row tile;
 //   * y = q . k scale log2(e), p = 2^(y - m), m moved only when a tile's maximum exceeds it by more
 //     than 8 (the final quotient does not depend on m); p is rounded to bf16 for the product with V
-//     (the sums keep it in 32 bits), which adds as much error as the output's own rounding;
-//   * the waves' (m, l, O) meet in LDS when the unit's part is done.
+//     (the sums keep it in 32 bits), which adds as much error as the output's own rounding.
 // Reading the cache bounds it: 4 R / element-size flops a byte is far below the matrix units' rate
-// for the usual group sizes.
+// for the usual group sizes.  Latents of 512 have a kernel of their own (paged_latent.h).
 #pragma once
 
 #include <algorithm>
@@ -48,10 +48,10 @@ struct PagedAttnArgs {
   const int32_t* table;
   const int32_t* lens;
   uint16_t* o;
-  float* part;    // 2 W slots of (m, l)[16 RT] and O[16 RT][D]
+  float* part;    // 2 W slots of m[rows], l[rows] and O[rows][D]
   float* ml;      // accumulate: per unit and row the final maximum and 1 / sum
   float* scores;  // accumulate: y [B, heads, R, capacity]
-  int width, B, S, H, W;
+  int width, B, S, H, W, rows;  // rows: of a partial, min(R, the unit's)
   int64_t capacity;  // slots of the table, width * page
   float scale2;      // softmax scale * log2(e)
 };
@@ -156,54 +156,91 @@ __device__ __forceinline__ pv8s paged_widen(int lo, int hi) {
   return u.v;
 }
 
+// One row of Q (bf16) against one row of the cache, this lane group's share g of the products; the rest of
+// the row is with the lanes 16 apart.  For the few tokens that not every row sees: Q is read again.
+template <int D, bool FP8>
+__device__ __forceinline__ float paged_dot(const uint16_t* qrow, const uint8_t* krow, int g) {
+  float dot = 0.0f;
+#pragma unroll 2
+  for (int cc = 0; cc < D / 32; ++cc) {
+    const int d = 32 * cc + 8 * g;
+    const pv8s q = *reinterpret_cast<const pv8s*>(qrow + d);
+    pv8s k;
+    if constexpr (FP8) {
+      const pv2i c8 = *reinterpret_cast<const pv2i*>(krow + d);
+      k = paged_widen(c8[0], c8[1]);
+    } else {
+      k = *reinterpret_cast<const pv8s*>(krow + 2 * d);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dot = fmaf(bf16_to_f32(uint16_t(k[i])), bf16_to_f32(uint16_t(q[i])), dot);
+  }
+  dot += __shfl_xor(dot, 16, 64);
+  dot += __shfl_xor(dot, 32, 64);
+  return dot;
+}
+
+// Four neighbouring values of a row, from column d on.
+template <bool FP8>
+__device__ __forceinline__ v4f paged_four(const uint8_t* row, int d) {
+  if constexpr (FP8) {
+    const int c = *reinterpret_cast<const int*>(row + d);
+    return v4f{__builtin_amdgcn_cvt_f32_fp8(c, 0), __builtin_amdgcn_cvt_f32_fp8(c, 1), __builtin_amdgcn_cvt_f32_fp8(c, 2),
+               __builtin_amdgcn_cvt_f32_fp8(c, 3)};
+  } else {
+    const uint2 c = *reinterpret_cast<const uint2*>(row + 2 * d);
+    return v4f{bf16lo(c.x), bf16hi(c.x), bf16lo(c.y), bf16hi(c.y)};
+  }
+}
+
 // Sizes of one compiled kernel.
-template <int D, bool FP8, bool SHARED, int RT>
+template <int D, bool FP8, bool SHARED, int RT, int RH>
 struct PagedCfg {
-  static constexpr int ESZ = FP8 ? 1 : 2;
-  static constexpr int RB = D * ESZ;
-  static constexpr int TILE = kPagedTile * RB;                    // one side of a tile
-  static constexpr int STAGE = TILE * (SHARED ? 1 : 2);
-  static constexpr int SCALES = FP8 ? 256 : 0;                    // a tile's K and V scales
-  static constexpr int NW = STAGE >= 32768 ? 2 : 4;               // waves
-  static constexpr int WAVE = NW == 2 ? 65536 : 32768;            // ring bytes a wave
-  static constexpr int NS = WAVE / STAGE > 4 ? 4 : WAVE / STAGE;  // tiles in the ring
-  static constexpr int LOADS = STAGE / 1024 + (FP8 ? 1 : 0);      // loads a tile
-  static constexpr int G = kPagedTile * NW;                       // tokens of a granule
-  static constexpr int ROWS = 16 * RT;
-  static constexpr int MERGE = ROWS * D * 4;                      // a wave's O in LDS
-  static constexpr int RING = NS * (STAGE + SCALES) > MERGE ? NS * (STAGE + SCALES) : MERGE;
-  static constexpr int SMALL = NW * ROWS * 8 + NW * NS * 4;       // (m, l) of the waves, valid masks
-  static constexpr int LDS = NW * RING + SMALL;
-  static constexpr int64_t SLOT = int64_t(ROWS) * (D + 2);        // floats of a partial
+  static constexpr int RB = D * (FP8 ? 1 : 2);
+  static constexpr int SIDE = kPagedTile * RB;                 // one side of a tile
+  static constexpr int STAGE = SIDE * (SHARED ? 1 : 2);
+  static constexpr int SCALES = FP8 ? 256 : 0;                 // a tile's K and V scales
+  static constexpr int NS = STAGE <= 4096 ? 4 : 2;
+  static constexpr int LOADS = STAGE / 1024 / RH + (FP8 ? 1 : 0);  // a wave's loads of a tile
+  static constexpr int WROWS = 16 * RT;                        // rows of a wave
+  static constexpr int ROWS = WROWS * RH;                      // rows of a unit
+  static constexpr int RING = NS * (STAGE + SCALES);
+  static constexpr int LDS = RING + RH * NS * 4;               // valid masks
+  // waves a SIMD: O and Q take 3 RT D / 8 registers of a lane
+  static constexpr int EU = 3 * RT * D / 8 <= 112 ? 2 : 1;
+  static constexpr int PER_CU = 160 * 1024 / LDS < 4 * EU / RH ? 160 * 1024 / LDS : 4 * EU / RH;
   static_assert(NS >= 2 && (NS - 1) * LOADS < 64, "the waits count the loads in flight");
+  static_assert(PER_CU >= 1 && SIDE / 1024 % RH == 0, "a worker fits, and its waves share a tile's loads evenly");
 };
 
-template <int D, bool FP8, bool SHARED, int RT>
-__global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void paged_attn_kernel(PagedAttnArgs a) {
-  using C = PagedCfg<D, FP8, SHARED, RT>;
+template <int D, bool FP8, bool SHARED, int RT, int RH>
+__global__ __launch_bounds__(64 * RH, (PagedCfg<D, FP8, SHARED, RT, RH>::EU))
+void paged_attn_kernel(PagedAttnArgs a) {
+  using C = PagedCfg<D, FP8, SHARED, RT, RH>;
   using L = PagedRow<C::RB>;
-  constexpr int NW = C::NW, NS = C::NS, RB = C::RB, ROWS = C::ROWS;
+  constexpr int NS = C::NS, RB = C::RB, ROWS = C::ROWS;
   constexpr int KC = D / 32, NT = D / 16;
   extern __shared__ __align__(1024) uint8_t lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, rh = RH == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nl = lane & 15, g = lane >> 4;
-  uint8_t* const ring = lds + wave * C::RING;
+  uint8_t* const ring = lds;
   uint8_t* const scales = ring + NS * C::STAGE;  // e4m3: 256 bytes a tile
-  float* const s_m = reinterpret_cast<float*>(lds + NW * C::RING);  // [wave][row]
-  float* const s_l = s_m + NW * ROWS;
-  uint32_t* const s_valid = reinterpret_cast<uint32_t*>(s_l + NW * ROWS) + wave * NS;
+  uint32_t* const s_valid = reinterpret_cast<uint32_t*>(lds + C::RING) + rh * NS;
   const uint32_t ring_lds = lds_addr(ring), scales_lds = lds_addr(scales);
+  auto meet = [&]() {  // the worker's waves; loads stay in flight
+    if constexpr (RH > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
 
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
   const int w = blockIdx.x;
-  const int64_t total = paged_uniform(paged_total<C::G>(a, upb));
+  const int64_t total = paged_uniform(paged_total<kPagedTile>(a, upb));
   const int W = paged_workers(total, a.W);
   if (w >= W) return;
   int64_t x = paged_uniform(paged_share(total, W, w));
   const int64_t x_end = paged_uniform(paged_share(total, W, w + 1));
   int b;
   int64_t before;
-  paged_find<C::G>(a, upb, x, &b, &before);
+  paged_find<kPagedTile>(a, upb, x, &b, &before);
   b = __builtin_amdgcn_readfirstlane(b);
   before = paged_uniform(before);
   int n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
@@ -211,19 +248,20 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
   const int ish = page >= kPagedTile ? 0 : 1;  // page ids a tile: 1 or 2
 
   for (bool first_piece = true; x < x_end; first_piece = false) {
-    int gran = (n + C::G - 1) / C::G;
+    int gran = (n + kPagedTile - 1) / kPagedTile;
     while (x >= before + int64_t(gran) * upb) {  // the next sequence that holds anything
       before += int64_t(gran) * upb;
       ++b;
       n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-      gran = (n + C::G - 1) / C::G;
+      gran = (n + kPagedTile - 1) / kPagedTile;
     }
     const int u = __builtin_amdgcn_readfirstlane(int((x - before) / gran));  // unit of the sequence
     const int64_t ubeg = before + int64_t(u) * gran;
     const int g0 = int(x - ubeg), g1 = int(min(x_end - ubeg, int64_t(gran)));
     const bool whole = g0 == 0 && g1 == gran;
     const int hk = __builtin_amdgcn_readfirstlane(u / RG), rg = u - hk * RG;
-    const int t0 = g0 * C::G, t1 = min(g1 * C::G, n);
+    const int row0 = rg * ROWS + rh * C::WROWS;  // this wave's first row
+    const int t0 = g0 * kPagedTile, t1 = min(g1 * kPagedTile, n);
     // the last S - 1 tokens are seen by some rows only: they are added one by one below
     const int tm = min(t1, max(n - a.S + 1, t0));
     const int32_t* const trow = a.table + int64_t(b) * a.width;
@@ -233,7 +271,7 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
     pv8s qf[RT][KC];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int r = min(rg * ROWS + 16 * rt + nl, R - 1);
+      const int r = min(row0 + 16 * rt + nl, R - 1);
       const uint16_t* const qrow = a.q + b * a.qb + (r / grp) * a.qs + (hk * grp + r % grp) * a.qh;
 #pragma unroll
       for (int cc = 0; cc < KC; ++cc) {
@@ -251,22 +289,21 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
       for (int nt = 0; nt < NT; ++nt) acc[rt][nt] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    // ---- this wave's tiles: t0 + 32 (wave + NW k), k < nk ----
-    const int ntile = (tm - t0 + kPagedTile - 1) / kPagedTile;
-    const int nk = max(0, (ntile - wave + NW - 1) / NW);
+    // ---- the tiles t0 + 32 k, k < nk ----
+    const int nk = (tm - t0 + kPagedTile - 1) / kPagedTile;
     // page ids of the next 64 >> ish tiles, lane e: tile base + (e >> ish), part e & ish
     int ids = -1, ids_base = 0;
     auto fetch_ids = [&](int k0) {
       ids_base = k0;
       const int k = k0 + (lane >> ish);
-      const int t = t0 + kPagedTile * (wave + NW * k) + ((lane & ish) << 4);
+      const int t = t0 + kPagedTile * k + ((lane & ish) << 4);
       int id = -1;
       if (k < nk && t < tm) id = trow[t >> ps];
       ids = uint32_t(id) < uint32_t(a.c.pages) ? id : -1;
     };
     auto issue = [&](int k, int stage) {
       if (((k - ids_base) << ish) >= 64) fetch_ids(k);
-      const int t = t0 + kPagedTile * (wave + NW * k);
+      const int t = t0 + kPagedTile * k;
       const int e = (k - ids_base) << ish;
       int id[2];
       id[0] = __builtin_amdgcn_readlane(ids, e);
@@ -285,15 +322,17 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
 #pragma unroll
       for (int side = 0; side < (SHARED ? 1 : 2); ++side) {
         const uint8_t* const pool = side ? a.c.v : a.c.k;
+        constexpr int N = C::SIDE / 1024 / RH;  // consecutive loads of each of the waves that share the tile
 #pragma unroll
-        for (int j = 0; j < kPagedTile / L::RPI; ++j) {
+        for (int jj = 0; jj < N; ++jj) {
+          const int j = rh * N + jj;
           constexpr int HALF = 16 / L::RPI > 0 ? 16 / L::RPI : 1;  // loads of half a tile
           const int half = j / HALF, r = (j % HALF) * L::RPI;
           const uint32_t voff = uint32_t(rin * RB + ((slot ^ L::swz(r + rin)) << 4));
-          paged_load16(pool + (row[half] + r) * RB, voff, dst + side * C::TILE + j * 1024);
+          paged_load16(pool + ((half ? row[1] : row[0]) + r) * RB, voff, dst + side * C::SIDE + j * 1024);
         }
       }
-      if constexpr (FP8) {
+      if constexpr (FP8) {  // (each wave of the worker loads them: the same bytes)
         const int tok = lane & 31;
         const int64_t at = tok < 16 ? row[0] + tok : row[1] + tok - 16;
         paged_load4((lane < 32 ? a.c.ks : a.c.vs) + at,
@@ -309,16 +348,22 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
     int stage = 0;
 #pragma unroll 1
     for (int k = 0; k < nk; ++k) {
+      // the tile before has been read out of its stage, by every wave of the worker
+      if constexpr (RH > 1) meet();
+      else __builtin_amdgcn_s_waitcnt(lgkmcnt_only(0));
       if (k + NS - 1 < nk) {
-        __builtin_amdgcn_s_waitcnt(lgkmcnt_only(0));  // the tile before has been read out of its stage
         issue(k + NS - 1, stage == 0 ? NS - 1 : stage - 1);
         __builtin_amdgcn_s_waitcnt(vmcnt_only((NS - 1) * C::LOADS));
       } else {
         __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
       }
-      asm volatile("" ::: "memory");
+      if constexpr (RH > 1) {
+        meet();  // and every wave's part of this one has landed
+      } else {
+        asm volatile("" ::: "memory");
+      }
       uint8_t* const kt = ring + stage * C::STAGE;
-      uint8_t* const vt = SHARED ? kt : kt + C::TILE;
+      uint8_t* const vt = SHARED ? kt : kt + C::SIDE;
       const uint32_t valid = __builtin_amdgcn_readfirstlane(s_valid[stage]);
       if (valid != 0xFFFFFFFFu) {
         // rows that hold nothing become zeros, whatever bits their memory has
@@ -385,7 +430,7 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         if (a.scores) {
-          const int r = rg * ROWS + 16 * rt + nl, t = t0 + kPagedTile * (wave + NW * k) + 4 * g;
+          const int r = row0 + 16 * rt + nl, t = t0 + kPagedTile * k + 4 * g;
           if (r < R) {
             float* const row = a.scores + ((int64_t(b) * a.c.heads + hk) * R + r) * a.capacity;
 #pragma unroll
@@ -452,9 +497,9 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
       stage = stage + 1 == NS ? 0 : stage + 1;
     }
 
-    // ---- the tokens that only some rows see, by the first wave: a row takes nothing, not even a
-    // NaN, from a token it does not see ----
-    if (wave == 0) {
+    // ---- the tokens that only some rows see: a row takes nothing, not even a NaN, from one that it
+    // does not see ----
+    {
       for (int t = tm; t < t1; ++t) {
         const int64_t at = paged_row(a.c, trow, a.width, hk, t);
         if (at < 0) continue;
@@ -463,23 +508,10 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
         const float ksc = FP8 ? a.c.ks[at] : 1.0f, vsc = FP8 ? a.c.vs[at] : 1.0f;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          float dot = 0.0f;
-#pragma unroll
-          for (int cc = 0; cc < KC; ++cc) {
-            pv8s kf;
-            if constexpr (!FP8) {
-              kf = *reinterpret_cast<const pv8s*>(kr + (32 * cc + 8 * g) * 2);
-            } else {
-              const pv2i c8 = *reinterpret_cast<const pv2i*>(kr + 64 * (cc >> 1) + 16 * g + 8 * (cc & 1));
-              kf = paged_widen(c8[0], c8[1]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dot = fmaf(bf16_to_f32(uint16_t(kf[i])), bf16_to_f32(uint16_t(qf[rt][cc][i])), dot);
-          }
-          dot += __shfl_xor(dot, 16, 64);
-          dot += __shfl_xor(dot, 32, 64);
-          const int r = rg * ROWS + 16 * rt + nl;
+          const int rq = min(row0 + 16 * rt + nl, R - 1);
+          const float dot =
+              paged_dot<D, FP8>(a.q + b * a.qb + (rq / grp) * a.qs + (hk * grp + rq % grp) * a.qh, kr, g);
+          const int r = row0 + 16 * rt + nl;
           const bool sees = r < R && t < n - (a.S - 1 - r / grp);
           const float y = FP8 ? dot * ksc * a.scale2 : dot * a.scale2;
           if (a.scores && r < R && g == 0)
@@ -493,193 +525,214 @@ __global__ __launch_bounds__((64 * PagedCfg<D, FP8, SHARED, RT>::NW), 1) void pa
             l_run[rt] = l_run[rt] * resc + (g == 0 ? p : 0.0f);
             const float pv = p * vsc;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              const v4f v = paged_four<FP8>(vr, 16 * nt + 4 * g);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int d = 16 * nt + 4 * g + i;
-                float v;
-                if constexpr (!FP8)
-                  v = bf16_to_f32(reinterpret_cast<const uint16_t*>(vr)[d]);
-                else
-                  v = __builtin_amdgcn_cvt_f32_fp8(vr[d], 0);
-                acc[rt][nt][i] = fmaf(pv, v, acc[rt][nt][i] * resc);
-              }
+              for (int i = 0; i < 4; ++i) acc[rt][nt][i] = fmaf(pv, v[i], acc[rt][nt][i] * resc);
+            }
           }
         }
       }
     }
 
-    // ---- the waves' parts meet ----
-    __builtin_amdgcn_s_waitcnt(0);
+    // ---- the part's end ----
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       l_run[rt] += __shfl_xor(l_run[rt], 16, 64);
       l_run[rt] += __shfl_xor(l_run[rt], 32, 64);
-      if (g == 0) {
-        s_m[wave * ROWS + 16 * rt + nl] = m_run[rt];
-        s_l[wave * ROWS + 16 * rt + nl] = l_run[rt];
-      }
     }
-    __syncthreads();
+    {
+      float* const part = a.part + (first_piece ? 2 * int64_t(w) : 2 * int64_t(w) + 1) * (int64_t(a.rows) * (D + 2));
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = 16 * rt + nl;
-      float M = -INFINITY;
-      for (int i = 0; i < NW; ++i) M = fmaxf(M, s_m[i * ROWS + r]);
-      const float f = m_run[rt] == -INFINITY && M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[rt] - M);
+      for (int rt = 0; rt < RT; ++rt) {
+        const int rl = rh * C::WROWS + 16 * rt + nl, r = rg * ROWS + rl;
+        if (r >= R) continue;
+        if (whole) {
+          const int head = hk * grp + r % grp, s = r / grp;
+          float den = l_run[rt], f = 1.0f, M = m_run[rt];
+          if (a.sink) {
+            const float sk = a.sink[head] * kLog2e;
+            M = fmaxf(M, sk);
+            const float Me = M == -INFINITY ? 0.0f : M;
+            f = m_run[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[rt] - Me);
+            den = den * f + __builtin_amdgcn_exp2f(sk - Me);
+          }
+          const float inv = den == 0.0f ? 0.0f : f / den;
+          uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D + 4 * g;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        *reinterpret_cast<v4f*>(ring + r * (D * 4) + (((4 * nt + g) ^ nl) << 4)) = acc[rt][nt] * f;
-    }
-    __syncthreads();
-    // row r, four columns a thread
-    float* const part = a.part + (first_piece ? 2 * int64_t(w) : 2 * int64_t(w) + 1) * C::SLOT;
-    for (int i = tid; i < ROWS * (D / 4); i += 64 * NW) {
-      const int r = i / (D / 4), ch = i % (D / 4);
-      const int rr = rg * ROWS + r;
-      if (rr >= R) continue;
-      float M = -INFINITY, l = 0.0f;
-      for (int j = 0; j < NW; ++j) M = fmaxf(M, s_m[j * ROWS + r]);
-      for (int j = 0; j < NW; ++j) {
-        const float m = s_m[j * ROWS + r];
-        l += s_l[j * ROWS + r] * (m == -INFINITY && M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M));
-      }
-      v4f o = v4f{0.f, 0.f, 0.f, 0.f};
-      for (int j = 0; j < NW; ++j)
-        o += *reinterpret_cast<const v4f*>(lds + j * C::RING + r * (D * 4) + ((ch ^ (r & 15)) << 4));
-      if (whole) {
-        const int head = hk * grp + rr % grp, s = rr / grp;
-        float den = l, f = 1.0f, Mf = M;
-        if (a.sink) {
-          const float sk = a.sink[head] * kLog2e;
-          Mf = fmaxf(M, sk);
-          const float Me = Mf == -INFINITY ? 0.0f : Mf;
-          f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Me);
-          den = l * f + __builtin_amdgcn_exp2f(sk - Me);
-        }
-        const float inv = den == 0.0f ? 0.0f : f / den;
-        uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D + ch * 4;
-        *reinterpret_cast<uint2*>(orow) =
-            make_uint2(f32x2_to_bf16x2(o[0] * inv, o[1] * inv), f32x2_to_bf16x2(o[2] * inv, o[3] * inv));
-        if (a.ml && ch == 0) {
-          float* const e = a.ml + 2 * ((int64_t(b) * a.c.heads + hk) * R + rr);
-          e[0] = Mf == -INFINITY ? 0.0f : Mf;
-          e[1] = den == 0.0f ? 0.0f : 1.0f / den;
-        }
-      } else {
-        *reinterpret_cast<v4f*>(part + 2 * ROWS + r * D + ch * 4) = o;
-        if (ch == 0) {
-          part[r] = M;
-          part[ROWS + r] = l;
+          for (int nt = 0; nt < NT; ++nt)
+            *reinterpret_cast<uint2*>(orow + 16 * nt) =
+                make_uint2(f32x2_to_bf16x2(acc[rt][nt][0] * inv, acc[rt][nt][1] * inv),
+                           f32x2_to_bf16x2(acc[rt][nt][2] * inv, acc[rt][nt][3] * inv));
+          if (a.ml && g == 0) {
+            float* const e = a.ml + 2 * ((int64_t(b) * a.c.heads + hk) * R + r);
+            e[0] = M == -INFINITY ? 0.0f : M;
+            e[1] = den == 0.0f ? 0.0f : 1.0f / den;
+          }
+        } else {
+          if (g == 0) {
+            part[rl] = m_run[rt];
+            part[a.rows + rl] = l_run[rt];
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            *reinterpret_cast<v4f*>(part + 2 * a.rows + rl * D + 16 * nt + 4 * g) = acc[rt][nt];
         }
       }
     }
-    __syncthreads();
+    meet();  // the ring is free for the next part's tiles
     x = ubeg + g1;
   }
 }
 
-// Merges a cut unit's partials, four rows a workgroup; a unit without tokens gets zeros.
-template <int D, int ROWS, int G>
+// Merges a cut unit's partials, a workgroup a row: every partial's (m, l) at once, then O with 256 / (D / 4)
+// partials in flight at a time.  A row without tokens gets zeros.
+constexpr int kPagedMaxWorkers = 4096;
+
+template <int D, int G, int ROWS>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
-  constexpr int64_t SLOT = int64_t(ROWS) * (D + 2);
+  __shared__ float s_f[kPagedMaxWorkers];
+  __shared__ float s_red[2][4];
+  __shared__ v4f s_o[256];
+  constexpr int CH = D / 4, GR = 256 / CH;
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
-  const int r4 = blockIdx.x % (ROWS / 4) * 4, unit = blockIdx.x / (ROWS / 4);
-  const int b = unit / upb, u = unit % upb, hk = u / RG, rg = u % RG;
-  if (rg * ROWS + r4 >= R) return;
+  const int bh = blockIdx.x / R, r = blockIdx.x - bh * R, b = bh / a.c.heads, hk = bh - b * a.c.heads;
+  const int u = hk * RG + r / ROWS, rl = r % ROWS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = paged_len(a, b), gran = (n + G - 1) / G;
-  const int64_t total = paged_total<G>(a, upb);
+  const int head = hk * grp + r % grp, s = r / grp;
+  uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D;
+  if (n == 0) {
+    if (tid < CH) *reinterpret_cast<uint2*>(orow + 4 * tid) = make_uint2(0, 0);
+    if (a.ml && tid == 0) {
+      float* const e = a.ml + 2 * (int64_t(bh) * R + r);
+      e[0] = e[1] = 0.0f;
+    }
+    return;
+  }
+  int64_t before = 0, total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int x = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
+    int all = x, lower = b0 + lane < b ? x : 0;
+    for (int o = 1; o < 64; o <<= 1) {
+      all += __shfl_xor(all, o, 64);
+      lower += __shfl_xor(lower, o, 64);
+    }
+    total += all;
+    before += lower;
+  }
+  total *= upb;
   const int W = paged_workers(total, a.W);
-  int w0 = 0, w1 = -1;
-  int64_t ubeg = 0;
-  if (n > 0) {
-    const int lane = threadIdx.x & 63;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < b; b0 += 64) {
-      int gs = b0 + lane < b ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
-      for (int o = 1; o < 64; o <<= 1) gs += __shfl_xor(gs, o, 64);
-      before += gs;
+  const int64_t ubeg = before * upb + int64_t(u) * gran;
+  const int w0 = paged_owner(total, W, ubeg), w1 = paged_owner(total, W, ubeg + gran - 1);
+  const int np = w1 - w0 + 1;
+  if (np == 1) return;  // finished by its worker
+  // the first one's part of the unit is its first if its share begins here, else its last
+  const int64_t slot = int64_t(a.rows) * (D + 2);
+  const float* const part = a.part + 2 * int64_t(w0) * slot;
+  const int64_t step0 = paged_share(total, W, w0) >= ubeg ? 0 : slot;
+  auto at = [&](int j) { return part + (j == 0 ? step0 : 2 * int64_t(j) * slot); };
+  const float sk = a.sink ? a.sink[head] * kLog2e : -INFINITY;
+  float M = sk, m[kPagedMaxWorkers / 256], l[kPagedMaxWorkers / 256];
+#pragma unroll
+  for (int i = 0; i < kPagedMaxWorkers / 256; ++i) {
+    const int j = i * 256 + tid;
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+    if (j < np) {
+      m[i] = at(j)[rl];
+      l[i] = at(j)[a.rows + rl];
     }
-    ubeg = before * upb + int64_t(u) * gran;
-    w0 = paged_owner(total, W, ubeg);
-    w1 = paged_owner(total, W, ubeg + gran - 1);
-    if (w0 == w1) return;  // finished by its workgroup
+    M = fmaxf(M, m[i]);
+    if ((i + 1) * 256 >= np) break;
   }
-  const int64_t slot0 = n > 0 ? 2 * int64_t(w0) + (paged_share(total, W, w0) >= ubeg ? 0 : 1) : 0;
-  for (int i = threadIdx.x; i < 4 * (D / 4); i += 256) {
-    const int r = r4 + i / (D / 4), ch = i % (D / 4), rr = rg * ROWS + r;
-    if (rr >= R) continue;
-    const int head = hk * grp + rr % grp, s = rr / grp;
-    const float sk = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-    float M = sk;
-    for (int w = w0; w <= w1; ++w) M = fmaxf(M, a.part[(w == w0 ? slot0 : 2 * int64_t(w)) * SLOT + r]);
-    const float Me = M == -INFINITY ? 0.0f : M;
-    float den = a.sink ? __builtin_amdgcn_exp2f(sk - Me) : 0.0f;
-    v4f o = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int w = w0; w <= w1; ++w) {
-      const float* const p = a.part + (w == w0 ? slot0 : 2 * int64_t(w)) * SLOT;
-      const float f = __builtin_amdgcn_exp2f(p[r] - Me);
-      den += f * p[ROWS + r];
-      o += *reinterpret_cast<const v4f*>(p + 2 * ROWS + r * D + ch * 4) * f;
+  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  if (lane == 0) s_red[0][wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+  const float Me = M == -INFINITY ? 0.0f : M;
+  float den = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPagedMaxWorkers / 256; ++i) {
+    const int j = i * 256 + tid;
+    if (j < np) {
+      const float f = __builtin_amdgcn_exp2f(m[i] - Me);
+      s_f[j] = f;
+      den += f * l[i];
     }
-    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-    uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D + ch * 4;
-    *reinterpret_cast<uint2*>(orow) =
-        make_uint2(f32x2_to_bf16x2(o[0] * inv, o[1] * inv), f32x2_to_bf16x2(o[2] * inv, o[3] * inv));
-    if (a.ml && ch == 0) {
-      float* const e = a.ml + 2 * ((int64_t(b) * a.c.heads + hk) * R + rr);
-      e[0] = Me;
-      e[1] = inv;
-    }
+    if ((i + 1) * 256 >= np) break;
+  }
+  for (int o = 1; o < 64; o <<= 1) den += __shfl_xor(den, o, 64);
+  if (lane == 0) s_red[1][wave] = den;
+  __syncthreads();
+  den = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  if (a.sink) den += __builtin_amdgcn_exp2f(sk - Me);
+  const int ch = tid % CH, gr = tid / CH;
+  v4f o = v4f{0.f, 0.f, 0.f, 0.f};
+  const int64_t off = 2 * a.rows + rl * D + 4 * ch;
+#pragma unroll 4
+  for (int j = gr; j < np; j += GR) o += *reinterpret_cast<const v4f*>(at(j) + off) * s_f[j];
+  s_o[tid] = o;
+  __syncthreads();
+  if (tid >= CH) return;
+#pragma unroll
+  for (int i = 1; i < GR; ++i) o += s_o[i * CH + tid];
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  *reinterpret_cast<uint2*>(orow + 4 * tid) =
+      make_uint2(f32x2_to_bf16x2(o[0] * inv, o[1] * inv), f32x2_to_bf16x2(o[2] * inv, o[3] * inv));
+  if (a.ml && tid == 0) {
+    float* const e = a.ml + 2 * (int64_t(bh) * R + r);
+    e[0] = Me;
+    e[1] = inv;
   }
 }
 
-// Row tiles of a unit: as many as hold the rows, up to what the registers hold.
-constexpr int paged_row_tiles(int D, int R) {
-  const int most = D <= 128 ? 4 : D == 256 ? 2 : 1;
-  const int want = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  return want < most ? want : most;
-}
-
-template <int D, bool FP8, bool SHARED, int RT>
-int paged_attn_launch_rt(PagedAttnArgs a, hipStream_t stream) {
-  using C = PagedCfg<D, FP8, SHARED, RT>;
+// The kernel of R rows a KV head: 16, 32 or 64 rows a unit.
+template <int D, bool FP8, bool SHARED, int RT, int RH>
+int paged_attn_launch_rt(PagedAttnArgs a, bool ask, int* workers, hipStream_t stream) {
+  using C = PagedCfg<D, FP8, SHARED, RT, RH>;
   static_assert(C::LDS <= 160 * 1024, "a workgroup's LDS");
-  static LdsGrant grant;
-  auto* const kernel = paged_attn_kernel<D, FP8, SHARED, RT>;
-  if (int rc = allow_lds("paged_attn", kernel, C::LDS, grant)) return rc;
-  WZ_LAUNCH("paged_attn", stream, kernel, dim3{unsigned(a.W)}, dim3(64 * C::NW), C::LDS, a);
-  if (int rc = check_launch("paged_attn")) return rc;
   const int R = a.S * (a.H / a.c.heads);
-  const int64_t units = int64_t(a.B) * a.c.heads * ((R + C::ROWS - 1) / C::ROWS);
-  auto* const join = paged_attn_join_kernel<D, C::ROWS, C::G>;
-  WZ_LAUNCH("paged_attn_join", stream, join, dim3{unsigned(units * (C::ROWS / 4))}, dim3(256), 0, a);
+  a.W = std::min(cu_count() * C::PER_CU, kPagedMaxWorkers);
+  a.rows = std::min(R, C::ROWS);
+  if (ask) {
+    *workers = a.W;
+    return a.rows;
+  }
+  static LdsGrant grant;
+  auto* const kernel = paged_attn_kernel<D, FP8, SHARED, RT, RH>;
+  if (int rc = allow_lds("paged_attn", kernel, C::LDS, grant)) return rc;
+  WZ_LAUNCH("paged_attn", stream, kernel, dim3{unsigned(a.W)}, dim3(64 * RH), C::LDS, a);
+  if (int rc = check_launch("paged_attn")) return rc;
+  auto* const join = paged_attn_join_kernel<D, kPagedTile, C::ROWS>;
+  WZ_LAUNCH("paged_attn_join", stream, join, dim3{unsigned(int64_t(a.B) * a.c.heads * R)}, dim3(256), 0, a);
   return check_launch("paged_attn_join");
 }
 
 template <int D, bool FP8, bool SHARED>
-int paged_attn_launch_d(const PagedAttnArgs& a, hipStream_t stream) {
-  const int rt = paged_row_tiles(D, a.S * (a.H / a.c.heads));
-  if constexpr (D <= 128)
-    if (rt == 4) return paged_attn_launch_rt<D, FP8, SHARED, 4>(a, stream);
-  if constexpr (D <= 256)
-    if (rt == 2) return paged_attn_launch_rt<D, FP8, SHARED, 2>(a, stream);
-  return paged_attn_launch_rt<D, FP8, SHARED, 1>(a, stream);
+int paged_attn_launch_d(const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
+  const int R = a.S * (a.H / a.c.heads);
+  if (R <= 16) return paged_attn_launch_rt<D, FP8, SHARED, 1, 1>(a, ask, workers, stream);
+  if (R <= 32) return paged_attn_launch_rt<D, FP8, SHARED, 2, 1>(a, ask, workers, stream);
+  return paged_attn_launch_rt<D, FP8, SHARED, 2, 2>(a, ask, workers, stream);
 }
 
+int paged_latent(bool fp8, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
+
+// Launches, or with `ask` -> the rows of a partial, and *workers.
 template <bool FP8>
-int paged_attn_launch(int D, const PagedAttnArgs& a, hipStream_t stream) {
+int paged_attn_launch(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
   if (a.c.shared) {
-    if (D == 128) return paged_attn_launch_d<128, FP8, true>(a, stream);
-    if (D == 256) return paged_attn_launch_d<256, FP8, true>(a, stream);
-    return paged_attn_launch_d<512, FP8, true>(a, stream);
+    if (D == 128) return paged_attn_launch_d<128, FP8, true>(a, ask, workers, stream);
+    if (D == 256) return paged_attn_launch_d<256, FP8, true>(a, ask, workers, stream);
+    return paged_latent(FP8, a, ask, workers, stream);
   }
-  if (D == 64) return paged_attn_launch_d<64, FP8, false>(a, stream);
-  if (D == 128) return paged_attn_launch_d<128, FP8, false>(a, stream);
-  return paged_attn_launch_d<256, FP8, false>(a, stream);
+  if (D == 64) return paged_attn_launch_d<64, FP8, false>(a, ask, workers, stream);
+  if (D == 128) return paged_attn_launch_d<128, FP8, false>(a, ask, workers, stream);
+  return paged_attn_launch_d<256, FP8, false>(a, ask, workers, stream);
 }
 
-int paged_attn_bf16(int D, const PagedAttnArgs& a, hipStream_t stream);
-int paged_attn_e4m3(int D, const PagedAttnArgs& a, hipStream_t stream);
+int paged_attn_bf16(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
+int paged_attn_e4m3(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
 
 }  // namespace wz

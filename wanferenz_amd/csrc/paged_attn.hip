@@ -3,7 +3,14 @@
 
 namespace wz {
 
-int paged_attn_bf16(int D, const PagedAttnArgs& a, hipStream_t stream) { return paged_attn_launch<false>(D, a, stream); }
+int paged_attn_bf16(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
+  return paged_attn_launch<false>(D, a, ask, workers, stream);
+}
+
+static int paged_attn_any(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
+  return a.c.dtype == WZ_KV_E4M3 ? paged_attn_e4m3(D, a, ask, workers, stream)
+                                 : paged_attn_bf16(D, a, ask, workers, stream);
+}
 
 // weights[slot] += sum over the KV head's rows that see the slot of 2^(y - m) / sum, rows in
 // ascending order.  A thread per slot; blockIdx.y = (sequence, head).
@@ -34,8 +41,15 @@ static PagedAttnSizes paged_attn_sizes(const wz_paged_kv* c, int64_t B, int64_t 
                                        bool accumulate) {
   PagedAttnSizes z{};
   const int64_t R = S * (H / c->kv_heads);
-  const int rows = 16 * paged_row_tiles(c->head_dim, int(R));
-  z.part = 2 * int64_t(cu_count()) * rows * (c->head_dim + 2);
+  PagedAttnArgs a{};
+  a.c.heads = c->kv_heads;
+  a.c.shared = c->v == nullptr;
+  a.c.dtype = c->dtype;
+  a.S = int(S);
+  a.H = int(H);
+  int workers = 0;
+  const int64_t rows = paged_attn_any(c->head_dim, a, true, &workers, nullptr);
+  z.part = (2 * workers * rows * (c->head_dim + 2) + 3) / 4 * 4;
   if (accumulate) {
     z.ml = (2 * B * c->kv_heads * R + 3) / 4 * 4;
     z.scores = B * c->kv_heads * R * width * c->page_size;
@@ -48,7 +62,9 @@ static PagedAttnSizes paged_attn_sizes(const wz_paged_kv* c, int64_t B, int64_t 
 extern "C" int64_t wz_paged_attn_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t S, int64_t H,
                                                  int64_t table_width, int accumulate) {
   using namespace wz;
-  if (!cache || cache->kv_heads <= 0 || B <= 0 || S <= 0 || S > kPagedMaxS || H <= 0 || H > 65536 || table_width <= 0)
+  PagedView view;
+  if (paged_view("paged_attn", cache, table_width, &view) != WZ_OK) return 0;
+  if (B <= 0 || S <= 0 || S > kPagedMaxS || H <= 0 || H > 65536 || H % view.heads)
     return 0;
   const PagedAttnSizes z = paged_attn_sizes(cache, B, S, H, table_width, accumulate != 0);
   return (z.part + z.ml + z.scores) * int64_t(sizeof(float));
@@ -75,8 +91,7 @@ extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const
        reinterpret_cast<uintptr_t>(workspace)) & 15 || ((q_strides[0] | q_strides[1] | q_strides[2]) & 7))
     return set_error(WZ_EINVAL, "paged_attn: q rows, o and the workspace must be 16-byte aligned");
   const int64_t R = S * (H / a.c.heads);
-  const int64_t units = B * a.c.heads * ((R + 15) / 16);
-  if (units * 16 > 0x7FFFFFFFLL || B * a.c.heads > 65535 * int64_t(accumulate ? 1 : 65535))
+  if (B * a.c.heads * R > 0x7FFFFFFFLL || B * a.c.heads > 65535 * int64_t(accumulate ? 1 : 65535))
     return set_error(WZ_EINVAL, "paged_attn: %lld sequences of %lld heads", (long long)B, (long long)H);
   if (2 * R * int64_t(sizeof(float)) > 65536)
     return set_error(WZ_EINVAL, "paged_attn: %lld query rows on a KV head", (long long)R);
@@ -100,10 +115,9 @@ extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const
   a.B = int(B);
   a.S = int(S);
   a.H = int(H);
-  a.W = cu_count();
   a.capacity = table_width * a.c.page;
   a.scale2 = softmax_scale * kLog2e;
-  const int rc = a.c.ks ? paged_attn_e4m3(cache->head_dim, a, stream) : paged_attn_bf16(cache->head_dim, a, stream);
+  const int rc = paged_attn_any(cache->head_dim, a, false, nullptr, stream);
   if (rc != WZ_OK || !accumulate || a.capacity == 0) return rc;
   const int64_t blocks = std::min<int64_t>((a.capacity + 255) / 256, 1024);
   WZ_LAUNCH("paged_attn_weigh", stream, paged_attn_weigh_kernel, dim3(unsigned(blocks), unsigned(B * a.c.heads)),

@@ -2,5 +2,7 @@
 #include "paged_attn.h"
 
 namespace wz {
-int paged_attn_e4m3(int D, const PagedAttnArgs& a, hipStream_t stream) { return paged_attn_launch<true>(D, a, stream); }
+int paged_attn_e4m3(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
+  return paged_attn_launch<true>(D, a, ask, workers, stream);
+}
 }  // namespace wz
