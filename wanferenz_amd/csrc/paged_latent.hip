@@ -26,19 +26,24 @@ struct LatentCfg {
   static constexpr int LOADS = RPW * RB / 1024;
 };
 
-template <bool FP8, int HT>
+// EXTRA: several new tokens, or weights to accumulate; without them 64 rows just fit the registers.
+template <bool FP8, int HT, bool EXTRA>
 __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(PagedAttnArgs a) {
   using C = LatentCfg<FP8>;
   using L = PagedRow<C::RB>;
   constexpr int D = kLatentD, RB = C::RB, ROWS = 16 * HT, T = kLatentTile;
   constexpr int KC = D / 32, NT = D / 16 / kLatentWaves;
   constexpr int SHT = HT == 4 ? 2 : 1;  // row tiles of S a wave
+  // the last KQ chunks of Q are read from LDS for each tile: with all of 64 rows in registers some were
+  // spilled, and a reload waits for the loads of the next tile (102 us, 268 MB; so: see below)
+  constexpr int KQ = HT == 4 ? 2 : 0;
   __shared__ __align__(1024) uint8_t kb[2][C::TILE];
   __shared__ __align__(16) uint8_t s_p[2][ROWS][64];  // [tokens / 32][row]: group g's 8 k slots at 16 g
   __shared__ float s_max[4][ROWS], s_l[4][ROWS];      // [token tile][row]
   __shared__ float s_scale[2][T], s_y[ROWS];
   __shared__ __align__(8) uint8_t s_valid[2][8];      // a bit a token
   __shared__ int s_bump[2];
+  __shared__ __align__(16) uint8_t s_q[KQ ? ROWS : 1][128];  // [row]: chunk KC - 2 + c, group g at (4 c + g) ^ swz(row)
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nl = lane & 15, g = lane >> 4;
@@ -76,19 +81,23 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
     const bool whole = g0 == 0 && g1 == gran;
     const int hk = __builtin_amdgcn_readfirstlane(u / RG), rg = u - hk * RG, row0 = rg * ROWS;
     const int t0 = g0 * T, t1 = min(g1 * T, n);
-    const int tm = min(t1, max(n - a.S + 1, t0));  // the last S - 1 tokens are added one by one below
+    const int tm = EXTRA ? min(t1, max(n - a.S + 1, t0)) : t1;  // the last S - 1 tokens are added one by one below
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
     // Q fragments (B operand of S^T): lane (row nl, group g); as in paged_attn_kernel
-    pv8s qb[SHT][KC];
+    pv8s qb[SHT][KC - KQ];
 #pragma unroll
     for (int h = 0; h < SHT; ++h) {
-      const int r = min(row0 + 16 * (has_s ? ht0 + h : 0) + nl, R - 1);
+      const int rl = 16 * (has_s ? ht0 + h : 0) + nl, r = min(row0 + rl, R - 1);
       const uint16_t* const qrow = a.q + b * a.qb + (r / grp) * a.qs + (hk * grp + r % grp) * a.qh;
 #pragma unroll
       for (int cc = 0; cc < KC; ++cc) {
         const int d = FP8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g;
-        qb[h][cc] = *reinterpret_cast<const pv8s*>(qrow + d);
+        const pv8s q = *reinterpret_cast<const pv8s*>(qrow + d);
+        if (cc < KC - KQ)
+          qb[h][cc] = q;
+        else if (rt == 0)
+          *reinterpret_cast<pv8s*>(&s_q[rl][(((cc - (KC - KQ)) * 4 + g) ^ PagedRow<128>::swz(rl)) << 4]) = q;
       }
     }
     v4f acc[HT][NT];  // acc[ht][nt][i] = O[row 16ht + nl][64 wave + 16nt + 4g + i]
@@ -148,8 +157,8 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       meet();                                     // ... and every wave's; the other buffer and s_p are free
       if (k + 1 < nk) issue(k + 1, buf ^ 1);
       uint8_t* const ks = kb[buf];
-      const uint64_t valid = *reinterpret_cast<const uint64_t*>(s_valid[buf]);
-      if (__builtin_amdgcn_readfirstlane(uint32_t(valid & (valid >> 32))) != 0xFFFFFFFFu) {
+      const uint64_t valid = uint64_t(paged_uniform(*reinterpret_cast<const int64_t*>(s_valid[buf])));
+      if (~valid) {
         // rows that hold nothing become zeros, whatever bits their memory has
         for (int i = tid; i < T * L::CH; i += 64 * kLatentWaves)
           if (!((valid >> (i / L::CH)) & 1)) *reinterpret_cast<v4i*>(ks + i * 16) = v4i{0, 0, 0, 0};
@@ -195,16 +204,21 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
           if (c + kAhead < NC) kload(c + kAhead);
           __builtin_amdgcn_sched_barrier(0);  // keep the reads ahead of their use
           const v4i kc = kf[c % (kAhead + 1)];
+          auto q_of = [&](int h, int cc) -> pv8s {
+            if (cc < KC - KQ) return qb[h][cc < KC - KQ ? cc : 0];
+            const int rl = 16 * (ht0 + h) + nl;
+            return *reinterpret_cast<const pv8s*>(&s_q[KQ ? rl : 0][(((cc - (KC - KQ)) * 4 + g) ^ PagedRow<128>::swz(rl)) << 4]);
+          };
           if constexpr (FP8) {
             const pv8s k0 = paged_widen(kc[0], kc[1]), k1 = paged_widen(kc[2], kc[3]);
 #pragma unroll
             for (int h = 0; h < SHT; ++h) {
-              y[h] = paged_mfma(k0, qb[h][2 * c], y[h]);
-              y[h] = paged_mfma(k1, qb[h][2 * c + 1], y[h]);
+              y[h] = paged_mfma(k0, q_of(h, 2 * c), y[h]);
+              y[h] = paged_mfma(k1, q_of(h, 2 * c + 1), y[h]);
             }
           } else {
 #pragma unroll
-            for (int h = 0; h < SHT; ++h) y[h] = paged_mfma(__builtin_bit_cast(pv8s, kc), qb[h][c], y[h]);
+            for (int h = 0; h < SHT; ++h) y[h] = paged_mfma(__builtin_bit_cast(pv8s, kc), q_of(h, c), y[h]);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -222,7 +236,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           bump |= top > m_s[h] + kPagedLazy;
           if (g == 0) s_max[rt][16 * (ht0 + h) + nl] = top;
-          if (a.scores) {
+          if (EXTRA && a.scores) {
             const int r = row0 + 16 * (ht0 + h) + nl, t = t0 + T * k + 16 * rt + 4 * g;
             if (r < R) {
               float* const out = a.scores + ((int64_t(b) * a.c.heads + hk) * R + r) * a.capacity + t;
@@ -324,7 +338,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
 
     // ---- the tokens that only some rows see: a row takes nothing, not even a NaN, from one that it
     // does not see ----
-    for (int t = tm; t < t1; ++t) {
+    for (int t = tm; EXTRA && t < t1; ++t) {
       const int64_t at = paged_row(a.c, trow, a.width, hk, t);
       if (at < 0) continue;  // the same in every wave
       const uint8_t* const kr = a.c.k + at * RB;
@@ -439,7 +453,10 @@ static int latent_launch(PagedAttnArgs a, bool ask, int* workers, hipStream_t st
     *workers = a.W;
     return a.rows;
   }
-  WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
+  if (a.S > 1 || a.scores)
+    WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, true>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
+  else
+    WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, false>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
   if (int rc = check_launch("paged_attn")) return rc;
   WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<kLatentD, kLatentTile, 16 * HT>),
             dim3{unsigned(int64_t(a.B) * a.c.heads * R)}, dim3(256), 0, a);
