@@ -164,17 +164,33 @@ def test_attend_missing_pages_and_long_lengths(gpu, page, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
-def test_attend_row_takes_nothing_from_tokens_it_does_not_see(gpu, dtype):
-    """The newest tokens hold NaN (K of one, V of another): the rows before them stay finite."""
-    lens, S, HK, D = [200, 33], 4, 2, 64
-    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype)
-    q, qd = queries(gpu, 4, 2, S, 4, D)
+@pytest.mark.parametrize("HK,g,D,shared", [(2, 2, 64, False), (1, 16, 128, False), (2, 8, 256, False), (1, 6, 128, True),
+                                           (1, 16, 512, True), (1, 64, 512, True)])
+def test_attend_row_takes_nothing_from_tokens_it_does_not_see(gpu, HK, g, D, shared, dtype):
+    """The newest tokens hold NaN (K of one, V of another): the rows before them stay finite, and the
+    weights that every token gets are those of the formula."""
+    lens, S = [200, 33, 3], 4
+    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared, track=True)
+    q, qd = queries(gpu, 4, len(lens), S, HK * g, D)
     ref = op.attend(vals, qd, table, lens, D ** -0.5)
-    for b, n in enumerate(lens):
-        for t, pool in ((n - 1, cache.k), (n - 2, cache.v)):
-            row = pool[table[b, t // 16], :, t % 16]
-            row.view(torch.uint8 if dtype == E4M3 else torch.int16).fill_(0x7F if dtype == E4M3 else 0x7FC0)
-    o = cache.attend(q, tab, torch.tensor(lens, dtype=torch.int32, device=gpu), D ** -0.5)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+
+    def poison(t, pool, b):
+        row = pool[table[b, t // 16], :, t % 16]
+        row.view(torch.uint8 if dtype == E4M3 else torch.int16).fill_(0x7F if dtype == E4M3 else 0x7FC0)
+
+    if not shared:  # V alone: no score changes
+        for b, m in enumerate(lens):
+            poison(m - 2, cache.v, b)
+        before = cache.weights.cpu().double().numpy()
+        cache.attend(q, tab, n, D ** -0.5, accumulate=True)
+        got = cache.weights.cpu().double().numpy()
+        _, e32 = bounds(ref[0], ref[1], ref[3], D)
+        assert (np.abs(got - before - ref[2]) <= e32 * ref[2] + 2.0 ** -23 * (np.abs(got) + 1e-30)).all()
+    for b, m in enumerate(lens):
+        poison(m - 1, cache.k, b)
+        poison(m - 2, cache.k if shared else cache.v, b)
+    o = cache.attend(q, tab, n, D ** -0.5)
     check(o[:, :2], tuple(x[:, :2] if i < 2 else x for i, x in enumerate(ref)), D)
     assert torch.isnan(o[:, 2:]).all()
 

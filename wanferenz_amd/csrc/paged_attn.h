@@ -6,7 +6,7 @@
 // of 32.  All units' granules in a row are cut into one equal share per worker, so the chip is filled
 // whatever the lengths: a unit inside one share is finished there, a cut one leaves (m, l, O) partials
 // that paged_attn_join_kernel merges.  A worker's share holds at most two cut units, its first and its
-// last, which own its partial slots 2w and 2w + 1.
+// last, which own its partial slots 2w and 2w + 1; the worker that a cut unit begins in says so.
 //
 // A worker is one wave, or two that split 64 rows (RH = 2) and the loads.  One wave waits for nobody:
 // while it begins a unit or ends one, the compute unit's other workers keep loading.  Tiles of 32 tokens
@@ -40,6 +40,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kPagedLazy = 8.0f;       // the running maximum moves when a tile exceeds it by more
 constexpr int kPagedMaxS = 16;
 
+// A unit's parts: np of them (1: nothing to join, 0: no unit), the first in partial slot `slot`, the
+// others in the first slots of the workers after it.
+struct PagedCut {
+  int32_t b, u, np, slot;
+};
+
 struct PagedAttnArgs {
   PagedView c;
   const uint16_t* q;
@@ -49,12 +55,18 @@ struct PagedAttnArgs {
   const int32_t* lens;
   uint16_t* o;
   float* part;    // 2 W slots of m[rows], l[rows] and O[rows][D]
+  PagedCut* cut;  // a unit where by_unit, else the cut unit that begins in a worker's share
   float* ml;      // accumulate: per unit and row the final maximum and 1 / sum
   float* scores;  // accumulate: y [B, heads, R, capacity]
-  int width, B, S, H, W, rows;  // rows: of a partial, min(R, the unit's)
+  int width, B, S, H, W, rows, unit_rows, by_unit;  // rows: of a partial, min(R, unit_rows)
   int64_t capacity;  // slots of the table, width * page
   float scale2;      // softmax scale * log2(e)
 };
+
+static inline int64_t paged_units(const PagedAttnArgs& a) {
+  const int R = a.S * (a.H / a.c.heads);
+  return int64_t(a.B) * a.c.heads * ((R + a.unit_rows - 1) / a.unit_rows);
+}
 
 // Tokens of a sequence, and its granules.
 __device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
@@ -156,6 +168,33 @@ __device__ __forceinline__ pv8s paged_widen(int lo, int hi) {
   return u.v;
 }
 
+// The sequences without tokens among w, w + a.W, ...: zeros, and nothing to join.
+__device__ __forceinline__ void paged_empty(const PagedAttnArgs& a, int w, int upb, int D, int threads) {
+  for (int b = w; b < a.B; b += a.W) {
+    if (paged_len(a, b) > 0) continue;
+    const int64_t chunks = int64_t(a.S) * a.H * (D / 8);
+    for (int64_t i = threadIdx.x; i < chunks; i += threads)
+      *reinterpret_cast<v4i*>(a.o + (b * chunks + i) * 8) = v4i{0, 0, 0, 0};
+    if (a.by_unit)
+      for (int u = threadIdx.x; u < upb; u += threads) a.cut[int64_t(b) * upb + u] = PagedCut{b, u, 0, 0};
+  }
+}
+
+// Whether 16 bytes of V hold an infinity or a NaN.
+template <bool FP8>
+__device__ __forceinline__ bool paged_odd(v4i v) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = uint32_t(v[i]);
+    if constexpr (FP8)  // e4m3's NaN: all ones but the sign
+      odd |= (w & 0x7Fu) == 0x7Fu || (w & 0x7F00u) == 0x7F00u || (w & 0x7F0000u) == 0x7F0000u || (w & 0x7F000000u) == 0x7F000000u;
+    else
+      odd |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+  }
+  return odd;
+}
+
 // One row of Q (bf16) against one row of the cache, this lane group's share g of the products; the rest of
 // the row is with the lanes 16 apart.  For the few tokens that not every row sees: Q is read again.
 template <int D, bool FP8>
@@ -221,8 +260,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
   constexpr int NS = C::NS, RB = C::RB, ROWS = C::ROWS;
   constexpr int KC = D / 32, NT = D / 16;
   extern __shared__ __align__(1024) uint8_t lds[];
-  const int tid = threadIdx.x, lane = tid & 63, rh = RH == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nl = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, rh = RH == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   uint8_t* const ring = lds;
   uint8_t* const scales = ring + NS * C::STAGE;  // e4m3: 256 bytes a tile
   uint32_t* const s_valid = reinterpret_cast<uint32_t*>(lds + C::RING) + rh * NS;
@@ -235,7 +273,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
   const int w = blockIdx.x;
   const int64_t total = paged_uniform(paged_total<kPagedTile>(a, upb));
   const int W = paged_workers(total, a.W);
-  if (w >= W) return;
+  if (!a.by_unit && tid == 0) a.cut[w] = PagedCut{0, 0, 0, 0};
+  if (w >= W) {
+    paged_empty(a, w, upb, D, 64 * RH);
+    return;
+  }
   int64_t x = paged_uniform(paged_share(total, W, w));
   const int64_t x_end = paged_uniform(paged_share(total, W, w + 1));
   int b;
@@ -248,6 +290,10 @@ void paged_attn_kernel(PagedAttnArgs a) {
   const int ish = page >= kPagedTile ? 0 : 1;  // page ids a tile: 1 or 2
 
   for (bool first_piece = true; x < x_end; first_piece = false) {
+    // the lane's coordinates, made anew for each part: addresses computed from them stay inside it
+    int lane = tid & 63;
+    asm volatile("" : "+v"(lane));
+    const int nl = lane & 15, g = lane >> 4;
     int gran = (n + kPagedTile - 1) / kPagedTile;
     while (x >= before + int64_t(gran) * upb) {  // the next sequence that holds anything
       before += int64_t(gran) * upb;
@@ -261,9 +307,14 @@ void paged_attn_kernel(PagedAttnArgs a) {
     const bool whole = g0 == 0 && g1 == gran;
     const int hk = __builtin_amdgcn_readfirstlane(u / RG), rg = u - hk * RG;
     const int row0 = rg * ROWS + rh * C::WROWS;  // this wave's first row
-    const int t0 = g0 * kPagedTile, t1 = min(g1 * kPagedTile, n);
-    // the last S - 1 tokens are seen by some rows only: they are added one by one below
-    const int tm = min(t1, max(n - a.S + 1, t0));
+    const int t0 = g0 * kPagedTile, tm = min(g1 * kPagedTile, n);
+    // The last S - 1 tokens, from n0 on, are seen by some rows only.  The others' p is 0 there, which keeps
+    // a finite value out of them; a token whose V is not finite is added by itself after the tiles.
+    const int n0 = n - a.S + 1;
+    int odd0 = 0, odd1 = 0;  // those tokens
+    if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
+      a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
+          PagedCut{b, u, paged_owner(total, W, ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
     // Q fragments: lane (row nl, group g); e4m3 rows are read 16 codes at a time, so there the
@@ -364,7 +415,25 @@ void paged_attn_kernel(PagedAttnArgs a) {
       }
       uint8_t* const kt = ring + stage * C::STAGE;
       uint8_t* const vt = SHARED ? kt : kt + C::SIDE;
-      const uint32_t valid = __builtin_amdgcn_readfirstlane(s_valid[stage]);
+      uint32_t valid = __builtin_amdgcn_readfirstlane(s_valid[stage]);
+      const int t = t0 + kPagedTile * k;
+      const bool last = a.S > 1 && t + kPagedTile > n0;
+      if (last) {
+        const uint32_t some = valid & ~((1u << max(n0 - t, 0)) - 1u);  // tokens that some rows see
+        bool odd = false;
+        for (int i = lane; i < kPagedTile * L::CH; i += 64)
+          if ((some >> (i / L::CH)) & 1) odd |= paged_odd<FP8>(*reinterpret_cast<const v4i*>(vt + i * 16));
+        if constexpr (FP8) {
+          const float sc = reinterpret_cast<const float*>(scales + stage * C::SCALES)[32 + (lane & 31)];
+          odd |= ((some >> (lane & 31)) & 1) && !is_finite_f32(sc);
+        }
+        if (__ballot(odd)) {
+          odd0 = odd1 > 0 ? odd0 : max(n0, t);
+          odd1 = min(t + kPagedTile, tm);
+          valid &= ~some;
+        }
+        meet();  // both waves have looked at V before its rows are cleared
+      }
       if (valid != 0xFFFFFFFFu) {
         // rows that hold nothing become zeros, whatever bits their memory has
         for (int i = lane; i < kPagedTile * L::CH; i += 64)
@@ -425,22 +494,29 @@ void paged_attn_kernel(PagedAttnArgs a) {
           for (int i = 0; i < 8; ++i)
             if (!((valid >> (16 * (i >> 2) + 4 * g + (i & 3))) & 1)) y[i] = -INFINITY;
         }
+        if (last) {
+          const int sees = n0 + min(row0 + 16 * rt + nl, R - 1) / grp - t;  // tokens of the tile that the row sees
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (16 * (i >> 2) + 4 * g + (i & 3) >= sees) y[i] = -INFINITY;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, y[i]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         if (a.scores) {
-          const int r = row0 + 16 * rt + nl, t = t0 + kPagedTile * k + 4 * g;
+          const int r = row0 + 16 * rt + nl;
           if (r < R) {
-            float* const row = a.scores + ((int64_t(b) * a.c.heads + hk) * R + r) * a.capacity;
+            float* const row = a.scores + ((int64_t(b) * a.c.heads + hk) * R + r) * a.capacity + t + 4 * g;
+            const int left = tm - t - 4 * g;
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
-              if (t + 16 * tt + 3 < tm) {
-                *reinterpret_cast<v4f*>(row + t + 16 * tt) = v4f{y[4 * tt], y[4 * tt + 1], y[4 * tt + 2], y[4 * tt + 3]};
+              if (16 * tt + 3 < left) {
+                *reinterpret_cast<v4f*>(row + 16 * tt) = v4f{y[4 * tt], y[4 * tt + 1], y[4 * tt + 2], y[4 * tt + 3]};
               } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                  if (t + 16 * tt + i < tm) row[t + 16 * tt + i] = y[4 * tt + i];
+                  if (16 * tt + i < left) row[16 * tt + i] = y[4 * tt + i];
               }
             }
           }
@@ -497,10 +573,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
       stage = stage + 1 == NS ? 0 : stage + 1;
     }
 
-    // ---- the tokens that only some rows see: a row takes nothing, not even a NaN, from one that it
-    // does not see ----
-    {
-      for (int t = tm; t < t1; ++t) {
+    // ---- tokens that only some rows see and whose V is not finite: a row takes nothing from one that
+    // it does not see ----
+    if (odd0 < odd1) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // scores that the tiles stored for these tokens
+      for (int t = odd0; t < odd1; ++t) {
         const int64_t at = paged_row(a.c, trow, a.width, hk, t);
         if (at < 0) continue;
         const uint8_t* const kr = a.c.k + at * RB;
@@ -583,108 +660,102 @@ void paged_attn_kernel(PagedAttnArgs a) {
     meet();  // the ring is free for the next part's tiles
     x = ubeg + g1;
   }
+  paged_empty(a, w, upb, D, 64 * RH);
 }
 
-// Merges a cut unit's partials, a workgroup a row: every partial's (m, l) at once, then O with 256 / (D / 4)
-// partials in flight at a time.  A row without tokens gets zeros.
+// Merges the cut units' partials.  WIDE: a workgroup a row of a unit, every partial's (m, l) at once,
+// then O with GR partials in flight at a time, for few units of many parts (131071 tokens of one sequence: 128
+// parts of 8 units).  Else GR rows a workgroup, each by the CH threads that hold its columns, without
+// a barrier: a unit of a large batch has two or three parts.
 constexpr int kPagedMaxWorkers = 4096;
 
-template <int D, int G, int ROWS>
+template <int D, bool WIDE>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
-  __shared__ float s_f[kPagedMaxWorkers];
-  __shared__ float s_red[2][4];
-  __shared__ v4f s_o[256];
   constexpr int CH = D / 4, GR = 256 / CH;
-  const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
-  const int bh = blockIdx.x / R, r = blockIdx.x - bh * R, b = bh / a.c.heads, hk = bh - b * a.c.heads;
-  const int u = hk * RG + r / ROWS, rl = r % ROWS;
+  const PagedCut cut = a.cut[blockIdx.x];
+  const int np = cut.np;
+  if (np < 2) return;
+  const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + a.unit_rows - 1) / a.unit_rows;
+  const int hk = cut.u / RG, rg = cut.u - hk * RG, b = cut.b;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = paged_len(a, b), gran = (n + G - 1) / G;
-  const int head = hk * grp + r % grp, s = r / grp;
-  uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D;
-  if (n == 0) {
-    if (tid < CH) *reinterpret_cast<uint2*>(orow + 4 * tid) = make_uint2(0, 0);
-    if (a.ml && tid == 0) {
-      float* const e = a.ml + 2 * (int64_t(bh) * R + r);
-      e[0] = e[1] = 0.0f;
-    }
-    return;
-  }
-  int64_t before = 0, total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int x = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
-    int all = x, lower = b0 + lane < b ? x : 0;
-    for (int o = 1; o < 64; o <<= 1) {
-      all += __shfl_xor(all, o, 64);
-      lower += __shfl_xor(lower, o, 64);
-    }
-    total += all;
-    before += lower;
-  }
-  total *= upb;
-  const int W = paged_workers(total, a.W);
-  const int64_t ubeg = before * upb + int64_t(u) * gran;
-  const int w0 = paged_owner(total, W, ubeg), w1 = paged_owner(total, W, ubeg + gran - 1);
-  const int np = w1 - w0 + 1;
-  if (np == 1) return;  // finished by its worker
-  // the first one's part of the unit is its first if its share begins here, else its last
-  const int64_t slot = int64_t(a.rows) * (D + 2);
-  const float* const part = a.part + 2 * int64_t(w0) * slot;
-  const int64_t step0 = paged_share(total, W, w0) >= ubeg ? 0 : slot;
-  auto at = [&](int j) { return part + (j == 0 ? step0 : 2 * int64_t(j) * slot); };
-  const float sk = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-  float M = sk, m[kPagedMaxWorkers / 256], l[kPagedMaxWorkers / 256];
-#pragma unroll
-  for (int i = 0; i < kPagedMaxWorkers / 256; ++i) {
-    const int j = i * 256 + tid;
-    m[i] = -INFINITY;
-    l[i] = 0.0f;
-    if (j < np) {
-      m[i] = at(j)[rl];
-      l[i] = at(j)[a.rows + rl];
-    }
-    M = fmaxf(M, m[i]);
-    if ((i + 1) * 256 >= np) break;
-  }
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  if (lane == 0) s_red[0][wave] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-  const float Me = M == -INFINITY ? 0.0f : M;
-  float den = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPagedMaxWorkers / 256; ++i) {
-    const int j = i * 256 + tid;
-    if (j < np) {
-      const float f = __builtin_amdgcn_exp2f(m[i] - Me);
-      s_f[j] = f;
-      den += f * l[i];
-    }
-    if ((i + 1) * 256 >= np) break;
-  }
-  for (int o = 1; o < 64; o <<= 1) den += __shfl_xor(den, o, 64);
-  if (lane == 0) s_red[1][wave] = den;
-  __syncthreads();
-  den = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-  if (a.sink) den += __builtin_amdgcn_exp2f(sk - Me);
   const int ch = tid % CH, gr = tid / CH;
+  const int rl = WIDE ? blockIdx.y : blockIdx.y * GR + gr, r = rg * a.unit_rows + rl;
+  if (rl >= a.rows || r >= R) return;  // WIDE: the whole workgroup
+  const int64_t slot = int64_t(a.rows) * (D + 2);
+  const float* const part = a.part + rl;
+  auto at = [&](int j) { return part + (j == 0 ? int64_t(cut.slot) : 2 * (int64_t(cut.slot >> 1) + j)) * slot; };
+  const int head = hk * grp + r % grp;
+  const float sk = a.sink ? a.sink[head] * kLog2e : -INFINITY;
+  const int off = 2 * a.rows + rl * (D - 1) + 4 * ch;
+  float M = sk, den = 0.0f;
   v4f o = v4f{0.f, 0.f, 0.f, 0.f};
-  const int64_t off = 2 * a.rows + rl * D + 4 * ch;
-#pragma unroll 4
-  for (int j = gr; j < np; j += GR) o += *reinterpret_cast<const v4f*>(at(j) + off) * s_f[j];
-  s_o[tid] = o;
-  __syncthreads();
-  if (tid >= CH) return;
+  float Me;
+  if constexpr (WIDE) {
+    __shared__ float s_f[kPagedMaxWorkers];
+    __shared__ float s_red[2][4];
+    __shared__ v4f s_o[256];
+    float l0 = 0.0f;  // of this thread's first partial; there are seldom more
+    for (int j = tid; j < np; j += 256) {
+      const float m = at(j)[0];
+      if (j == tid) l0 = at(j)[a.rows];
+      s_f[j] = m;
+      M = fmaxf(M, m);
+    }
+    for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
+    if (lane == 0) s_red[0][wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    Me = M == -INFINITY ? 0.0f : M;
+    for (int j = tid; j < np; j += 256) {
+      const float f = __builtin_amdgcn_exp2f(s_f[j] - Me);
+      s_f[j] = f;
+      den += f * (j == tid ? l0 : at(j)[a.rows]);
+    }
+    for (int i = 1; i < 64; i <<= 1) den += __shfl_xor(den, i, 64);
+    if (lane == 0) s_red[1][wave] = den;
+    __syncthreads();
+    den = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+#pragma unroll 8
+    for (int j = gr; j < np; j += GR) o += *reinterpret_cast<const v4f*>(at(j) + off) * s_f[j];
+    s_o[tid] = o;
+    __syncthreads();
+    if (tid >= CH) return;
 #pragma unroll
-  for (int i = 1; i < GR; ++i) o += s_o[i * CH + tid];
+    for (int i = 1; i < GR; ++i) o += s_o[i * CH + tid];
+  } else {
+#pragma unroll 4
+    for (int j = 0; j < np; ++j) M = fmaxf(M, at(j)[0]);
+    Me = M == -INFINITY ? 0.0f : M;
+#pragma unroll 4
+    for (int j = 0; j < np; ++j) {
+      const float f = __builtin_amdgcn_exp2f(at(j)[0] - Me);
+      den += f * at(j)[a.rows];
+      o += *reinterpret_cast<const v4f*>(at(j) + off) * f;
+    }
+  }
+  if (a.sink) den += __builtin_amdgcn_exp2f(sk - Me);
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-  *reinterpret_cast<uint2*>(orow + 4 * tid) =
+  uint16_t* const orow = a.o + ((int64_t(b) * a.S + r / grp) * a.H + head) * D;
+  *reinterpret_cast<uint2*>(orow + 4 * ch) =
       make_uint2(f32x2_to_bf16x2(o[0] * inv, o[1] * inv), f32x2_to_bf16x2(o[2] * inv, o[3] * inv));
-  if (a.ml && tid == 0) {
-    float* const e = a.ml + 2 * (int64_t(bh) * R + r);
+  if (a.ml && ch == 0) {
+    float* const e = a.ml + 2 * ((int64_t(b) * a.c.heads + hk) * R + r);
     e[0] = Me;
     e[1] = inv;
   }
+}
+
+template <int D>
+int paged_attn_join(const PagedAttnArgs& a, hipStream_t stream) {
+  constexpr int GR = 256 / (D / 4);
+  const int64_t units = paged_units(a);
+  const unsigned n = unsigned(std::min<int64_t>(units, a.W));
+  if (8 * units <= a.W)
+    WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<D, true>), dim3(n, unsigned(a.rows)), dim3(256), 0, a);
+  else
+    WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<D, false>), dim3(n, unsigned((a.rows + GR - 1) / GR)),
+              dim3(256), 0, a);
+  return check_launch("paged_attn_join");
 }
 
 // The kernel of R rows a KV head: 16, 32 or 64 rows a unit.
@@ -694,19 +765,19 @@ int paged_attn_launch_rt(PagedAttnArgs a, bool ask, int* workers, hipStream_t st
   static_assert(C::LDS <= 160 * 1024, "a workgroup's LDS");
   const int R = a.S * (a.H / a.c.heads);
   a.W = std::min(cu_count() * C::PER_CU, kPagedMaxWorkers);
+  a.unit_rows = C::ROWS;
   a.rows = std::min(R, C::ROWS);
   if (ask) {
     *workers = a.W;
     return a.rows;
   }
+  a.by_unit = paged_units(a) <= a.W;
   static LdsGrant grant;
   auto* const kernel = paged_attn_kernel<D, FP8, SHARED, RT, RH>;
   if (int rc = allow_lds("paged_attn", kernel, C::LDS, grant)) return rc;
   WZ_LAUNCH("paged_attn", stream, kernel, dim3{unsigned(a.W)}, dim3(64 * RH), C::LDS, a);
   if (int rc = check_launch("paged_attn")) return rc;
-  auto* const join = paged_attn_join_kernel<D, kPagedTile, C::ROWS>;
-  WZ_LAUNCH("paged_attn_join", stream, join, dim3{unsigned(int64_t(a.B) * a.c.heads * R)}, dim3(256), 0, a);
-  return check_launch("paged_attn_join");
+  return paged_attn_join<D>(a, stream);
 }
 
 template <int D, bool FP8, bool SHARED>

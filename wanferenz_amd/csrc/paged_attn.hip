@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void paged_attn_weigh_kernel(PagedAttnArgs a) 
 }
 
 struct PagedAttnSizes {
-  int64_t part, ml, scores;  // floats
+  int64_t part, cut, ml, scores;  // floats
 };
 
 static PagedAttnSizes paged_attn_sizes(const wz_paged_kv* c, int64_t B, int64_t S, int64_t H, int64_t width,
@@ -50,6 +50,7 @@ static PagedAttnSizes paged_attn_sizes(const wz_paged_kv* c, int64_t B, int64_t 
   int workers = 0;
   const int64_t rows = paged_attn_any(c->head_dim, a, true, &workers, nullptr);
   z.part = (2 * workers * rows * (c->head_dim + 2) + 3) / 4 * 4;
+  z.cut = workers * int64_t(sizeof(PagedCut) / sizeof(float));
   if (accumulate) {
     z.ml = (2 * B * c->kv_heads * R + 3) / 4 * 4;
     z.scores = B * c->kv_heads * R * width * c->page_size;
@@ -67,7 +68,7 @@ extern "C" int64_t wz_paged_attn_workspace_bytes(const wz_paged_kv* cache, int64
   if (B <= 0 || S <= 0 || S > kPagedMaxS || H <= 0 || H > 65536 || H % view.heads)
     return 0;
   const PagedAttnSizes z = paged_attn_sizes(cache, B, S, H, table_width, accumulate != 0);
-  return (z.part + z.ml + z.scores) * int64_t(sizeof(float));
+  return (z.part + z.cut + z.ml + z.scores) * int64_t(sizeof(float));
 }
 
 extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q_strides,
@@ -96,7 +97,7 @@ extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const
   if (2 * R * int64_t(sizeof(float)) > 65536)
     return set_error(WZ_EINVAL, "paged_attn: %lld query rows on a KV head", (long long)R);
   const PagedAttnSizes z = paged_attn_sizes(cache, B, S, H, table_width, accumulate != 0);
-  const int64_t need = (z.part + z.ml + z.scores) * int64_t(sizeof(float));
+  const int64_t need = (z.part + z.cut + z.ml + z.scores) * int64_t(sizeof(float));
   if (!workspace || workspace_bytes < need)
     return set_error(WZ_ESPACE, "paged_attn: workspace of %lld bytes, %lld needed",
                      (long long)(workspace ? workspace_bytes : 0), (long long)need);
@@ -109,8 +110,9 @@ extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const
   a.lens = lens;
   a.o = static_cast<uint16_t*>(o_bf16);
   a.part = static_cast<float*>(workspace);
-  a.ml = accumulate ? a.part + z.part : nullptr;
-  a.scores = accumulate ? a.part + z.part + z.ml : nullptr;
+  a.cut = reinterpret_cast<PagedCut*>(a.part + z.part);
+  a.ml = accumulate ? a.part + z.part + z.cut : nullptr;
+  a.scores = accumulate ? a.ml + z.ml : nullptr;
   a.width = int(table_width);
   a.B = int(B);
   a.S = int(S);

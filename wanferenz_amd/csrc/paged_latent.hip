@@ -23,7 +23,7 @@ struct LatentCfg {
   static constexpr int RB = kLatentD * (FP8 ? 1 : 2);
   static constexpr int TILE = kLatentTile * RB;
   static constexpr int RPW = kLatentTile / kLatentWaves;      // rows that a wave loads
-  static constexpr int LOADS = RPW * RB / 1024;
+  static constexpr int LOADS = RPW * RB / 1024 + (FP8 ? 1 : 0);
 };
 
 // EXTRA: several new tokens, or weights to accumulate; without them 64 rows just fit the registers.
@@ -37,7 +37,9 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
   // the last KQ chunks of Q are read from LDS for each tile: with all of 64 rows in registers some were
   // spilled, and a reload waits for the loads of the next tile (102 us, 268 MB; so: see below)
   constexpr int KQ = HT == 4 ? 2 : 0;
+  constexpr int QB = 2 * D;  // bytes of a row of Q
   __shared__ __align__(1024) uint8_t kb[2][C::TILE];
+  __shared__ __align__(1024) uint8_t s_qf[FP8 ? ROWS * QB : 16];  // e4m3: 64 rows of Q are two tiles
   __shared__ __align__(16) uint8_t s_p[2][ROWS][64];  // [tokens / 32][row]: group g's 8 k slots at 16 g
   __shared__ float s_max[4][ROWS], s_l[4][ROWS];      // [token tile][row]
   __shared__ float s_scale[2][T], s_y[ROWS];
@@ -45,8 +47,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
   __shared__ int s_bump[2];
   __shared__ __align__(16) uint8_t s_q[KQ ? ROWS : 1][128];  // [row]: chunk KC - 2 + c, group g at (4 c + g) ^ swz(row)
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nl = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rt = wave & 3, ht0 = (wave >> 2) * SHT;  // this wave's token tile and first row tile of S
   const bool has_s = ht0 < HT;
   const uint32_t kb_lds = lds_addr(&kb[0][0]), sc_lds = lds_addr(&s_scale[0][0]);
@@ -56,7 +57,11 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
   const int w = blockIdx.x;
   const int64_t total = paged_uniform(paged_total<T>(a, upb));
   const int W = paged_workers(total, a.W);
-  if (w >= W) return;
+  if (!a.by_unit && tid == 0) a.cut[w] = PagedCut{0, 0, 0, 0};
+  if (w >= W) {
+    paged_empty(a, w, upb, D, 64 * kLatentWaves);
+    return;
+  }
   int64_t x = paged_uniform(paged_share(total, W, w));
   const int64_t x_end = paged_uniform(paged_share(total, W, w + 1));
   int b;
@@ -68,6 +73,10 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
   const int ps = a.c.shift, page = a.c.page;
 
   for (bool first_piece = true; x < x_end; first_piece = false) {
+    // the lane's coordinates, made anew for each part: addresses computed from them stay inside it
+    int lane = tid & 63;
+    asm volatile("" : "+v"(lane));
+    const int nl = lane & 15, g = lane >> 4;
     int gran = (n + T - 1) / T;
     while (x >= before + int64_t(gran) * upb) {  // the next sequence that holds anything
       before += int64_t(gran) * upb;
@@ -80,26 +89,14 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
     const int g0 = int(x - ubeg), g1 = int(min(x_end - ubeg, int64_t(gran)));
     const bool whole = g0 == 0 && g1 == gran;
     const int hk = __builtin_amdgcn_readfirstlane(u / RG), rg = u - hk * RG, row0 = rg * ROWS;
-    const int t0 = g0 * T, t1 = min(g1 * T, n);
-    const int tm = EXTRA ? min(t1, max(n - a.S + 1, t0)) : t1;  // the last S - 1 tokens are added one by one below
+    const int t0 = g0 * T, tm = min(g1 * T, n);
+    const int n0 = n - a.S + 1;  // from here on a token is seen by some rows only, as in paged_attn_kernel
+    int odd0 = 0, odd1 = 0;
+    if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
+      a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
+          PagedCut{b, u, paged_owner(total, W, ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
-    // Q fragments (B operand of S^T): lane (row nl, group g); as in paged_attn_kernel
-    pv8s qb[SHT][KC - KQ];
-#pragma unroll
-    for (int h = 0; h < SHT; ++h) {
-      const int rl = 16 * (has_s ? ht0 + h : 0) + nl, r = min(row0 + rl, R - 1);
-      const uint16_t* const qrow = a.q + b * a.qb + (r / grp) * a.qs + (hk * grp + r % grp) * a.qh;
-#pragma unroll
-      for (int cc = 0; cc < KC; ++cc) {
-        const int d = FP8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g;
-        const pv8s q = *reinterpret_cast<const pv8s*>(qrow + d);
-        if (cc < KC - KQ)
-          qb[h][cc] = q;
-        else if (rt == 0)
-          *reinterpret_cast<pv8s*>(&s_q[rl][(((cc - (KC - KQ)) * 4 + g) ^ PagedRow<128>::swz(rl)) << 4]) = q;
-      }
-    }
     v4f acc[HT][NT];  // acc[ht][nt][i] = O[row 16ht + nl][64 wave + 16nt + 4g + i]
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht)
@@ -134,7 +131,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       asm volatile("" : "+v"(ln));  // recomputed for each tile: the registers go to Q and O
       const int rin = ln / L::CH, slot = ln % L::CH;
 #pragma unroll
-      for (int j = 0; j < C::LOADS; ++j) {
+      for (int j = 0; j < C::RPW / L::RPI; ++j) {
         const int r = j * L::RPI;  // of the wave's rows; the swizzle goes by the tile's
         const uint32_t voff = uint32_t(rin * RB + ((slot ^ L::swz(C::RPW * wave + r + rin)) << 4));
         paged_load16(a.c.k + (row + r) * RB, voff, dst + j * 1024);
@@ -145,10 +142,42 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
                       __builtin_amdgcn_readfirstlane(sc_lds + (buf * T + C::RPW * wave) * 4));
       }
     };
+    // Q's rows in whole lines through the second buffer (fragments loaded by the four waves that share them
+    // took 4 us more), while the first tile is on its way
     if (nk > 0) fetch_ids(0);
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // Q too: no wait for it is left inside the loop
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+    uint8_t* const qbuf = FP8 ? s_qf : kb[1];
+    const uint32_t q_lds = lds_addr(qbuf);
+    using QL = PagedRow<QB>;
+#pragma unroll
+    for (int j = 0; j < ROWS / kLatentWaves; ++j) {
+      const int rl = j * kLatentWaves + wave, r = min(row0 + rl, R - 1);
+      paged_load16(reinterpret_cast<const uint8_t*>(a.q + b * a.qb + (r / grp) * a.qs + (hk * grp + r % grp) * a.qh),
+                   uint32_t((lane ^ QL::swz(rl)) << 4), __builtin_amdgcn_readfirstlane(q_lds + rl * QB));
+    }
     if (tid < 2) s_bump[tid] = 0;
-    if (nk > 0) issue(0, 0);
+    if (nk > 0) {
+      issue(0, 0);
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(C::LOADS));
+    } else {
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+    }
+    meet();
+    // fragments (B operand of S^T): lane (row nl, group g); the order of d as in paged_attn_kernel
+    pv8s qb[SHT][KC - KQ];
+#pragma unroll
+    for (int h = 0; h < SHT; ++h) {
+      const int rl = 16 * (has_s ? ht0 + h : 0) + nl;
+#pragma unroll
+      for (int cc = 0; cc < KC; ++cc) {
+        const int ch = FP8 ? 8 * (cc >> 1) + 2 * g + (cc & 1) : 4 * cc + g;
+        const pv8s q = *reinterpret_cast<const pv8s*>(qbuf + rl * QB + ((ch ^ QL::swz(rl)) << 4));
+        if (cc < KC - KQ)
+          qb[h][cc] = q;
+        else if (rt == 0)
+          *reinterpret_cast<pv8s*>(&s_q[rl][(((cc - (KC - KQ)) * 4 + g) ^ PagedRow<128>::swz(rl)) << 4]) = q;
+      }
+    }
 
 #pragma unroll 1
     for (int k = 0; k < nk; ++k) {
@@ -157,7 +186,22 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       meet();                                     // ... and every wave's; the other buffer and s_p are free
       if (k + 1 < nk) issue(k + 1, buf ^ 1);
       uint8_t* const ks = kb[buf];
-      const uint64_t valid = uint64_t(paged_uniform(*reinterpret_cast<const int64_t*>(s_valid[buf])));
+      uint64_t valid = uint64_t(paged_uniform(*reinterpret_cast<const int64_t*>(s_valid[buf])));
+      const int tk = t0 + T * k;
+      const bool last = EXTRA && a.S > 1 && tk + T > n0;
+      if (last) {
+        const uint64_t some = valid & ~((1ull << max(n0 - tk, 0)) - 1ull);  // tokens that some rows see
+        bool odd = false;  // every wave looks at all of them, and comes to the same
+        for (int i = lane; i < T * L::CH; i += 64)
+          if ((some >> (i / L::CH)) & 1) odd |= paged_odd<FP8>(*reinterpret_cast<const v4i*>(ks + i * 16));
+        if constexpr (FP8) odd |= ((some >> lane) & 1) && !is_finite_f32(s_scale[buf][lane]);
+        if (__ballot(odd)) {
+          odd0 = odd1 > 0 ? odd0 : max(n0, tk);
+          odd1 = min(tk + T, tm);
+          valid &= ~some;
+        }
+        meet();  // every wave has looked before the rows are cleared
+      }
       if (~valid) {
         // rows that hold nothing become zeros, whatever bits their memory has
         for (int i = tid; i < T * L::CH; i += 64 * kLatentWaves)
@@ -230,8 +274,15 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
           for (int i = 0; i < 4; ++i) {
             const float s = FP8 ? y[h][i] * ksc[i] * a.scale2 : y[h][i] * a.scale2;
             y[h][i] = (valid >> (16 * rt + 4 * g + i)) & 1 ? s : -INFINITY;
-            top = fmaxf(top, y[h][i]);
           }
+          if (last) {
+            const int sees = n0 + min(row0 + 16 * (ht0 + h) + nl, R - 1) / grp - tk;  // tokens that the row sees
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (16 * rt + 4 * g + i >= sees) y[h][i] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, y[h][i]);
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           bump |= top > m_s[h] + kPagedLazy;
@@ -336,9 +387,10 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       }
     }
 
-    // ---- the tokens that only some rows see: a row takes nothing, not even a NaN, from one that it
+    // ---- tokens that only some rows see and that are not finite: a row takes nothing from one that it
     // does not see ----
-    for (int t = tm; EXTRA && t < t1; ++t) {
+    if (EXTRA && odd0 < odd1) __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // scores that the tiles stored for them
+    for (int t = odd0; EXTRA && t < odd1; ++t) {
       const int64_t at = paged_row(a.c, trow, a.width, hk, t);
       if (at < 0) continue;  // the same in every wave
       const uint8_t* const kr = a.c.k + at * RB;
@@ -442,25 +494,26 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
     meet();  // the buffers are free for the next part's tiles
     x = ubeg + g1;
   }
+  paged_empty(a, w, upb, D, 64 * kLatentWaves);
 }
 
 template <bool FP8, int HT>
 static int latent_launch(PagedAttnArgs a, bool ask, int* workers, hipStream_t stream) {
   const int R = a.S * (a.H / a.c.heads);
   a.W = std::min(cu_count(), kPagedMaxWorkers);
-  a.rows = std::min(R, 16 * HT);
+  a.unit_rows = 16 * HT;
+  a.rows = std::min(R, a.unit_rows);
   if (ask) {
     *workers = a.W;
     return a.rows;
   }
+  a.by_unit = paged_units(a) <= a.W;
   if (a.S > 1 || a.scores)
     WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, true>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
   else
     WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, false>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
   if (int rc = check_launch("paged_attn")) return rc;
-  WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<kLatentD, kLatentTile, 16 * HT>),
-            dim3{unsigned(int64_t(a.B) * a.c.heads * R)}, dim3(256), 0, a);
-  return check_launch("paged_attn_join");
+  return paged_attn_join<kLatentD>(a, stream);
 }
 
 int paged_latent(bool fp8, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
