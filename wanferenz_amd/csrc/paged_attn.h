@@ -73,25 +73,25 @@ __device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
   return int(min(int64_t(max(a.lens[b], 0)), a.capacity));
 }
 
-// Where the units' granules begin: upb units a sequence, each of ceil(n / G).  Every lane of a wave
-// gets the result; B sequences are summed 64 at a time.
+// All granules: upb units a sequence, each of ceil(n / G) (the host has checked that they fit 31 bits).
+// Every lane of a wave gets the result; B sequences are summed 64 at a time.
 template <int G>
-__device__ __forceinline__ int64_t paged_total(const PagedAttnArgs& a, int upb) {
+__device__ __forceinline__ int paged_total(const PagedAttnArgs& a, int upb) {
   const int lane = threadIdx.x & 63;
-  int64_t sum = 0;
+  int sum = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     int g = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
     for (int o = 1; o < 64; o <<= 1) g += __shfl_xor(g, o, 64);
     sum += g;
   }
-  return sum * upb;
+  return __builtin_amdgcn_readfirstlane(sum * upb);
 }
 
 // The sequence that holds granule x (0 <= x < total) and the granules before it.
 template <int G>
-__device__ __forceinline__ void paged_find(const PagedAttnArgs& a, int upb, int64_t x, int* seq, int64_t* before) {
+__device__ __forceinline__ void paged_find(const PagedAttnArgs& a, int upb, int x, int* seq, int* before) {
   const int lane = threadIdx.x & 63;
-  int64_t sum = 0;
+  int sum = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int g = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
     int inc = g;
@@ -99,25 +99,31 @@ __device__ __forceinline__ void paged_find(const PagedAttnArgs& a, int upb, int6
       const int y = __shfl_up(inc, o, 64);
       if (lane >= o) inc += y;
     }
-    const int64_t end = (sum + inc) * upb;  // granules up to and with this lane's sequence
-    const uint64_t past = __ballot(end > x);
+    const uint64_t past = __ballot((sum + inc) * upb > x);  // granules up to and with this lane's sequence
     if (past) {
       const int l = __builtin_ctzll(past);
       *seq = b0 + l;
-      *before = (sum + __shfl(inc - g, l, 64)) * upb;
+      *before = __builtin_amdgcn_readlane((sum + inc - g) * upb, l);
       return;
     }
-    sum += __shfl(inc, 63, 64);
+    sum += __builtin_amdgcn_readlane(inc, 63);
   }
   *seq = a.B - 1;  // not reached: x < total
   *before = sum * upb;
 }
 
-// Workgroups with a share (one granule at least each), the first granule of workgroup w's, and the
-// workgroup that holds granule x.
-__device__ __forceinline__ int paged_workers(int64_t total, int W) { return int(min(total, int64_t(W))); }
-__device__ __forceinline__ int64_t paged_share(int64_t total, int W, int w) { return total * w / W; }
-__device__ __forceinline__ int paged_owner(int64_t total, int W, int64_t x) { return int(((x + 1) * W - 1) / total); }
+// The workers' shares: `workers` of them (one granule at least each), the first `rest` one granule longer
+// than `each`; where worker w's begins, and who holds granule x.
+struct PagedShares {
+  int workers, each, rest;
+  __device__ __forceinline__ PagedShares(int total, int W)
+      : workers(min(total, W)), each(total / max(workers, 1)), rest(total - each * workers) {}
+  __device__ __forceinline__ int begin(int w) const { return w * each + min(w, rest); }
+  __device__ __forceinline__ int owner(int x) const {
+    const int longer = rest * (each + 1);
+    return x < longer ? x / (each + 1) : rest + (x - longer) / each;
+  }
+};
 
 // LDS image of a tile: rows of RB bytes, 16-byte chunk c of row r at slot c ^ swz(r).  The
 // fragments' 16-byte reads of one chunk of 16 rows are served in passes that mix rows 0-3 and 12-15
@@ -271,21 +277,18 @@ void paged_attn_kernel(PagedAttnArgs a) {
 
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
   const int w = blockIdx.x;
-  const int64_t total = paged_uniform(paged_total<kPagedTile>(a, upb));
-  const int W = paged_workers(total, a.W);
+  const PagedShares shares(paged_total<kPagedTile>(a, upb), a.W);
   if (!a.by_unit && tid == 0) a.cut[w] = PagedCut{0, 0, 0, 0};
-  if (w >= W) {
+  if (w >= shares.workers) {
     paged_empty(a, w, upb, D, 64 * RH);
     return;
   }
-  int64_t x = paged_uniform(paged_share(total, W, w));
-  const int64_t x_end = paged_uniform(paged_share(total, W, w + 1));
-  int b;
-  int64_t before;
+  int x = shares.begin(w);
+  const int x_end = shares.begin(w + 1);
+  int b, before;  // sequence, and the granules before it
   paged_find<kPagedTile>(a, upb, x, &b, &before);
-  b = __builtin_amdgcn_readfirstlane(b);
-  before = paged_uniform(before);
-  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b)), gran = (n + kPagedTile - 1) / kPagedTile;
+  int u = (x - before) / gran, ubeg = before + u * gran;  // unit of the sequence
   const int ps = a.c.shift, page = a.c.page;
   const int ish = page >= kPagedTile ? 0 : 1;  // page ids a tile: 1 or 2
 
@@ -294,18 +297,9 @@ void paged_attn_kernel(PagedAttnArgs a) {
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));
     const int nl = lane & 15, g = lane >> 4;
-    int gran = (n + kPagedTile - 1) / kPagedTile;
-    while (x >= before + int64_t(gran) * upb) {  // the next sequence that holds anything
-      before += int64_t(gran) * upb;
-      ++b;
-      n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-      gran = (n + kPagedTile - 1) / kPagedTile;
-    }
-    const int u = __builtin_amdgcn_readfirstlane(int((x - before) / gran));  // unit of the sequence
-    const int64_t ubeg = before + int64_t(u) * gran;
-    const int g0 = int(x - ubeg), g1 = int(min(x_end - ubeg, int64_t(gran)));
+    const int g0 = x - ubeg, g1 = min(x_end - ubeg, gran);
     const bool whole = g0 == 0 && g1 == gran;
-    const int hk = __builtin_amdgcn_readfirstlane(u / RG), rg = u - hk * RG;
+    const int hk = u / RG, rg = u - hk * RG;
     const int row0 = rg * ROWS + rh * C::WROWS;  // this wave's first row
     const int t0 = g0 * kPagedTile, tm = min(g1 * kPagedTile, n);
     // The last S - 1 tokens, from n0 on, are seen by some rows only.  The others' p is 0 there, which keeps
@@ -314,7 +308,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
     int odd0 = 0, odd1 = 0;  // those tokens
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
       a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
-          PagedCut{b, u, paged_owner(total, W, ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
+          PagedCut{b, u, whole ? 1 : shares.owner(ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
     // Q fragments: lane (row nl, group g); e4m3 rows are read 16 codes at a time, so there the
@@ -659,6 +653,16 @@ void paged_attn_kernel(PagedAttnArgs a) {
     }
     meet();  // the ring is free for the next part's tiles
     x = ubeg + g1;
+    if (g1 < gran) break;
+    ubeg += gran;
+    if (++u == upb && x < x_end) {  // the next sequence that holds anything
+      do {
+        ++b;
+        n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+      } while (n == 0);
+      gran = (n + kPagedTile - 1) / kPagedTile;
+      u = 0;
+    }
   }
   paged_empty(a, w, upb, D, 64 * RH);
 }

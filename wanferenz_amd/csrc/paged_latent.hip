@@ -55,21 +55,18 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
 
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
   const int w = blockIdx.x;
-  const int64_t total = paged_uniform(paged_total<T>(a, upb));
-  const int W = paged_workers(total, a.W);
+  const PagedShares shares(paged_total<T>(a, upb), a.W);
   if (!a.by_unit && tid == 0) a.cut[w] = PagedCut{0, 0, 0, 0};
-  if (w >= W) {
+  if (w >= shares.workers) {
     paged_empty(a, w, upb, D, 64 * kLatentWaves);
     return;
   }
-  int64_t x = paged_uniform(paged_share(total, W, w));
-  const int64_t x_end = paged_uniform(paged_share(total, W, w + 1));
-  int b;
-  int64_t before;
+  int x = shares.begin(w);
+  const int x_end = shares.begin(w + 1);
+  int b, before;  // sequence, and the granules before it
   paged_find<T>(a, upb, x, &b, &before);
-  b = __builtin_amdgcn_readfirstlane(b);
-  before = paged_uniform(before);
-  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b)), gran = (n + T - 1) / T;
+  int u = (x - before) / gran, ubeg = before + u * gran;  // unit of the sequence
   const int ps = a.c.shift, page = a.c.page;
 
   for (bool first_piece = true; x < x_end; first_piece = false) {
@@ -77,24 +74,15 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));
     const int nl = lane & 15, g = lane >> 4;
-    int gran = (n + T - 1) / T;
-    while (x >= before + int64_t(gran) * upb) {  // the next sequence that holds anything
-      before += int64_t(gran) * upb;
-      ++b;
-      n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-      gran = (n + T - 1) / T;
-    }
-    const int u = __builtin_amdgcn_readfirstlane(int((x - before) / gran));
-    const int64_t ubeg = before + int64_t(u) * gran;
-    const int g0 = int(x - ubeg), g1 = int(min(x_end - ubeg, int64_t(gran)));
+    const int g0 = x - ubeg, g1 = min(x_end - ubeg, gran);
     const bool whole = g0 == 0 && g1 == gran;
-    const int hk = __builtin_amdgcn_readfirstlane(u / RG), rg = u - hk * RG, row0 = rg * ROWS;
+    const int hk = u / RG, rg = u - hk * RG, row0 = rg * ROWS;
     const int t0 = g0 * T, tm = min(g1 * T, n);
     const int n0 = n - a.S + 1;  // from here on a token is seen by some rows only, as in paged_attn_kernel
     int odd0 = 0, odd1 = 0;
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
       a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
-          PagedCut{b, u, paged_owner(total, W, ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
+          PagedCut{b, u, whole ? 1 : shares.owner(ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
     v4f acc[HT][NT];  // acc[ht][nt][i] = O[row 16ht + nl][64 wave + 16nt + 4g + i]
@@ -493,6 +481,16 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
     }
     meet();  // the buffers are free for the next part's tiles
     x = ubeg + g1;
+    if (g1 < gran) break;
+    ubeg += gran;
+    if (++u == upb && x < x_end) {  // the next sequence that holds anything
+      do {
+        ++b;
+        n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+      } while (n == 0);
+      gran = (n + T - 1) / T;
+      u = 0;
+    }
   }
   paged_empty(a, w, upb, D, 64 * kLatentWaves);
 }
