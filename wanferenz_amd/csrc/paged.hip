@@ -92,9 +92,10 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedView c, WriteArgs
 constexpr int kEvictBins = 2048;         // keys are taken 11, 11 and 10 bits at a time
 constexpr int kEvictSmall = 8192;        // slots that one workgroup holds
 constexpr int kEvictThreads = 1024;
-constexpr int kEvictChunk = 4096;        // slots of a workgroup where several share a unit
+constexpr int kEvictChunk = 1024;        // slots of a workgroup where several share a unit
 constexpr int kEvictChunkThreads = 256;
-constexpr int64_t kEvictFused = 65536;   // bytes of K a unit's one workgroup moves itself
+constexpr int64_t kEvictFused = 65536;   // bytes of K a unit's one workgroup moves itself,
+constexpr int kEvictPairs = 1024;        // in up to as many rows
 constexpr int kNoPosition = -0x7FFFFFFF - 1;
 
 // A slot's place in the order of what stays, as an unsigned number: the float's bits, ordered
@@ -133,11 +134,9 @@ __device__ __forceinline__ int evict_len(const EvictArgs& a, int b) {
   return int(min(int64_t(max(a.lens[b], 0)), a.capacity));
 }
 
-// Pair i of a unit: row `fro` over row `to`, 16 bytes a thread of lpr.
-__device__ __forceinline__ void evict_move(const EvictArgs& a, const int32_t* trow, int h, int hole, int mover, int ch,
-                                           int row_bytes) {
+// A pair of rows (of [pages, heads, page]): `fro` over `to`, 16 bytes a thread.
+__device__ __forceinline__ void evict_move(const EvictArgs& a, int64_t to, int64_t fro, int ch, int row_bytes) {
   const PagedView& c = a.c;
-  const int64_t to = paged_row(c, trow, a.width, h, hole), fro = paged_row(c, trow, a.width, h, mover);
   if (to < 0 || fro < 0) return;
   const v4i k = load16(c.k + fro * row_bytes + ch * 16);
   v4i v = v4i{0, 0, 0, 0};
@@ -232,11 +231,13 @@ __device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, in
   }
 }
 
-// A wave's part of the lists.  `before`: evict_count's sums of the slots before the wave's, `all`: of
-// the unit.  Of the ties the lowest `need` stay, so those below keep go first.  -> the unit's pairs
-template <int R>
-__device__ __forceinline__ int evict_list(const EvictArgs& a, int u, const uint32_t (&key)[R], int t0, int n, uint32_t top,
-                                          int need, const int (&before)[4], const int (&all)[4]) {
+// A wave's part of the lists: hole(i, r) and mover(i, r) take the i-th of the unit, which is in round r of
+// this lane.  `before`: evict_count's sums of the slots before the wave's, `all`: of the unit.  Of the
+// ties the lowest `need` stay, so those below keep go first.  -> the unit's pairs
+template <int R, typename Hole, typename Mover>
+__device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&key)[R], int t0, int n, uint32_t top, int need,
+                                          const int (&before)[4], const int (&all)[4], Hole&& put_hole,
+                                          Mover&& put_mover) {
   const int lane = threadIdx.x & 63;
   const uint64_t below = (1ull << lane) - 1;
   const int high = max(0, need - all[1]);  // ties past keep that stay
@@ -244,8 +245,6 @@ __device__ __forceinline__ int evict_list(const EvictArgs& a, int u, const uint3
   int ties = before[1] + before[3];
   int ih = min(t0 - lane, a.keep) - before[0] - min(before[1], need);  // dropped slots below keep
   int im = before[2] + min(before[3], high);                          // kept slots past it
-  int32_t* const holes = a.holes + u * a.moves;
-  int32_t* const movers = a.movers + u * a.moves;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int t = t0 + 64 * i;
@@ -255,8 +254,8 @@ __device__ __forceinline__ int evict_list(const EvictArgs& a, int u, const uint3
     const bool hole = t < n && !kept && t < a.keep, mover = kept && t >= a.keep;
     const uint64_t bh = __ballot(hole), bm = __ballot(mover);
     const int x = ih + __popcll(bh & below), y = im + __popcll(bm & below);
-    if (hole && x < pairs) holes[x] = t;
-    if (mover && y < pairs) movers[y] = t;
+    if (hole && x < pairs) put_hole(x, i);
+    if (mover && y < pairs) put_mover(y, i);
     ih += __popcll(bh);
     im += __popcll(bm);
   }
@@ -325,22 +324,29 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
     all[j] = wave_sum(x);
     before[j] = wave_sum(lane < wave ? x : 0);
   }
-  const int pairs = evict_list<R>(a, u, key, t0, end, top, need, before, all);
   if constexpr (MOVE) {
-    __threadfence_block();
-    __syncthreads();  // the lists, written and read by this workgroup
+    // the pairs' rows stay in LDS, in the histograms' place
+    int64_t* const holes = reinterpret_cast<int64_t*>(&s_hist[0][0]);
+    int64_t* const movers = holes + kEvictPairs;
+    const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = at[r]; },
+                                    [&](int i, int r) { movers[i] = at[r]; });
+    __syncthreads();
     const int lpr = row_bytes / 16;
-    const int64_t list = u * a.moves;
-    for (int i = tid; i < pairs * lpr; i += kEvictThreads)
-      evict_move(a, trow, h, a.holes[list + i / lpr], a.movers[list + i / lpr], i % lpr, row_bytes);
-  } else if (tid == 0) {
-    a.counts[u] = pairs;
+    for (int i = tid; i < pairs * lpr; i += kEvictThreads) evict_move(a, holes[i / lpr], movers[i / lpr], i % lpr, row_bytes);
+  } else {
+    int32_t* const holes = a.holes + u * a.moves;
+    int32_t* const movers = a.movers + u * a.moves;
+    const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
+                                    [&](int i, int r) { movers[i] = t0 + 64 * r; });
+    if (tid == 0) a.counts[u] = pairs;
   }
 }
 
 // The same for longer units, which one compute unit's instruction rate would bound (32767 slots of 16
 // units took it 87 us, 65535 of one 160): a workgroup per chunk of kEvictChunk slots, a launch for
-// each time that the workgroups have to meet.  STEP 0: the chunk's newest position, and the unit's
+// each time that the workgroups have to meet.  Every launch costs its 4 us whatever it does, so a chunk
+// is what one workgroup of four waves does in that time: 28 us in all for both sizes with 1024 slots,
+// 48 with 4096.  STEP 0: the chunk's newest position, and the unit's
 // histograms cleared.  1: keys and the first digit's histogram.  2, 3: the second's and third's.
 // 4: the chunk's counts.  5: its part of the lists.
 template <int STEP>
@@ -379,7 +385,8 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
       last = wave_max(last);
       if (lane == 0) s_wave[0][wave] = last;
       __syncthreads();
-      if (tid == 0) newest[chunk] = max(max(s_wave[0][0], s_wave[0][1]), max(s_wave[0][2], s_wave[0][3]));
+      last = wave_max(s_wave[0][lane & (NW - 1)]);
+      if (tid == 0) newest[chunk] = last;
       return;
     }
     int last = kNoPosition;
@@ -430,7 +437,11 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
       for (int j = 0; j < 4; ++j) s_wave[j][wave] = sum[j];
     __syncthreads();
     if constexpr (STEP == 4) {
-      if (tid < 4) tally[chunk * 4 + tid] = s_wave[tid][0] + s_wave[tid][1] + s_wave[tid][2] + s_wave[tid][3];
+      if (tid < 4) {
+        int all = 0;
+        for (int i = 0; i < NW; ++i) all += s_wave[tid][i];
+        tally[chunk * 4 + tid] = all;
+      }
     } else {
       int before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
       for (int i = lane; i < chunks; i += 64)
@@ -446,7 +457,10 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
         before[j] = wave_sum(before[j]);
         for (int i = 0; i < wave; ++i) before[j] += s_wave[j][i];
       }
-      const int pairs = evict_list<R>(a, u, key, t0, end, top, need, before, all);
+      int32_t* const holes = a.holes + u * a.moves;
+      int32_t* const movers = a.movers + u * a.moves;
+      const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
+                                      [&](int i, int r) { movers[i] = t0 + 64 * r; });
       if (chunk == 0 && tid == 0) a.counts[u] = pairs;
     }
   }
@@ -461,7 +475,8 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a, int 
   const int32_t* const trow = a.table + int64_t(b) * a.width;
   for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < int64_t(count) * lpr; t += int64_t(gridDim.x) * 256) {
     const int64_t i = u * a.moves + t / lpr;
-    evict_move(a, trow, h, a.holes[i], a.movers[i], int(t % lpr), row_bytes);
+    evict_move(a, paged_row(a.c, trow, a.width, h, a.holes[i]), paged_row(a.c, trow, a.width, h, a.movers[i]), int(t % lpr),
+               row_bytes);
   }
 }
 
@@ -602,7 +617,7 @@ extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, in
   if (z.chunks == 0) {
     // Up to kEvictFused bytes of a unit are moved by the workgroup that chose them.  The lengths can
     // then be written there too, unless other heads' workgroups still read them.
-    const bool move = z.moves * row_bytes <= kEvictFused && new_lens != lens;
+    const bool move = z.moves * row_bytes <= kEvictFused && z.moves <= kEvictPairs && new_lens != lens;
     if (move)
       WZ_LAUNCH("paged_evict", stream, paged_evict_small_kernel<true>, dim3{units}, dim3(kEvictThreads), 0, a, row_bytes);
     else
