@@ -5,8 +5,9 @@
 // taken in groups of up to 64; a group of a sequence is a unit, and its n cached tokens are granules
 // of 32.  All units' granules in a row are cut into one equal share per worker, so the chip is filled
 // whatever the lengths: a unit inside one share is finished there, a cut one leaves (m, l, O) partials
-// that paged_attn_join_kernel merges.  A worker's share holds at most two cut units, its first and its
-// last, which own its partial slots 2w and 2w + 1; the worker that a cut unit begins in says so.
+// that paged_attn_join_kernel merges.  A worker's share holds at most two cut units, one
+// that began before it and one that goes on after it, which own its partial slots 2w and 2w + 1; the
+// worker that a cut unit begins in says so.
 //
 // A worker is one wave, or two that split 64 rows (RH = 2) and the loads.  One wave waits for nobody:
 // while it begins a unit or ends one, the compute unit's other workers keep loading.  Tiles of 32 tokens
@@ -39,11 +40,11 @@ constexpr int kPagedTile = 32;           // tokens of a wave's tile
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kPagedLazy = 8.0f;       // the running maximum moves when a tile exceeds it by more
 constexpr int kPagedMaxS = 16;
+constexpr int kPagedStart = 3;           // a worker's start of a unit, in tiles (paged_cost)
 
-// A unit's parts: np of them (1: nothing to join, 0: no unit), the first in partial slot `slot`, the
-// others in the first slots of the workers after it.
+// A unit's parts: np of them (1: nothing to join, 0: no unit), of worker w and those after it.
 struct PagedCut {
-  int32_t b, u, np, slot;
+  int32_t b, u, np, w;
 };
 
 struct PagedAttnArgs {
@@ -73,14 +74,23 @@ __device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
   return int(min(int64_t(max(a.lens[b], 0)), a.capacity));
 }
 
-// All granules: upb units a sequence, each of ceil(n / G) (the host has checked that they fit 31 bits).
-// Every lane of a wave gets the result; B sequences are summed 64 at a time.
-template <int G>
+// What a unit of n tokens counts for: its granules of G, and START more for the time in which a worker
+// loads nothing (the query, the pages' ids, the first tile's way).  64 sequences of 16 to 16384 tokens took
+// 133 us with START = 0, since some worker had to begin a dozen short ones, and 118 with 3 (128, 119, 118
+// with 1, 2, 4).
+template <int G, int START>
+__device__ __forceinline__ int paged_cost(int n) {
+  return n > 0 ? (n + G - 1) / G + START : 0;
+}
+
+// All of that: upb units a sequence (the host has checked that it fits 31 bits).  Every lane of a wave
+// gets the result; B sequences are summed 64 at a time.
+template <int G, int START>
 __device__ __forceinline__ int paged_total(const PagedAttnArgs& a, int upb) {
   const int lane = threadIdx.x & 63;
   int sum = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int g = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
+    int g = b0 + lane < a.B ? paged_cost<G, START>(paged_len(a, b0 + lane)) : 0;
     for (int o = 1; o < 64; o <<= 1) g += __shfl_xor(g, o, 64);
     sum += g;
   }
@@ -88,12 +98,12 @@ __device__ __forceinline__ int paged_total(const PagedAttnArgs& a, int upb) {
 }
 
 // The sequence that holds granule x (0 <= x < total) and the granules before it.
-template <int G>
+template <int G, int START>
 __device__ __forceinline__ void paged_find(const PagedAttnArgs& a, int upb, int x, int* seq, int* before) {
   const int lane = threadIdx.x & 63;
   int sum = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int g = b0 + lane < a.B ? (paged_len(a, b0 + lane) + G - 1) / G : 0;
+    const int g = b0 + lane < a.B ? paged_cost<G, START>(paged_len(a, b0 + lane)) : 0;
     int inc = g;
     for (int o = 1; o < 64; o <<= 1) {
       const int y = __shfl_up(inc, o, 64);
@@ -277,7 +287,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
 
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
   const int w = blockIdx.x;
-  const PagedShares shares(paged_total<kPagedTile>(a, upb), a.W);
+  const PagedShares shares(paged_total<kPagedTile, kPagedStart>(a, upb), a.W);
   if (!a.by_unit && tid == 0) a.cut[w] = PagedCut{0, 0, 0, 0};
   if (w >= shares.workers) {
     paged_empty(a, w, upb, D, 64 * RH);
@@ -286,19 +296,35 @@ void paged_attn_kernel(PagedAttnArgs a) {
   int x = shares.begin(w);
   const int x_end = shares.begin(w + 1);
   int b, before;  // sequence, and the granules before it
-  paged_find<kPagedTile>(a, upb, x, &b, &before);
-  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b)), gran = (n + kPagedTile - 1) / kPagedTile;
-  int u = (x - before) / gran, ubeg = before + u * gran;  // unit of the sequence
+  paged_find<kPagedTile, kPagedStart>(a, upb, x, &b, &before);
+  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b)), cost = paged_cost<kPagedTile, kPagedStart>(n);
+  int u = (x - before) / cost, ubeg = before + u * cost;  // unit of the sequence, and where it begins
   const int ps = a.c.shift, page = a.c.page;
   const int ish = page >= kPagedTile ? 0 : 1;  // page ids a tile: 1 or 2
 
-  for (bool first_piece = true; x < x_end; first_piece = false) {
+  auto next = [&] {  // the next unit that holds anything
+    ubeg += cost;
+    if (ubeg >= x_end) return false;
+    x = ubeg;
+    if (++u == upb) {
+      do {
+        ++b;
+        n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+      } while (n == 0);
+      cost = paged_cost<kPagedTile, kPagedStart>(n);
+      u = 0;
+    }
+    return true;
+  };
+  for (bool more = true; more; more = next()) {
     // the lane's coordinates, made anew for each part: addresses computed from them stay inside it
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));
     const int nl = lane & 15, g = lane >> 4;
-    const int g0 = x - ubeg, g1 = min(x_end - ubeg, gran);
-    const bool whole = g0 == 0 && g1 == gran;
+    // this worker's granules of the unit
+    const int g0 = max(x - ubeg - kPagedStart, 0), g1 = min(x_end - ubeg, cost) - kPagedStart;
+    if (g1 <= 0) continue;
+    const bool whole = g0 == 0 && g1 == cost - kPagedStart;
     const int hk = u / RG, rg = u - hk * RG;
     const int row0 = rg * ROWS + rh * C::WROWS;  // this wave's first row
     const int t0 = g0 * kPagedTile, tm = min(g1 * kPagedTile, n);
@@ -308,7 +334,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
     int odd0 = 0, odd1 = 0;  // those tokens
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
       a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
-          PagedCut{b, u, whole ? 1 : shares.owner(ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
+          PagedCut{b, u, whole ? 1 : shares.owner(ubeg + cost - 1) - w + 1, w};
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
     // Q fragments: lane (row nl, group g); e4m3 rows are read 16 codes at a time, so there the
@@ -613,7 +639,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
       l_run[rt] += __shfl_xor(l_run[rt], 32, 64);
     }
     {
-      float* const part = a.part + (first_piece ? 2 * int64_t(w) : 2 * int64_t(w) + 1) * (int64_t(a.rows) * (D + 2));
+      float* const part = a.part + (2 * int64_t(w) + (g0 == 0 ? 1 : 0)) * (int64_t(a.rows) * (D + 2));
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int rl = rh * C::WROWS + 16 * rt + nl, r = rg * ROWS + rl;
@@ -652,17 +678,6 @@ void paged_attn_kernel(PagedAttnArgs a) {
       }
     }
     meet();  // the ring is free for the next part's tiles
-    x = ubeg + g1;
-    if (g1 < gran) break;
-    ubeg += gran;
-    if (++u == upb && x < x_end) {  // the next sequence that holds anything
-      do {
-        ++b;
-        n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-      } while (n == 0);
-      gran = (n + kPagedTile - 1) / kPagedTile;
-      u = 0;
-    }
   }
   paged_empty(a, w, upb, D, 64 * RH);
 }
@@ -687,7 +702,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
   if (rl >= a.rows || r >= R) return;  // WIDE: the whole workgroup
   const int64_t slot = int64_t(a.rows) * (D + 2);
   const float* const part = a.part + rl;
-  auto at = [&](int j) { return part + (j == 0 ? int64_t(cut.slot) : 2 * (int64_t(cut.slot >> 1) + j)) * slot; };
+  auto at = [&](int j) { return part + (2 * (int64_t(cut.w) + j) + (j == 0 ? 1 : 0)) * slot; };
   const int head = hk * grp + r % grp;
   const float sk = a.sink ? a.sink[head] * kLog2e : -INFINITY;
   const int off = 2 * a.rows + rl * (D - 1) + 4 * ch;

@@ -94,7 +94,7 @@ extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const
   const int64_t R = S * (H / a.c.heads);
   if (B * a.c.heads * R > 0x7FFFFFFFLL || B * a.c.heads > 65535 * int64_t(accumulate ? 1 : 65535))
     return set_error(WZ_EINVAL, "paged_attn: %lld sequences of %lld heads", (long long)B, (long long)H);
-  if (B * a.c.heads * ((R + 15) / 16) > 0x7FFFFFFFLL / std::max<int64_t>(1, table_width * a.c.page / 16))
+  if (B * a.c.heads * ((R + 15) / 16) > 0x7FFFFFFFLL / (table_width * a.c.page / kPagedTile + 8))
     return set_error(WZ_EINVAL, "paged_attn: %lld sequences of up to %lld slots", (long long)B,
                      (long long)(table_width * a.c.page));
   if (2 * R * int64_t(sizeof(float)) > 65536)

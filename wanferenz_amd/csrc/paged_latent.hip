@@ -16,7 +16,7 @@
 
 namespace wz {
 
-constexpr int kLatentD = 512, kLatentTile = 64, kLatentWaves = 8;
+constexpr int kLatentD = 512, kLatentTile = 64, kLatentWaves = 8, kLatentStart = 4;
 
 template <bool FP8>
 struct LatentCfg {
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
 
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
   const int w = blockIdx.x;
-  const PagedShares shares(paged_total<T>(a, upb), a.W);
+  const PagedShares shares(paged_total<T, kLatentStart>(a, upb), a.W);
   if (!a.by_unit && tid == 0) a.cut[w] = PagedCut{0, 0, 0, 0};
   if (w >= shares.workers) {
     paged_empty(a, w, upb, D, 64 * kLatentWaves);
@@ -64,25 +64,41 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
   int x = shares.begin(w);
   const int x_end = shares.begin(w + 1);
   int b, before;  // sequence, and the granules before it
-  paged_find<T>(a, upb, x, &b, &before);
-  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b)), gran = (n + T - 1) / T;
-  int u = (x - before) / gran, ubeg = before + u * gran;  // unit of the sequence
+  paged_find<T, kLatentStart>(a, upb, x, &b, &before);
+  int n = __builtin_amdgcn_readfirstlane(paged_len(a, b)), cost = paged_cost<T, kLatentStart>(n);
+  int u = (x - before) / cost, ubeg = before + u * cost;  // unit of the sequence, and where it begins
   const int ps = a.c.shift, page = a.c.page;
 
-  for (bool first_piece = true; x < x_end; first_piece = false) {
+  auto next = [&] {  // the next unit that holds anything
+    ubeg += cost;
+    if (ubeg >= x_end) return false;
+    x = ubeg;
+    if (++u == upb) {
+      do {
+        ++b;
+        n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+      } while (n == 0);
+      cost = paged_cost<T, kLatentStart>(n);
+      u = 0;
+    }
+    return true;
+  };
+  for (bool more = true; more; more = next()) {
     // the lane's coordinates, made anew for each part: addresses computed from them stay inside it
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));
     const int nl = lane & 15, g = lane >> 4;
-    const int g0 = x - ubeg, g1 = min(x_end - ubeg, gran);
-    const bool whole = g0 == 0 && g1 == gran;
+    // this worker's granules of the unit
+    const int g0 = max(x - ubeg - kLatentStart, 0), g1 = min(x_end - ubeg, cost) - kLatentStart;
+    if (g1 <= 0) continue;
+    const bool whole = g0 == 0 && g1 == cost - kLatentStart;
     const int hk = u / RG, rg = u - hk * RG, row0 = rg * ROWS;
     const int t0 = g0 * T, tm = min(g1 * T, n);
     const int n0 = n - a.S + 1;  // from here on a token is seen by some rows only, as in paged_attn_kernel
     int odd0 = 0, odd1 = 0;
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
       a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
-          PagedCut{b, u, whole ? 1 : shares.owner(ubeg + gran - 1) - w + 1, 2 * w + (first_piece ? 0 : 1)};
+          PagedCut{b, u, whole ? 1 : shares.owner(ubeg + cost - 1) - w + 1, w};
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
     v4f acc[HT][NT];  // acc[ht][nt][i] = O[row 16ht + nl][64 wave + 16nt + 4g + i]
@@ -465,7 +481,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
                                                                  f32x2_to_bf16x2(acc[ht][nt][2] * iv, acc[ht][nt][3] * iv));
       }
     } else {
-      float* const part = a.part + (first_piece ? 2 * int64_t(w) : 2 * int64_t(w) + 1) * (int64_t(a.rows) * (D + 2));
+      float* const part = a.part + (2 * int64_t(w) + (g0 == 0 ? 1 : 0)) * (int64_t(a.rows) * (D + 2));
       if (wave == 0 && lane < ROWS && row0 + lane < R) {
         part[lane] = m_run;
         part[a.rows + lane] = l;
@@ -480,17 +496,6 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       }
     }
     meet();  // the buffers are free for the next part's tiles
-    x = ubeg + g1;
-    if (g1 < gran) break;
-    ubeg += gran;
-    if (++u == upb && x < x_end) {  // the next sequence that holds anything
-      do {
-        ++b;
-        n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-      } while (n == 0);
-      gran = (n + T - 1) / T;
-      u = 0;
-    }
   }
   paged_empty(a, w, upb, D, 64 * kLatentWaves);
 }
