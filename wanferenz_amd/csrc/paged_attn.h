@@ -255,14 +255,16 @@ struct PagedCfg {
   static constexpr int SIDE = kPagedTile * RB;                 // one side of a tile
   static constexpr int STAGE = SIDE * (SHARED ? 1 : 2);
   static constexpr int SCALES = FP8 ? 256 : 0;                 // a tile's K and V scales
-  static constexpr int NS = STAGE <= 4096 ? 4 : 2;
+  static constexpr int NS = 2;                                 // one being read, one on its way
   static constexpr int LOADS = STAGE / 1024 / RH + (FP8 ? 1 : 0);  // a wave's loads of a tile
   static constexpr int WROWS = 16 * RT;                        // rows of a wave
   static constexpr int ROWS = WROWS * RH;                      // rows of a unit
   static constexpr int RING = NS * (STAGE + SCALES);
   static constexpr int LDS = RING + RH * NS * 4;               // valid masks
-  // waves a SIMD: O and Q take 3 RT D / 8 registers of a lane
-  static constexpr int EU = 3 * RT * D / 8 <= 112 ? 2 : 1;
+  // Waves a SIMD.  One of tiles of 8 KB and more keeps the memory busy, and a second adds partial results:
+  // 48 sequences of 9001 tokens, 64 heads on 8, us with one / two: bf16 of 64 157 / 160, e4m3 of 128
+  // 164 / 172; tiles of 4 KB need two: e4m3 of 64 111 / 91 (rings of four tiles 109 / 95).
+  static constexpr int EU = STAGE <= 4096 ? 2 : 1;
   static constexpr int PER_CU = 160 * 1024 / LDS < 4 * EU / RH ? 160 * 1024 / LDS : 4 * EU / RH;
   static_assert(NS >= 2 && (NS - 1) * LOADS < 64, "the waits count the loads in flight");
   static_assert(PER_CU >= 1 && SIDE / 1024 % RH == 0, "a worker fits, and its waves share a tile's loads evenly");
