@@ -46,44 +46,68 @@ struct WriteArgs {
   const uint16_t* src[2];
   int64_t sb[2], ss[2], sh[2];
   const int32_t *table, *start, *count, *position;
-  int width, S;
-  int64_t rows;  // B * S * heads
+  int width, B, S, block;  // block: tokens of a workgroup
 };
 
-// A thread per 16 bytes of a new row, D / 8 threads a row; heads of one token are neighbours, as
-// they are in the projection's output.  An e4m3 row's amax is the maximum over its threads, its
-// scale and codes act_quant's (act_scale, quant_div) over the whole row.  blockIdx.y: K, V.
+// A workgroup takes a few new tokens of a sequence (`block`: 512 pieces of 16 bytes, if the batch has as
+// many), D / 8 threads a row and a token's heads next to each other, so whole lines of the projection's
+// rows are read.  An e4m3 row's amax is the maximum over its threads, its scale and codes act_quant's
+// (act_scale, quant_div) over the whole row.  blockIdx.z: K, V.  Two loads of a thread are in flight
+// together: 2 x 32767 tokens of 8 heads of 128 (537 MB) 116 us, with one 123, with four 164, since fewer
+// workgroups are left to hide a load's way.  Nothing is read twice here, so loads and stores pass the
+// caches by: 109 us, 4.9 TB/s, as a large copy.
+constexpr int kWriteLoads = 2;
+
 template <int D, bool FP8>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedView c, WriteArgs a) {
-  constexpr int LPR = D / 8;
-  const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = t / LPR;
-  const int ch = int(t % LPR), side = blockIdx.y;
-  if (row >= a.rows) return;
-  const int h = int(row % c.heads), i = int(row / c.heads % a.S), b = int(row / c.heads / a.S);
-  if (a.count && i >= a.count[b]) return;
-  const int64_t slot64 = int64_t(a.start[b]) + i;
-  if (slot64 < 0 || slot64 > 0x7FFFFFFFLL) return;
-  const int slot = int(slot64);
-  const int64_t at = paged_row(c, a.table + int64_t(b) * a.width, a.width, h, slot);
-  if (at < 0) return;
-  const v4i x = load16(a.src[side] + b * a.sb[side] + i * a.ss[side] + h * a.sh[side] + ch * 8);
+  constexpr int LPR = D / 8, N = kWriteLoads;
+  const int side = blockIdx.z, i0 = blockIdx.x * a.block;
   uint8_t* const dst = side ? c.v : c.k;
-  if constexpr (!FP8) {
-    *reinterpret_cast<v4i*>(dst + (at * D + ch * 8) * 2) = x;
-  } else {
-    float m = bf16x8_absmax(x);
+  const uint32_t per = uint32_t(c.heads) * LPR;  // 16-byte pieces of a token
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    const int count = a.count ? min(a.count[b], a.S) : a.S;
+    const int tokens = min(count - i0, a.block);
+    if (tokens <= 0) continue;
+    const int start = a.start[b];
+    const int32_t* const trow = a.table + int64_t(b) * a.width;
+    const uint16_t* const src = a.src[side] + b * a.sb[side] + i0 * a.ss[side];
+    const uint32_t pieces = uint32_t(tokens) * per;  // up to 16 x 1024 x 64
+    for (uint32_t p0 = 0; p0 < pieces; p0 += 256 * N) {
+      v4i x[N];
+      int64_t at[N];
 #pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) m = wave_absmax_xor(m, o);
-    const ActScale sc = act_scale(m, false);
-    float f[8];
-    bf16x8_unpack(x, f);
-    *reinterpret_cast<uint2*>(dst + at * D + ch * 8) = quant8(f, sc, false, false);
-    if (ch == 0) (side ? c.vs : c.ks)[at] = sc.s;
-  }
-  if (side == 0 && ch == 0 && c.weights) {
-    c.weights[at] = 0.0f;
-    c.positions[at] = (a.position ? a.position[b] : a.start[b]) + i;
+      for (int j = 0; j < N; ++j) {
+        const uint32_t p = p0 + 256 * j + threadIdx.x;
+        at[j] = -1;
+        if (p >= pieces) continue;
+        const uint32_t i = p / per, hc = p - i * per, h = hc / LPR, ch = hc % LPR;
+        const int64_t slot = int64_t(start) + i0 + int(i);
+        if (slot > 0x7FFFFFFFLL) continue;
+        at[j] = paged_row(c, trow, a.width, int(h), int(slot));
+        if (at[j] >= 0) x[j] = load16_nt(src + i * a.ss[side] + h * a.sh[side] + ch * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (at[j] < 0) continue;  // the same in a row's threads
+        const uint32_t p = p0 + 256 * j + threadIdx.x, ch = p % LPR;
+        if constexpr (!FP8) {
+          __builtin_nontemporal_store(x[j], reinterpret_cast<v4i*>(dst + (at[j] * D + ch * 8) * 2));
+        } else {
+          float m = bf16x8_absmax(x[j]);
+#pragma unroll
+          for (int o = 1; o < LPR; o <<= 1) m = wave_absmax_xor(m, o);
+          const ActScale sc = act_scale(m, false);
+          float f[8];
+          bf16x8_unpack(x[j], f);
+          *reinterpret_cast<uint2*>(dst + at[j] * D + ch * 8) = quant8(f, sc, false, false);
+          if (ch == 0) (side ? c.vs : c.ks)[at[j]] = sc.s;
+        }
+        if (side == 0 && ch == 0 && c.weights) {
+          c.weights[at[j]] = 0.0f;
+          c.positions[at[j]] = (a.position ? a.position[b] : start) + i0 + int(p / per);
+        }
+      }
+    }
   }
 }
 
@@ -194,7 +218,8 @@ __device__ __forceinline__ void evict_pick(const int32_t* hist, int* bin, int* n
   }
   if (lane == 63) s_sum[wave] = up;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) up += s_sum[i];
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) up += i < wave ? s_sum[i] : 0;
   int before = up - sum;
   // the keys are at least `want` in all, so one thread has the crossing (none wanted: the topmost bin)
   if ((up >= want && before < want) || (want == 0 && tid == 0)) {
@@ -270,7 +295,8 @@ template <bool MOVE>
 __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictArgs a, int row_bytes) {
   constexpr int R = kEvictSmall / kEvictThreads, NW = kEvictThreads / 64;
   __shared__ int s_hist[3][kEvictBins];
-  __shared__ int s_wave[4][NW];
+  __shared__ int s_last[NW];
+  __shared__ __align__(16) uint2 s_count[NW];
   const int u = blockIdx.x, b = u / a.c.heads, h = u - b * a.c.heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t* const trow = a.table + int64_t(b) * a.width;
@@ -292,9 +318,10 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
 #pragma unroll
   for (int i = 0; i < R; ++i) last = max(last, p[i]);
   last = wave_max(last);
-  if (lane == 0) s_wave[0][wave] = last;
+  if (lane == 0) s_last[wave] = last;
   __syncthreads();
-  last = wave_max(s_wave[0][lane & (NW - 1)]);
+  #pragma unroll
+  for (int i = 0; i < NW; ++i) last = max(last, s_last[i]);
   const int64_t old = int64_t(last) - a.recent;  // positions above it are protected
   uint32_t key[R];
 #pragma unroll
@@ -313,17 +340,18 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
   }
   int sum[4] = {0, 0, 0, 0};
   evict_count<R>(key, t0, end, a.keep, top, sum);
-  if (lane == 0)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s_wave[j][wave] = sum[j];
+  // two counts a word: they add up to kEvictSmall at most
+  if (lane == 0) s_count[wave] = make_uint2(uint32_t(sum[0]) << 16 | uint32_t(sum[1]), uint32_t(sum[2]) << 16 | uint32_t(sum[3]));
   __syncthreads();
-  int before[4], all[4];
+  uint2 total = make_uint2(0, 0), mine = total;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int x = lane < NW ? s_wave[j][lane] : 0;
-    all[j] = wave_sum(x);
-    before[j] = wave_sum(lane < wave ? x : 0);
+  for (int i = 0; i < NW; ++i) {
+    const uint2 x = s_count[i];
+    mine = i == wave ? total : mine;
+    total = make_uint2(total.x + x.x, total.y + x.y);
   }
+  const int before[4] = {int(mine.x >> 16), int(mine.x & 0xFFFF), int(mine.y >> 16), int(mine.y & 0xFFFF)};
+  const int all[4] = {int(total.x >> 16), int(total.x & 0xFFFF), int(total.y >> 16), int(total.y & 0xFFFF)};
   if constexpr (MOVE) {
     // the pairs' rows stay in LDS, in the histograms' place
     int64_t* const holes = reinterpret_cast<int64_t*>(&s_hist[0][0]);
@@ -538,13 +566,13 @@ extern "C" int wz_paged_kv_write(const wz_paged_kv* cache, const void* k_bf16, c
   a.position = position;
   a.width = int(table_width);
   a.S = int(S);
+  a.B = int(B);
   if (B > (int64_t(1) << 40) / (S * c.heads))
     return set_error(WZ_EINVAL, "paged_kv_write: %lld x %lld tokens", (long long)B, (long long)S);
-  a.rows = B * S * c.heads;
   const int D = cache->head_dim;
-  const int64_t blocks = (a.rows * (D / 8) + 255) / 256;
-  if (blocks > 0x7FFFFFFFLL) return set_error(WZ_EINVAL, "paged_kv_write: %lld x %lld tokens", (long long)B, (long long)S);
-  const dim3 grid{unsigned(blocks), c.shared ? 1u : 2u};
+  a.block = std::max(1, 256 * kWriteLoads / (c.heads * (D / 8)));
+  const dim3 grid(unsigned((S + a.block - 1) / a.block), unsigned(std::min<int64_t>(B, 65535)),
+                  c.shared ? 1u : 2u);
 #define WZ_PAGED_WRITE(DD)                                                                                    \
   do {                                                                                                        \
     if (c.ks)                                                                                                 \
