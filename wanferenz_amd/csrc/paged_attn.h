@@ -691,16 +691,16 @@ void paged_attn_kernel(PagedAttnArgs a) {
 constexpr int kPagedMaxWorkers = 4096;
 
 template <int D, bool WIDE>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
+__device__ __forceinline__ void paged_join(const PagedAttnArgs& a, int unit, int rows) {
   constexpr int CH = D / 4, GR = 256 / CH;
-  const PagedCut cut = a.cut[blockIdx.x];
+  const PagedCut cut = a.cut[unit];
   const int np = cut.np;
   if (np < 2) return;
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + a.unit_rows - 1) / a.unit_rows;
   const int hk = cut.u / RG, rg = cut.u - hk * RG, b = cut.b;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int ch = tid % CH, gr = tid / CH;
-  const int rl = WIDE ? blockIdx.y : blockIdx.y * GR + gr, r = rg * a.unit_rows + rl;
+  const int rl = WIDE ? rows : rows * GR + gr, r = rg * a.unit_rows + rl;
   if (rl >= a.rows || r >= R) return;  // WIDE: the whole workgroup
   const int64_t slot = int64_t(a.rows) * (D + 2);
   const float* const part = a.part + rl;
@@ -766,17 +766,135 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
   }
 }
 
+template <int D, bool WIDE>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
+  paged_join<D, WIDE>(a, blockIdx.x, blockIdx.y);
+}
+
+// weights[slot] += sum over the KV head's rows that see the slot of 2^(y - m) / sum, rows in ascending
+// order.  A workgroup takes kWeighSlots slots of a head, four a thread.  Its bound is the launch: 4.3 us at 16 x
+// 3000 tokens of 8 heads, one slot a thread 7.7.  JOIN: the rows' m and sum come from the cut units'
+// partials, 16 threads a row, so that one launch does the join as well; that is for up to kWeighRows rows a KV
+// head, which the workgroup takes at once (4 rows: 5.6 us against 8.5 in two launches, 131071 tokens 9.4 against 11.8;
+// 64 rows 22.9 against 20.2).
+constexpr int kWeighSlots = 1024;
+constexpr int kWeighRows = 16;
+
+template <int D, bool JOIN>
+__device__ __forceinline__ void paged_weigh(const PagedAttnArgs& a, int bh, int block, float* s_ml) {
+  const int b = bh / a.c.heads, hk = bh - b * a.c.heads;
+  const int grp = a.H / a.c.heads, R = a.S * grp;
+  const int n = paged_len(a, b);
+  const int t = block * kWeighSlots + 4 * threadIdx.x;
+  if (block * kWeighSlots >= n) return;
+  const float* const ml = a.ml + 2 * int64_t(bh) * R;
+  if constexpr (JOIN) {
+    const int upb = (R + a.unit_rows - 1) / a.unit_rows, li = threadIdx.x & 15;
+    for (int r = threadIdx.x >> 4; r < R; r += 16) {  // 16 threads a row
+      const int u = r / a.unit_rows, rl = r - u * a.unit_rows;
+      const PagedCut cut = a.cut[int64_t(bh) * upb + u];
+      float m, inv;
+      if (cut.np < 2) {
+        m = ml[2 * r];
+        inv = ml[2 * r + 1];
+      } else {
+        const int64_t slot = int64_t(a.rows) * (D + 2);
+        const float* const part = a.part + rl;
+        auto at = [&](int j) { return part + (2 * (int64_t(cut.w) + j) + (j == 0 ? 1 : 0)) * slot; };
+        const float sk = a.sink ? a.sink[hk * grp + r % grp] * kLog2e : -INFINITY;
+        float M = -INFINITY, l = 0.0f;  // of this thread's partials
+        for (int j = li; j < cut.np; j += 16) {
+          const float mj = at(j)[0], lj = at(j)[a.rows], Mn = fmaxf(M, mj), e = Mn == -INFINITY ? 0.0f : Mn;
+          l = l * __builtin_amdgcn_exp2f(M - e) + lj * __builtin_amdgcn_exp2f(mj - e);
+          M = Mn;
+        }
+        m = fmaxf(M, sk);
+        for (int i = 1; i < 16; i <<= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+        m = m == -INFINITY ? 0.0f : m;
+        l *= __builtin_amdgcn_exp2f(M - m);
+        for (int i = 1; i < 16; i <<= 1) l += __shfl_xor(l, i, 64);
+        if (a.sink) l += __builtin_amdgcn_exp2f(sk - m);
+        inv = l == 0.0f ? 0.0f : 1.0f / l;
+      }
+      if (li == 0) {
+        s_ml[2 * r] = m;
+        s_ml[2 * r + 1] = inv;
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < 2 * R; i += 256) s_ml[i] = ml[i];
+  }
+  __syncthreads();
+  if (t >= n) return;
+  const int64_t at = paged_row(a.c, a.table + int64_t(b) * a.width, a.width, hk, t);  // of four slots of one page
+  if (at < 0) return;
+  const float* const y = a.scores + int64_t(bh) * R * a.capacity + t;
+  v4f sum = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int r = 0; r < R; ++r) {
+    const v4f v = *reinterpret_cast<const v4f*>(y + r * a.capacity);
+    const int seen = n - (a.S - 1 - r / grp) - t;  // of the four
+    const float m = s_ml[2 * r], inv = s_ml[2 * r + 1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += i < seen ? __builtin_amdgcn_exp2f(v[i] - m) * inv : 0.0f;
+  }
+  float* const w = a.c.weights + at;
+  if (t + 4 <= n) {
+    *reinterpret_cast<v4f*>(w) += sum;
+  } else {
+    for (int i = 0; t + i < n; ++i) w[i] += sum[i];
+  }
+}
+
+// The join and the weights in one launch.
+template <int D, bool WIDE>
+__global__ __launch_bounds__(256) void paged_attn_end_kernel(PagedAttnArgs a, int units, int row_blocks, int slot_blocks) {
+  extern __shared__ float s_ml[];
+  const int joins = units * row_blocks, block = blockIdx.x;
+  if (block < joins) {
+    paged_join<D, WIDE>(a, block / row_blocks, block % row_blocks);
+  } else {
+    const int i = block - joins;
+    paged_weigh<D, true>(a, i / slot_blocks, i % slot_blocks, s_ml);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void paged_attn_weigh_kernel(PagedAttnArgs a) {
+  extern __shared__ float s_ml[];
+  paged_weigh<D, false>(a, blockIdx.y, blockIdx.x, s_ml);
+}
+
+// What follows the main kernel: the join, and the weights.
 template <int D>
 int paged_attn_join(const PagedAttnArgs& a, hipStream_t stream) {
   constexpr int GR = 256 / (D / 4);
   const int64_t units = paged_units(a);
-  const unsigned n = unsigned(std::min<int64_t>(units, a.W));
-  if (8 * units <= a.W)
-    WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<D, true>), dim3(n, unsigned(a.rows)), dim3(256), 0, a);
+  const bool wide = 8 * units <= a.W;
+  const unsigned n = unsigned(std::min<int64_t>(units, a.W)), row_blocks = unsigned(wide ? a.rows : (a.rows + GR - 1) / GR);
+  const int64_t heads = int64_t(a.B) * a.c.heads, slot_blocks = (a.capacity + kWeighSlots - 1) / kWeighSlots;
+  const int64_t blocks = n * row_blocks + heads * slot_blocks;
+  const int R = a.S * (a.H / a.c.heads);
+  const size_t ml_bytes = 2 * sizeof(float) * R;
+  if (a.scores && a.by_unit && R <= kWeighRows && blocks <= 0x7FFFFFFF) {
+    if (wide)
+      WZ_LAUNCH("paged_attn_end", stream, (paged_attn_end_kernel<D, true>), dim3{unsigned(blocks)}, dim3(256), ml_bytes, a,
+                int(n), int(row_blocks), int(slot_blocks));
+    else
+      WZ_LAUNCH("paged_attn_end", stream, (paged_attn_end_kernel<D, false>), dim3{unsigned(blocks)}, dim3(256), ml_bytes, a,
+                int(n), int(row_blocks), int(slot_blocks));
+    return check_launch("paged_attn_end");
+  }
+  const dim3 grid(n, row_blocks);
+  if (wide)
+    WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<D, true>), grid, dim3(256), 0, a);
   else
-    WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<D, false>), dim3(n, unsigned((a.rows + GR - 1) / GR)),
-              dim3(256), 0, a);
-  return check_launch("paged_attn_join");
+    WZ_LAUNCH("paged_attn_join", stream, (paged_attn_join_kernel<D, false>), grid, dim3(256), 0, a);
+  if (int rc = check_launch("paged_attn_join")) return rc;
+  if (!a.scores || a.capacity == 0) return WZ_OK;
+  WZ_LAUNCH("paged_attn_weigh", stream, paged_attn_weigh_kernel<D>, dim3(unsigned(slot_blocks), unsigned(heads)), dim3(256),
+            ml_bytes, a);
+  return check_launch("paged_attn_weigh");
 }
 
 // The kernel of R rows a KV head: 16, 32 or 64 rows a unit.

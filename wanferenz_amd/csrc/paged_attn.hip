@@ -1,4 +1,4 @@
-// paged_attn: the kernels for bf16 rows, the weights' accumulation and the entry points.
+// paged_attn: the kernels for bf16 rows and the entry points.
 #include "paged_attn.h"
 
 namespace wz {
@@ -10,27 +10,6 @@ int paged_attn_bf16(int D, const PagedAttnArgs& a, bool ask, int* workers, hipSt
 static int paged_attn_any(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
   return a.c.dtype == WZ_KV_E4M3 ? paged_attn_e4m3(D, a, ask, workers, stream)
                                  : paged_attn_bf16(D, a, ask, workers, stream);
-}
-
-// weights[slot] += sum over the KV head's rows that see the slot of 2^(y - m) / sum, rows in
-// ascending order.  A thread per slot; blockIdx.y = (sequence, head).
-__global__ __launch_bounds__(256) void paged_attn_weigh_kernel(PagedAttnArgs a) {
-  extern __shared__ float s_ml[];
-  const int bh = blockIdx.y, b = bh / a.c.heads, hk = bh % a.c.heads;
-  const int grp = a.H / a.c.heads, R = a.S * grp;
-  const int n = paged_len(a, b);
-  if (int(blockIdx.x) * 256 >= n) return;
-  for (int i = threadIdx.x; i < 2 * R; i += 256) s_ml[i] = a.ml[2 * int64_t(bh) * R + i];
-  __syncthreads();
-  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < n; t += int64_t(gridDim.x) * 256) {
-    const int64_t at = paged_row(a.c, a.table + int64_t(b) * a.width, a.width, hk, int(t));
-    if (at < 0) continue;
-    const float* const y = a.scores + int64_t(bh) * R * a.capacity + t;
-    float sum = 0.0f;
-    for (int r = 0; r < R; ++r)
-      if (t < n - (a.S - 1 - r / grp)) sum += __builtin_amdgcn_exp2f(y[r * a.capacity] - s_ml[2 * r]) * s_ml[2 * r + 1];
-    a.c.weights[at] += sum;
-  }
 }
 
 struct PagedAttnSizes {
@@ -91,6 +70,8 @@ extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const
   if ((reinterpret_cast<uintptr_t>(q_bf16) | reinterpret_cast<uintptr_t>(o_bf16) |
        reinterpret_cast<uintptr_t>(workspace)) & 15 || ((q_strides[0] | q_strides[1] | q_strides[2]) & 7))
     return set_error(WZ_EINVAL, "paged_attn: q rows, o and the workspace must be 16-byte aligned");
+  if (accumulate && reinterpret_cast<uintptr_t>(a.c.weights) & 15)
+    return set_error(WZ_EINVAL, "paged_attn: weights must be 16-byte aligned");
   const int64_t R = S * (H / a.c.heads);
   if (B * a.c.heads * R > 0x7FFFFFFFLL || B * a.c.heads > 65535 * int64_t(accumulate ? 1 : 65535))
     return set_error(WZ_EINVAL, "paged_attn: %lld sequences of %lld heads", (long long)B, (long long)H);
@@ -122,10 +103,5 @@ extern "C" int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const
   a.H = int(H);
   a.capacity = table_width * a.c.page;
   a.scale2 = softmax_scale * kLog2e;
-  const int rc = paged_attn_any(cache->head_dim, a, false, nullptr, stream);
-  if (rc != WZ_OK || !accumulate || a.capacity == 0) return rc;
-  const int64_t blocks = std::min<int64_t>((a.capacity + 255) / 256, 1024);
-  WZ_LAUNCH("paged_attn_weigh", stream, paged_attn_weigh_kernel, dim3(unsigned(blocks), unsigned(B * a.c.heads)),
-            dim3(256), 2 * R * sizeof(float), a);
-  return check_launch("paged_attn_weigh");
+  return paged_attn_any(cache->head_dim, a, false, nullptr, stream);
 }
