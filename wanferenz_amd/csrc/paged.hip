@@ -120,6 +120,7 @@ constexpr int kEvictChunk = 1024;        // slots of a workgroup where several s
 constexpr int kEvictChunkThreads = 256;
 constexpr int64_t kEvictFused = 65536;   // bytes of K a unit's one workgroup moves itself,
 constexpr int kEvictPairs = 1024;        // in up to as many rows
+constexpr int kEvictTally = 1028;        // words of a chunk's sums over the last digit
 constexpr int kNoPosition = -0x7FFFFFFF - 1;
 
 // A slot's place in the order of what stays, as an unsigned number: the float's bits, ordered
@@ -133,7 +134,7 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
 }
 
 // What the workgroups that share a unit tell each other.
-struct EvictUnit {
+struct alignas(16) EvictUnit {
   int32_t hist[3][kEvictBins];  // of the keys' three digits, each under the digits before
   int32_t known[3][2];          // after each digit: the threshold's bits so far, and the keys still needed
 };
@@ -148,7 +149,7 @@ struct EvictArgs {
   int32_t* movers;
   EvictUnit* unit;  // shared units only, as the rest
   int32_t* newest;  // [unit][chunk]
-  int32_t* tally;   // [unit][chunk][4]
+  uint32_t* tally;  // [unit][chunk][kEvictTally]
   uint32_t* keys;   // [unit][capacity]
   int64_t moves, capacity;
   int width, keep, first, recent;
@@ -198,11 +199,11 @@ __device__ __forceinline__ int wave_sum(int x) {
 }
 
 // The bin, from the top, in which the need-th key lies, and how many of its keys are needed.  Called
-// by a whole workgroup; the bins are not changed until everyone has read them.
+// by a whole workgroup; the bins are not changed until everyone has read them.  -> whether all are needed
 template <int THREADS>
-__device__ __forceinline__ void evict_pick(const int32_t* hist, int* bin, int* need) {
+__device__ __forceinline__ bool evict_pick(const int32_t* hist, int* bin, int* need) {
   __shared__ int s_sum[THREADS / 64];
-  __shared__ int s_out[2];
+  __shared__ int s_out[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, want = *need;
   constexpr int P = kEvictBins / THREADS;
   int c[P], sum = 0;
@@ -227,10 +228,12 @@ __device__ __forceinline__ void evict_pick(const int32_t* hist, int* bin, int* n
     while (j < P - 1 && before + c[j] < want) before += c[j++];
     s_out[0] = kEvictBins - 1 - (tid * P + j);
     s_out[1] = want - before;
+    s_out[2] = want - before == c[j];
   }
   __syncthreads();
   *bin = s_out[0];
   *need = s_out[1];
+  return s_out[2] != 0;
 }
 
 // Digit d (0, 1, 2) of a key, its place, and whether a key has the threshold's digits before it.
@@ -335,8 +338,9 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
       if (t0 + 64 * i < end && evict_under(key[i], top, d)) atomicAdd(&s_hist[d][evict_digit(key[i], d)], 1);
     __syncthreads();
     int bin;
-    evict_pick<kEvictThreads>(s_hist[d], &bin, &need);
+    const bool whole = evict_pick<kEvictThreads>(s_hist[d], &bin, &need);
     top |= uint32_t(bin) << evict_shift(d);
+    if (whole) break;  // the bin's keys all stay: the threshold is its lowest, the digits below 0
   }
   int sum[4] = {0, 0, 0, 0};
   evict_count<R>(key, t0, end, a.keep, top, sum);
@@ -373,10 +377,12 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
 // The same for longer units, which one compute unit's instruction rate would bound (32767 slots of 16
 // units took it 87 us, 65535 of one 160): a workgroup per chunk of kEvictChunk slots, a launch for
 // each time that the workgroups have to meet.  Every launch costs its 4 us whatever it does, so a chunk
-// is what one workgroup of four waves does in that time: 28 us in all for both sizes with 1024 slots,
+// is what one workgroup of four waves does in that time: 26 us in all for both sizes with 1024 slots,
 // 48 with 4096.  STEP 0: the chunk's newest position, and the unit's
-// histograms cleared.  1: keys and the first digit's histogram.  2, 3: the second's and third's.
-// 4: the chunk's counts.  5: its part of the lists.
+// histograms cleared.  1: keys and the first digit's histogram.  2, 3: the second's and third's, the
+// third with the chunk's own: tally[j] = its keys of at least the first two digits' threshold followed
+// by j, those below keep in the low 16 bits and those past it in the high.  4: the threshold, what the other chunks
+// have above it and at it from their tallies, and the chunk's part of the lists.
 template <int STEP>
 __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(EvictArgs a) {
   constexpr int R = kEvictChunk / kEvictChunkThreads, NW = kEvictChunkThreads / 64;
@@ -386,13 +392,13 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
   const int n = evict_len(a, b);
   EvictUnit& st = a.unit[u];
   int32_t* const newest = a.newest + int64_t(u) * nb;
-  int32_t* const tally = a.tally + int64_t(u) * nb * 4;
+  uint32_t* const tally = a.tally + int64_t(u) * nb * kEvictTally;
   uint32_t* const keys = a.keys + u * a.capacity;
   if constexpr (STEP == 0)
     for (int i = chunk * kEvictChunkThreads + tid; i < 3 * kEvictBins; i += nb * kEvictChunkThreads)
       (&st.hist[0][0])[i] = 0;
   if (n <= a.keep) {
-    if (STEP == 5 && chunk == 0 && tid == 0) a.counts[u] = 0;
+    if (STEP == 4 && chunk == 0 && tid == 0) a.counts[u] = 0;
     return;
   }
   const int chunks = (n + kEvictChunk - 1) / kEvictChunk;
@@ -445,7 +451,7 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
       st.known[STEP - 2][1] = need;
     }
   }
-  if constexpr (STEP >= 1 && STEP <= 3) {
+  if constexpr (STEP == 1 || STEP == 2) {
     constexpr int d = STEP - 1;
     __shared__ int s_hist[kEvictBins];
     for (int i = tid; i < kEvictBins; i += kEvictChunkThreads) s_hist[i] = 0;
@@ -457,40 +463,81 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
     for (int i = tid; i < kEvictBins; i += kEvictChunkThreads)
       if (s_hist[i]) atomicAdd(&st.hist[d][i], s_hist[i]);  // integers: the order does not matter
   }
-  if constexpr (STEP >= 4) {
+  if constexpr (STEP == 3) {
+    __shared__ uint32_t s_hist[1024];
+    __shared__ uint32_t s_up[NW];
+    static_assert(kEvictChunkThreads * 4 == 1024);
+    for (int i = tid; i < 1024; i += kEvictChunkThreads) s_hist[i] = 0;
+    __syncthreads();
+    uint32_t more = 0;  // the wave's keys above the two digits
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int t = t0 + 64 * i;
+      const bool in = t < end, gt = in && key[i] >> 10 > top >> 10;
+      if (in && evict_under(key[i], top, 2)) atomicAdd(&s_hist[evict_digit(key[i], 2)], t < a.keep ? 1u : 1u << 16);
+      more += uint32_t(__popcll(__ballot(gt && t < a.keep))) + (uint32_t(__popcll(__ballot(gt && t >= a.keep))) << 16);
+    }
+    if (lane == 0) s_wave[0][wave] = int(more);
+    __syncthreads();
+    more = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) more += uint32_t(s_wave[0][i]);
+    uint32_t c[4], sum = 0;  // of the bins from 1023 - 4 tid down
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j] = s_hist[1023 - (4 * tid + j)];
+      sum += c[j];
+      if (c[j]) atomicAdd(&st.hist[2][1023 - (4 * tid + j)], int((c[j] & 0xFFFF) + (c[j] >> 16)));
+    }
+    uint32_t up = sum;  // inclusive over the workgroup
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = __shfl_up(up, o, 64);
+      if (lane >= o) up += y;
+    }
+    if (lane == 63) s_up[wave] = up;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) up += i < wave ? s_up[i] : 0;
+    uint32_t run = more + up - sum;
+    v4i g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      run += c[j];
+      g[3 - j] = int(run);
+    }
+    *reinterpret_cast<v4i*>(tally + chunk * int64_t(kEvictTally) + 1020 - 4 * tid) = g;
+    if (tid == 0) tally[chunk * int64_t(kEvictTally) + 1024] = more;
+  }
+  if constexpr (STEP == 4) {
     int sum[4] = {0, 0, 0, 0};
     evict_count<R>(key, t0, end, a.keep, top, sum);
     if (lane == 0)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s_wave[j][wave] = sum[j];
     __syncthreads();
-    if constexpr (STEP == 4) {
-      if (tid < 4) {
-        int all = 0;
-        for (int i = 0; i < NW; ++i) all += s_wave[tid][i];
-        tally[chunk * 4 + tid] = all;
-      }
-    } else {
-      int before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
-      for (int i = lane; i < chunks; i += 64)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int x = tally[i * 4 + j];
-          all[j] += x;
-          before[j] += i < chunk ? x : 0;
-        }
+    int before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
+    const int bin = evict_digit(top, 2);
+    for (int i = lane; i < chunks; i += 64) {
+      const uint32_t ge = tally[i * int64_t(kEvictTally) + bin], gt = tally[i * int64_t(kEvictTally) + bin + 1];
+      const uint32_t tie = ge - gt;
+      const int x[4] = {int(gt & 0xFFFF), int(tie & 0xFFFF), int(gt >> 16), int(tie >> 16)};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        all[j] = wave_sum(all[j]);
-        before[j] = wave_sum(before[j]);
-        for (int i = 0; i < wave; ++i) before[j] += s_wave[j][i];
+        all[j] += x[j];
+        before[j] += i < chunk ? x[j] : 0;
       }
-      int32_t* const holes = a.holes + u * a.moves;
-      int32_t* const movers = a.movers + u * a.moves;
-      const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
-                                      [&](int i, int r) { movers[i] = t0 + 64 * r; });
-      if (chunk == 0 && tid == 0) a.counts[u] = pairs;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      all[j] = wave_sum(all[j]);
+      before[j] = wave_sum(before[j]);
+      for (int i = 0; i < wave; ++i) before[j] += s_wave[j][i];
+    }
+    int32_t* const holes = a.holes + u * a.moves;
+    int32_t* const movers = a.movers + u * a.moves;
+    const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
+                                    [&](int i, int r) { movers[i] = t0 + 64 * r; });
+    if (chunk == 0 && tid == 0) a.counts[u] = pairs;
   }
 }
 
@@ -526,8 +573,8 @@ static EvictSizes evict_sizes(const wz_paged_kv* c, int64_t B, int64_t width, in
   if (capacity > kEvictSmall) {
     z.chunks = (capacity + kEvictChunk - 1) / kEvictChunk;
     z.unit = z.units * int64_t(sizeof(EvictUnit));
-    z.newest = 4 * z.units * z.chunks;
-    z.tally = 16 * z.units * z.chunks;
+    z.newest = (4 * z.units * z.chunks + 15) / 16 * 16;
+    z.tally = 4 * kEvictTally * z.units * z.chunks;
     z.keys = 4 * z.units * capacity;
   }
   z.counts = 4 * z.units;
@@ -629,7 +676,7 @@ extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, in
   a.new_lens = new_lens;
   a.unit = reinterpret_cast<EvictUnit*>(take(z.unit));
   a.newest = reinterpret_cast<int32_t*>(take(z.newest));
-  a.tally = reinterpret_cast<int32_t*>(take(z.tally));
+  a.tally = reinterpret_cast<uint32_t*>(take(z.tally));
   a.keys = reinterpret_cast<uint32_t*>(take(z.keys));
   a.counts = reinterpret_cast<int32_t*>(take(z.counts));
   a.holes = reinterpret_cast<int32_t*>(take(4 * z.units * z.moves));
@@ -664,7 +711,6 @@ extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, in
     WZ_EVICT(2);
     WZ_EVICT(3);
     WZ_EVICT(4);
-    WZ_EVICT(5);
 #undef WZ_EVICT
   }
   const int64_t blocks = std::min<int64_t>(std::max<int64_t>(1, (z.moves * (row_bytes / 16) + 255) / 256),
