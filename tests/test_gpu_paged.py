@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from oracle import paged as op
+from wanferenz_amd import _native as N
 from wanferenz_amd.paged import PagedKV
 
 pytestmark = pytest.mark.gpu
@@ -591,3 +592,158 @@ def test_workspace_and_outputs_of_the_caller(gpu):
         graphs[1].replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)
+
+
+# ---------------------------------------------------------------- the calls at the edges ----
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("B,HK,g,D,shared", [(300, 8, 2, 64, False), (600, 2, 3, 128, False), (300, 1, 16, 512, True)])
+def test_more_sequences_than_workers(gpu, B, HK, g, D, shared, dtype):
+    """More (sequence, head) units than the chip has workers, most of them short and every seventh empty; the
+    weights as well."""
+    rng = np.random.default_rng(B)
+    lens = [0 if b % 7 == 0 else int(n) for b, n in enumerate(rng.integers(1, 70, B))]
+    cache, vals, tab, table = make(gpu, B, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared, track=True)
+    q, qd = queries(gpu, g, B, 1, HK * g, D)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    ref = op.attend(vals, qd, table, lens, D ** -0.5)
+    before = cache.weights.cpu().double().numpy()
+    o = cache.attend(q, tab, n, D ** -0.5, accumulate=True)
+    check(o, ref, D)
+    _, e32 = bounds(ref[0], ref[1], ref[3], D)
+    after = cache.weights.cpu().double().numpy()
+    assert (np.abs(after - before - ref[2]) <= e32 * ref[2] + 2.0 ** -23 * (np.abs(after) + 1e-30)).all()
+    assert torch.equal(cache.attend(q, tab, n, D ** -0.5), o)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("S,g,D,shared", [(16, 24, 128, False), (16, 9, 64, False), (5, 30, 256, True), (16, 20, 512, True)])
+def test_many_rows_of_a_head(gpu, S, g, D, shared, dtype):
+    """More rows of a KV head than a group holds, lengths shorter than the new tokens, the weights and their
+    fixed order."""
+    lens = [S - 1, 700, 0, 64]
+    cache, vals, tab, table = make(gpu, S + g, lens, HK=1, D=D, page=32, dtype=dtype, shared=shared, track=True)
+    q, qd = queries(gpu, g, len(lens), S, g, D)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    ref = op.attend(vals, qd, table, lens, D ** -0.5)
+    cache.weights.zero_()
+    check(cache.attend(q, tab, n, D ** -0.5, accumulate=True), ref, D)
+    _, e32 = bounds(ref[0], ref[1], ref[3], D)
+    once = cache.weights.clone()
+    w = once.cpu().double().numpy()
+    # a sum of S g float32 terms of at most 1
+    assert (np.abs(w - ref[2]) <= (e32 + S * g * 2.0 ** -24) * ref[2] + 1e-30).all()
+    cache.weights.zero_()
+    cache.attend(q, tab, n, D ** -0.5, accumulate=True)
+    assert torch.equal(once, cache.weights)
+
+
+def test_nothing_to_do(gpu):
+    """No sequences, no new tokens, a table without pages, only empty sequences: zeros, and nothing changes."""
+    cache, _, tab, _ = make(gpu, 71, [40, 20], HK=2, D=64, page=16, track=True)
+    want = arrays(cache)
+    n = torch.tensor([40, 20], dtype=torch.int32, device=gpu)
+    none, no_table = n[:0], tab[:, :0]
+    q = torch.randn(2, 1, 4, 64, device=gpu).to(torch.bfloat16)
+    k = torch.randn(2, 3, 2, 64, device=gpu).to(torch.bfloat16)
+    assert cache.attend(q[:0], tab[:0], none, 0.1).shape == (0, 1, 4, 64)
+    assert cache.attend(q[:, :0], tab, n, 0.1).shape == (2, 0, 4, 64)
+    assert (cache.attend(q, no_table, n, 0.1, accumulate=True) == 0).all()
+    assert (cache.attend(q, tab, torch.zeros_like(n), 0.1, accumulate=True) == 0).all()
+    assert (cache.attend(q, tab, -n, 0.1, accumulate=True) == 0).all()
+    cache.write(k[:0], k[:0], tab[:0], none)
+    cache.write(k[:, :0], k[:, :0], tab, n)
+    cache.write(k, k, no_table, n)
+    cache.write(k, k, tab, n, count=-n)
+    cache.write(k, k, tab, torch.full_like(n, -7))
+    cache.write(k, k, tab, torch.full_like(n, 2 ** 31 - 2))
+    assert cache.evict(tab[:0], none, 5).shape == (0,)
+    assert cache.evict(no_table, n, 7).tolist() == [7, 7]
+    assert cache.evict(tab, n, 100).tolist() == [40, 20]
+    assert cache.evict(tab, n, 2 ** 31 - 1, first=5, recent=2 ** 31 - 6).tolist() == [40, 20]
+    for name, x in arrays(cache).items():
+        assert np.array_equal(x, want[name], equal_nan=name == "weights"), name
+
+
+def test_write_counts_past_the_rows(gpu):
+    """A count above the rows given means all of them."""
+    cache = PagedKV.empty(4, 16, 2, 64, device=gpu)
+    k = torch.randn(1, 3, 2, 64, device=gpu).to(torch.bfloat16)
+    one = lambda x: torch.tensor([x], dtype=torch.int32, device=gpu)  # noqa: E731
+    cache.write(k, k, torch.tensor([[2]], dtype=torch.int32, device=gpu), one(-1), count=one(2 ** 31 - 1))
+    assert torch.equal(cache.k[2, :, :2], k[0, 1:].transpose(0, 1)) and not cache.k[2, :, 2:].any() and not cache.k[:2].any()
+
+
+def test_captured_cut_of_long_sequences(gpu):
+    """Units that several workgroups share, cut in a captured graph: every replay equals the eager call."""
+    page, HK, n, keep = 64, 2, 12000, 1000
+    cache = PagedKV.empty(200, page, HK, 64, track=True, device=gpu)
+    table = torch.randperm(200, generator=torch.Generator().manual_seed(5))[:188].to(torch.int32)[None].to(gpu)
+    lens = torch.tensor([n], dtype=torch.int32, device=gpu)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(lens)
+
+    def fill(seed):
+        g = torch.Generator(device=gpu).manual_seed(seed)
+        cache.weights.copy_(torch.rand(cache.weights.shape, generator=g, device=gpu))
+        cache.k.copy_(torch.randn(cache.k.shape, generator=g, device=gpu))
+        slot = torch.arange(188 * page, dtype=torch.int32, device=gpu).view(188, 1, page)
+        cache.positions[table[0].long()] = slot.expand(-1, HK, -1).contiguous()
+
+    fill(0)
+    cache.evict(table, lens, keep, 4, 100)
+    fill(0)
+    with torch.cuda.graph(graph):
+        cache.evict(table, lens, keep, 4, 100, out=out)
+    for seed in range(4):
+        fill(seed)
+        cache.evict(table, lens, keep, 4, 100)
+        want = arrays(cache)
+        fill(seed)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert out.tolist() == [keep]
+        for name, x in arrays(cache).items():
+            assert np.array_equal(x, want[name]), (seed, name)
+
+
+def test_refusals_with_device_tensors(gpu):
+    """What does not fit is refused before a kernel runs."""
+    cache, _, tab, _ = make(gpu, 81, [40, 20], HK=2, D=64, page=16, track=True)
+    want = arrays(cache)
+    n = torch.tensor([40, 20], dtype=torch.int32, device=gpu)
+    q = torch.randn(2, 1, 4, 64, device=gpu).to(torch.bfloat16)
+    ws = torch.empty(16, dtype=torch.uint8, device=gpu)
+    for kw, error, what in (
+            (dict(q=q.float()), TypeError, "bf16 q"), (dict(q=q[..., :32]), ValueError, "q must be"),
+            (dict(q=q[:, :, :3]), N.WzError, "3 heads on 2"), (dict(q=q.expand(2, 17, 4, 64)), N.WzError, "S=17"),
+            (dict(q=q.cpu()), ValueError, "q is on cpu"), (dict(table=tab.long()), ValueError, "table must be int32"),
+            (dict(table=tab[:1]), ValueError, "table must be int32"), (dict(table=tab.cpu()), ValueError, "table is on cpu"),
+            (dict(lens=n.long()), ValueError, "lens must be int32"), (dict(lens=n.cpu()), ValueError, "lens is on cpu"),
+            (dict(attn_sink=torch.zeros(3, device=gpu)), ValueError, "attn_sink"),
+            (dict(out=torch.empty(2, 1, 4, 64, device=gpu)), ValueError, "out must be"),
+            (dict(workspace=ws), N.WzError, "workspace of 16 bytes"), (dict(workspace=ws.float()), ValueError, "workspace must be")):
+        args = {**dict(q=q, table=tab, lens=n, softmax_scale=0.1), **kw}
+        with pytest.raises(error, match=what):
+            cache.attend(**args)
+    k = torch.randn(2, 3, 2, 64, device=gpu).to(torch.bfloat16)
+    for kw, error, what in ((dict(v=None), ValueError, "v is given"), (dict(v=k[:, :2]), ValueError, "does not match"),
+                            (dict(k=k[..., :32]), ValueError, "k must be"), (dict(k=k.half(), v=k.half()), TypeError, "bf16 k"),
+                            (dict(start=n[:1]), ValueError, "start must be"), (dict(count=n.float()), ValueError, "count must be"),
+                            (dict(position=n.cpu()), ValueError, "position is on cpu")):
+        with pytest.raises(error, match=what):
+            cache.write(**{**dict(k=k, v=k, table=tab, start=n), **kw})
+    for kw, error, what in ((dict(keep=-1), N.WzError, "keep -1"), (dict(keep=5, first=3, recent=3), N.WzError, "first 3"),
+                            (dict(keep=5, out=n[:1]), ValueError, "out must be"),
+                            (dict(keep=5, lens=n.view(1, 2)), ValueError, "table must be"),
+                            (dict(keep=5, workspace=ws[:0]), N.WzError, "workspace of")):
+        with pytest.raises(error, match=what):
+            cache.evict(**{**dict(table=tab, lens=n), **kw})
+    plain = PagedKV(cache.k, cache.v)
+    with pytest.raises(ValueError, match="not tracked"):
+        plain.evict(tab, n, 5)
+    with pytest.raises(N.WzError, match="not tracked"):
+        plain.attend(q, tab, n, 0.1, accumulate=True)
+    for name, x in arrays(cache).items():
+        assert np.array_equal(x, want[name], equal_nan=name == "weights"), name
