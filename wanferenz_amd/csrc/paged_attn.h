@@ -18,8 +18,11 @@
 //   * y = q . k scale log2(e), p = 2^(y - m), m moved only when a tile's maximum exceeds it by more
 //     than 8 (the final quotient does not depend on m); p is rounded to bf16 for the product with V
 //     (the sums keep it in 32 bits), which adds as much error as the output's own rounding.
-// Reading the cache bounds it: 4 R / element-size flops a byte is far below the matrix units' rate
-// for the usual group sizes.  Latents of 512 have a kernel of their own (paged_latent.h).
+// Reading the cache bounds it: 2 R / element-size flops a byte is far below the matrix units' rate
+// for the usual group sizes.  At 5.5 to 5.8 TB/s: 131071 tokens of 8 heads of 128, 32 query heads (537 MB) 93 us, 64
+// sequences of 16 to 16384 (647 MB) 118, four new tokens on 16 x 8191 (538 MB) 99 to 102; 48 of 1125 to 9001 e4m3 rows of 64 (207 MB) 44,
+// 4.7 TB/s.  What is left is a worker's first tile and its last: 10 us whatever the length.  Latents of 512 have
+// a kernel of their own (paged_latent.hip).
 #pragma once
 
 #include <algorithm>
@@ -685,9 +688,9 @@ void paged_attn_kernel(PagedAttnArgs a) {
 }
 
 // Merges the cut units' partials.  WIDE: a workgroup a row of a unit, every partial's (m, l) at once,
-// then O with GR partials in flight at a time, for few units of many parts (131071 tokens of one sequence: 128
-// parts of 8 units).  Else GR rows a workgroup, each by the CH threads that hold its columns, without
-// a barrier: a unit of a large batch has two or three parts.
+// then O with GR partials in flight at a time, for units of eight parts and more (128 parts of 8 units 5.4 us against
+// 35.7, 16 of 64 5.0 against 7.8, 8 of 128 4.6 against 5.8).  Else GR rows a workgroup, each by the CH threads that hold
+// its columns, without a barrier (4 parts of 256 units 4.0 us against 4.3).
 constexpr int kPagedMaxWorkers = 4096;
 
 template <int D, bool WIDE>
@@ -778,7 +781,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
 // head, which the workgroup takes at once (4 rows: 5.6 us against 8.5 in two launches, 131071 tokens 9.4 against 11.8;
 // 64 rows 22.9 against 20.2).
 constexpr int kWeighSlots = 1024;
-constexpr int kWeighRows = 16;
+constexpr int kWeighRows = 16;  // and no more than a unit's
 
 template <int D, bool JOIN>
 __device__ __forceinline__ void paged_weigh(const PagedAttnArgs& a, int bh, int block, float* s_ml) {
@@ -789,17 +792,16 @@ __device__ __forceinline__ void paged_weigh(const PagedAttnArgs& a, int bh, int 
   if (block * kWeighSlots >= n) return;
   const float* const ml = a.ml + 2 * int64_t(bh) * R;
   if constexpr (JOIN) {
-    const int upb = (R + a.unit_rows - 1) / a.unit_rows, li = threadIdx.x & 15;
-    for (int r = threadIdx.x >> 4; r < R; r += 16) {  // 16 threads a row
-      const int u = r / a.unit_rows, rl = r - u * a.unit_rows;
-      const PagedCut cut = a.cut[int64_t(bh) * upb + u];
+    const int r = threadIdx.x >> 4, li = threadIdx.x & 15;  // one unit holds the rows
+    if (r < R) {
+      const PagedCut cut = a.cut[bh];
       float m, inv;
       if (cut.np < 2) {
         m = ml[2 * r];
         inv = ml[2 * r + 1];
       } else {
         const int64_t slot = int64_t(a.rows) * (D + 2);
-        const float* const part = a.part + rl;
+        const float* const part = a.part + r;
         auto at = [&](int j) { return part + (2 * (int64_t(cut.w) + j) + (j == 0 ? 1 : 0)) * slot; };
         const float sk = a.sink ? a.sink[hk * grp + r % grp] * kLog2e : -INFINITY;
         float M = -INFINITY, l = 0.0f;  // of this thread's partials
@@ -876,7 +878,7 @@ int paged_attn_join(const PagedAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = n * row_blocks + heads * slot_blocks;
   const int R = a.S * (a.H / a.c.heads);
   const size_t ml_bytes = 2 * sizeof(float) * R;
-  if (a.scores && a.by_unit && R <= kWeighRows && blocks <= 0x7FFFFFFF) {
+  if (a.scores && a.by_unit && R <= kWeighRows && blocks <= 0xFFFFFF) {
     if (wide)
       WZ_LAUNCH("paged_attn_end", stream, (paged_attn_end_kernel<D, true>), dim3{unsigned(blocks)}, dim3(256), ml_bytes, a,
                 int(n), int(row_blocks), int(slot_blocks));
@@ -897,7 +899,8 @@ int paged_attn_join(const PagedAttnArgs& a, hipStream_t stream) {
   return check_launch("paged_attn_weigh");
 }
 
-// The kernel of R rows a KV head: 16, 32 or 64 rows a unit.
+// The kernel of R rows a KV head: 16, 32 or 64 rows a unit.  With 4 rows 16 x 8000 tokens take 94.5 / 97.6 / 121.7 us with
+// each, 48 x 9001 e4m3 tokens of 128 with 8 rows 167 / 214 / 400.
 template <int D, bool FP8, bool SHARED, int RT, int RH>
 int paged_attn_launch_rt(PagedAttnArgs a, bool ask, int* workers, hipStream_t stream) {
   using C = PagedCfg<D, FP8, SHARED, RT, RH>;

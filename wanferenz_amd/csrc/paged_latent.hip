@@ -12,11 +12,18 @@
 //     with the m of the tiles before and flags a row that needs a new one; only then a second barrier
 //     follows, after the maxima have met, O is rescaled and P written again;
 //   * O^T[512, rows] += V^T P^T: wave w has columns 64 w .. +64 of every row.
+// 4 x 65536 latents (269 MB, 34 GF) take 68 to 75 us by card, 3.6 to 4 TB/s, and the join of the 131 KB partials 8: the
+// loads alone would take 56, and a tile's LDS traffic (K twice, V, Q's last chunks and P, 260 KB a tile and compute
+// unit) and its two barriers keep the products from hiding behind them.  With 16 heads 16 x 16000 latents (262 MB) take
+// 52, 5.1 TB/s.
 #include "paged_attn.h"
 
 namespace wz {
 
-constexpr int kLatentD = 512, kLatentTile = 64, kLatentWaves = 8, kLatentStart = 4;
+constexpr int kLatentD = 512, kLatentTile = 64, kLatentWaves = 8;
+// A unit's start in tiles (paged_cost): 64 sequences of 60 to 4000 latents, 64 heads, 40.1 / 31.1 / 29.3 / 31.6 us with 0 /
+// 2 / 4 / 8, four of 65536 75.9 / 79.9 / 73.4 / 76.4.
+constexpr int kLatentStart = 4;
 
 template <bool FP8>
 struct LatentCfg {
@@ -26,7 +33,8 @@ struct LatentCfg {
   static constexpr int LOADS = RPW * RB / 1024 + (FP8 ? 1 : 0);
 };
 
-// EXTRA: several new tokens, or weights to accumulate; without them 64 rows just fit the registers.
+// EXTRA: several new tokens, or weights to accumulate; without their code 64 rows just fit the registers (4 x 65536
+// latents 73.4 us, with it 76.9).
 template <bool FP8, int HT, bool EXTRA>
 __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(PagedAttnArgs a) {
   using C = LatentCfg<FP8>;
@@ -35,7 +43,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
   constexpr int KC = D / 32, NT = D / 16 / kLatentWaves;
   constexpr int SHT = HT == 4 ? 2 : 1;  // row tiles of S a wave
   // the last KQ chunks of Q are read from LDS for each tile: with all of 64 rows in registers some were
-  // spilled, and a reload waits for the loads of the next tile (102 us, 268 MB; so: see below)
+  // spilled, and a reload waits for the loads of the next tile (4 x 65536 latents 87.7 us; so 73.4)
   constexpr int KQ = HT == 4 ? 2 : 0;
   constexpr int QB = 2 * D;  // bytes of a row of Q
   __shared__ __align__(1024) uint8_t kb[2][C::TILE];
@@ -519,6 +527,8 @@ static int latent_launch(PagedAttnArgs a, bool ask, int* workers, hipStream_t st
   return paged_attn_join<kLatentD>(a, stream);
 }
 
+// The kernel of R rows: 16, 32 or 64 a unit.  16 x 16000 latents with 16 / 32 heads 51.6 / 54.2 us, in units of 64 rows 66.3 /
+// 65.2.
 int paged_latent(bool fp8, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
   const int R = a.S * (a.H / a.c.heads);
   if (R <= 16)
