@@ -405,7 +405,7 @@ int wz_paged_kv_write(const wz_paged_kv* cache, const void* k_bf16, const int64_
  * lens[b] - (S - 1 - i); o = sum_j p_j v_j / (sum_j p_j + exp(sink[h] - m)), p_j =
  * exp(q . k_j scale - m), m the maximum; a row that sees nothing gets 0.  q [B, S, H,
  * head_dim] bf16 (q_strides as above), H a multiple of kv_heads, query head h reading KV
- * head h / (H / kv_heads); attn_sink [H] float32 or NULL; o dense bf16.  accumulate adds to
+ * head h / (H / kv_heads); attn_sink [H] float32 or NULL; o dense bf16, not over q.  accumulate adds to
  * each slot's weight the attention that the rows of its KV head give it, in a fixed
  * order (a tracked cache with 16-byte aligned weights, one call at a time).  lens beyond the table are cut to it. */
 int64_t wz_paged_attn_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t S, int64_t H, int64_t table_width,

@@ -17,7 +17,8 @@ A decode loop::
     lens = cache.evict(table, lens + 1, keep=4096, first=4, recent=1024)
 
 Every call runs on the current stream of the cache's device, allocates only its outputs and
-(unless given) its workspace, never synchronises, and can be captured in a graph.
+(unless given) its workspace, never synchronises, and can be captured in a graph.  The operators
+are for serving: they have no gradients.
 """
 
 from __future__ import annotations
@@ -198,7 +199,7 @@ class PagedKV:
         sees nothing (a padded sequence of length 0) gives zeros.  -> [b, s, h, head_dim] bf16 (``out`` if given).
 
         ``accumulate`` adds to each slot's weight (a tracked cache) what the rows of its KV head gave it, in a
-        fixed order.  ``workspace``: a uint8 tensor of ``attend_workspace_bytes``, for calls that must not
+        fixed order.  ``out`` may not overlap q.  ``workspace``: a uint8 tensor of ``attend_workspace_bytes``, for calls that must not
         allocate; calls that overlap in time need one each."""
         if q.dim() != 4 or q.shape[3] != self.head_dim:
             raise ValueError(f"PagedKV.attend: q must be [b, s, h, {self.head_dim}], got {list(q.shape)}")
