@@ -740,6 +740,8 @@ def test_refusals_with_device_tensors(gpu):
                             (dict(keep=5, workspace=ws[:0]), N.WzError, "workspace of")):
         with pytest.raises(error, match=what):
             cache.evict(**{**dict(table=tab, lens=n), **kw})
+    with pytest.raises(ValueError, match="contiguous"):
+        PagedKV(cache.k[:, :1], cache.v[:, :1])
     plain = PagedKV(cache.k, cache.v)
     with pytest.raises(ValueError, match="not tracked"):
         plain.evict(tab, n, 5)

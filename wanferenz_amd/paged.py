@@ -80,7 +80,8 @@ class PagedKV:
             if not t.is_cuda:
                 raise RuntimeError("wanferenz_amd kernels run on the GPU only (got a CPU tensor); "
                                    "there is no CPU fallback in this package")
-            assert t.is_contiguous()
+            if not t.is_contiguous():
+                raise ValueError("PagedKV: the pools must be contiguous")
             if t.device != k.device:
                 raise ValueError("PagedKV: the pools are on different devices")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
