@@ -266,7 +266,8 @@ struct PagedCfg {
   static constexpr int LDS = RING + RH * NS * 4;               // valid masks
   // Waves a SIMD.  One of tiles of 8 KB and more keeps the memory busy, and a second adds partial results:
   // 48 sequences of 9001 tokens, 64 heads on 8, us with one / two: bf16 of 64 157 / 160, e4m3 of 128
-  // 164 / 172; tiles of 4 KB need two: e4m3 of 64 111 / 91 (rings of four tiles 109 / 95).
+  // 164 / 172; tiles of 4 KB need two: e4m3 of 64 111 / 91, with three
+  // and four 100 / 96 (rings of four tiles 109 / 95).
   static constexpr int EU = STAGE <= 4096 ? 2 : 1;
   static constexpr int PER_CU = 160 * 1024 / LDS < 4 * EU / RH ? 160 * 1024 / LDS : 4 * EU / RH;
   static_assert(NS >= 2 && (NS - 1) * LOADS < 64, "the waits count the loads in flight");

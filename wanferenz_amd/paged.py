@@ -200,8 +200,8 @@ class PagedKV:
         sees nothing (a padded sequence of length 0) gives zeros.  -> [b, s, h, head_dim] bf16 (``out`` if given).
 
         ``accumulate`` adds to each slot's weight (a tracked cache) what the rows of its KV head gave it, in a
-        fixed order.  ``out`` may not overlap q.  ``workspace``: a uint8 tensor of ``attend_workspace_bytes``, for calls that must not
-        allocate; calls that overlap in time need one each."""
+        fixed order.  ``out`` may not overlap q.  ``workspace``: a uint8 tensor of ``attend_workspace_bytes``, for
+        calls that must not allocate; calls that overlap in time need one each."""
         if q.dim() != 4 or q.shape[3] != self.head_dim:
             raise ValueError(f"PagedKV.attend: q must be [b, s, h, {self.head_dim}], got {list(q.shape)}")
         b, s, h, d = q.shape
