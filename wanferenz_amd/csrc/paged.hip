@@ -176,12 +176,16 @@ __device__ __forceinline__ void evict_move(const EvictArgs& a, int64_t to, int64
   if (!c.shared) *reinterpret_cast<v4i*>(c.v + to * row_bytes + ch * 16) = v;
 }
 
-// A thread's R keys, of the slots t0 + 64 i: their positions and weights, all loads in flight together.
+// A thread's keys, of the slots t0 + 64 i for i < per <= R (the same for the wave): their positions and
+// weights, all loads in flight together.
 template <int R>
-__device__ __forceinline__ void evict_load(const EvictArgs& a, const int32_t* trow, int h, int n, int t0, int64_t (&at)[R],
-                                           int (&p)[R], float (&w)[R]) {
+__device__ __forceinline__ void evict_load(const EvictArgs& a, const int32_t* trow, int h, int n, int t0, int per,
+                                           int64_t (&at)[R], int (&p)[R], float (&w)[R]) {
 #pragma unroll
-  for (int i = 0; i < R; ++i) at[i] = t0 + 64 * i < n ? paged_row(a.c, trow, a.width, h, t0 + 64 * i) : -1;
+  for (int i = 0; i < R; ++i) {
+    at[i] = -1;
+    if (i < per && t0 + 64 * i < n) at[i] = paged_row(a.c, trow, a.width, h, t0 + 64 * i);
+  }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     p[i] = at[i] >= 0 ? a.c.positions[at[i]] : kNoPosition;
@@ -260,9 +264,11 @@ __device__ __forceinline__ bool evict_under(uint32_t k, uint32_t prefix, int d) 
 
 // A wave's counts of its R rounds: kept slots above the threshold and ties, below keep and past it.
 template <int R>
-__device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, int n, int keep, uint32_t top, int (&sum)[4]) {
+__device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, int n, int per, int keep, uint32_t top,
+                                            int (&sum)[4]) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
+    if (i >= per) break;
     const int t = t0 + 64 * i;
     const bool in = t < n, low = t < keep, gt = in && key[i] > top, tie = in && key[i] == top;
     sum[0] += __popcll(__ballot(gt && low));
@@ -276,8 +282,8 @@ __device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, in
 // this lane.  `before`: evict_count's sums of the slots before the wave's, `all`: of the unit.  Of the
 // ties the lowest `need` stay, so those below keep go first.  -> the unit's pairs
 template <int R, typename Hole, typename Mover>
-__device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&key)[R], int t0, int n, uint32_t top, int need,
-                                          const int (&before)[4], const int (&all)[4], Hole&& put_hole,
+__device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&key)[R], int t0, int n, int per, uint32_t top,
+                                          int need,                                          const int (&before)[4], const int (&all)[4], Hole&& put_hole,
                                           Mover&& put_mover) {
   const int lane = threadIdx.x & 63;
   const uint64_t below = (1ull << lane) - 1;
@@ -288,6 +294,7 @@ __device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&k
   int im = before[2] + min(before[3], high);                          // kept slots past it
 #pragma unroll
   for (int i = 0; i < R; ++i) {
+    if (i >= per) break;
     const int t = t0 + 64 * i;
     const uint64_t tie = __ballot(t < n && key[i] == top);
     const bool kept = t < n && (key[i] > top || (key[i] == top && ties + __popcll(tie & below) < need));
@@ -307,7 +314,9 @@ __device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&k
 // holes below keep and the kept slots from keep on, in slot order.  Every wave has a range of
 // consecutive slots, 64 a round with the keys in registers, so the ranks need one exchange between the
 // waves.  MOVE: few pairs are moved here, which saves the second launch.  Its chain of dependent steps
-// bounds it: 128 units of 4160 slots cut to 4096 take 15.8 us, 13.7 and a move of 6.5 without MOVE, and 35 as chunks.
+// bounds it: 128 units of 4160 slots cut to 4096 take 15.8 us, 13.7 and a move of 6.5 without MOVE, and 35 as chunks;
+// without the rounds past a unit's own 14.4.  16 rounds a thread, for 16384 slots, cost the short ones more than the long
+// ones gain: 4160 slots 18.8 us against 13.8, 12000 23.5 against 24 as chunks.
 template <bool MOVE>
 __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictArgs a, int row_bytes) {
   constexpr int R = kEvictSmall / kEvictThreads, NW = kEvictThreads / 64;
@@ -329,7 +338,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
   int64_t at[R];
   int p[R];
   float w[R];
-  evict_load<R>(a, trow, h, end, t0, at, p, w);
+  evict_load<R>(a, trow, h, end, t0, per, at, p, w);
   for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
   int last = kNoPosition;
 #pragma unroll
@@ -337,7 +346,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
   last = wave_max(last);
   if (lane == 0) s_last[wave] = last;
   __syncthreads();
-  #pragma unroll
+#pragma unroll
   for (int i = 0; i < NW; ++i) last = max(last, s_last[i]);
   const int64_t old = int64_t(last) - a.recent;  // positions above it are protected
   uint32_t key[R];
@@ -348,8 +357,10 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
 #pragma unroll
   for (int d = 0; d < 3; ++d) {
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < R; ++i) {
+      if (i >= per) break;
       evict_add(s_hist[d], evict_digit(key[i], d), t0 + 64 * i < end && evict_under(key[i], top, d), false);
+    }
     __syncthreads();
     int bin;
     const bool whole = evict_pick<kEvictThreads>(s_hist[d], &bin, &need);
@@ -357,7 +368,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
     if (whole) break;  // the bin's keys all stay: the threshold is its lowest, the digits below 0
   }
   int sum[4] = {0, 0, 0, 0};
-  evict_count<R>(key, t0, end, a.keep, top, sum);
+  evict_count<R>(key, t0, end, per, a.keep, top, sum);
   // two counts a word: they add up to kEvictSmall at most
   if (lane == 0) s_count[wave] = make_uint2(uint32_t(sum[0]) << 16 | uint32_t(sum[1]), uint32_t(sum[2]) << 16 | uint32_t(sum[3]));
   __syncthreads();
@@ -374,7 +385,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
     // the pairs' rows stay in LDS, in the histograms' place
     int64_t* const holes = reinterpret_cast<int64_t*>(&s_hist[0][0]);
     int64_t* const movers = holes + kEvictPairs;
-    const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = at[r]; },
+    const int pairs = evict_list<R>(a, key, t0, end, per, top, need, before, all, [&](int i, int r) { holes[i] = at[r]; },
                                     [&](int i, int r) { movers[i] = at[r]; });
     __syncthreads();
     const int lpr = row_bytes / 16;
@@ -382,7 +393,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
   } else {
     int32_t* const holes = a.holes + u * a.moves;
     int32_t* const movers = a.movers + u * a.moves;
-    const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
+    const int pairs = evict_list<R>(a, key, t0, end, per, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
                                     [&](int i, int r) { movers[i] = t0 + 64 * r; });
     if (tid == 0) a.counts[u] = pairs;
   }
@@ -425,7 +436,7 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
     int64_t at[R];
     int p[R];
     float w[R];
-    evict_load<R>(a, trow, h, end, t0, at, p, w);
+    evict_load<R>(a, trow, h, end, t0, R, at, p, w);
     if constexpr (STEP == 0) {
       int last = kNoPosition;
 #pragma unroll
@@ -524,7 +535,7 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
   }
   if constexpr (STEP == 4) {
     int sum[4] = {0, 0, 0, 0};
-    evict_count<R>(key, t0, end, a.keep, top, sum);
+    evict_count<R>(key, t0, end, R, a.keep, top, sum);
     if (lane == 0)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s_wave[j][wave] = sum[j];
@@ -549,7 +560,7 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
     }
     int32_t* const holes = a.holes + u * a.moves;
     int32_t* const movers = a.movers + u * a.moves;
-    const int pairs = evict_list<R>(a, key, t0, end, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
+    const int pairs = evict_list<R>(a, key, t0, end, R, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
                                     [&](int i, int r) { movers[i] = t0 + 64 * r; });
     if (chunk == 0 && tid == 0) a.counts[u] = pairs;
   }
