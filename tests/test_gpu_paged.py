@@ -406,7 +406,8 @@ def test_evict_in_place_and_missing_pages(gpu, slots):
         assert np.array_equal(x, want[name]), name
 
 
-@pytest.mark.parametrize("n,keep", [(5000, 4096), (8200, 4000), (20000, 1500), (70001, 8192), (300000, 100000)])
+@pytest.mark.parametrize("n,keep", [(5000, 4096), (8200, 4000), (20000, 1500), (70001, 8192), (300000, 100000),
+                                    (8192, 5000), (1025, 600)])
 def test_evict_long(gpu, n, keep):
     """Lengths of many rounds of a workgroup, against torch's stable sort."""
     page, HK = 64, 2

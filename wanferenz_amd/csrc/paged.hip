@@ -202,9 +202,10 @@ __device__ __forceinline__ int wave_sum(int x) {
   return x;
 }
 
-// Counts a wave's keys (the lanes with `in`) in their bins, in a word's upper half where `high`.  The lanes that share the first one's
-// bin add up first: equal weights, as a prompt's zeros are, would meet in one word of LDS, an addition
-// after the other (32 units of 8000 zeros 27.6 us, so 16.6; random weights 16.8 and 16.4, of 4160 slots 14.3 and 15.0).
+// Counts a wave's keys (the lanes with `in`) in their bins, in a word's upper half where `high`.  The lanes
+// that share the first one's bin add up first: equal weights, as a prompt's zeros are, would meet in one
+// word of LDS, an addition after the other (32 units of 8000 zeros 27.6 us, so 16.6; random weights 16.8 and
+// 16.4, of 4160 slots 14.3 and 15.0).
 __device__ __forceinline__ void evict_add(uint32_t* hist, int bin, bool in, bool high) {
   const uint64_t some = __ballot(in);
   if (!some) return;
@@ -282,9 +283,9 @@ __device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, in
 // this lane.  `before`: evict_count's sums of the slots before the wave's, `all`: of the unit.  Of the
 // ties the lowest `need` stay, so those below keep go first.  -> the unit's pairs
 template <int R, typename Hole, typename Mover>
-__device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&key)[R], int t0, int n, int per, uint32_t top,
-                                          int need,                                          const int (&before)[4], const int (&all)[4], Hole&& put_hole,
-                                          Mover&& put_mover) {
+__device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&key)[R], int t0, int n, int per,
+                                          uint32_t top, int need, const int (&before)[4], const int (&all)[4],
+                                          Hole&& put_hole, Mover&& put_mover) {
   const int lane = threadIdx.x & 63;
   const uint64_t below = (1ull << lane) - 1;
   const int high = max(0, need - all[1]);  // ties past keep that stay
