@@ -676,6 +676,22 @@ def test_write_counts_past_the_rows(gpu):
     assert torch.equal(cache.k[2, :, :2], k[0, 1:].transpose(0, 1)) and not cache.k[2, :, 2:].any() and not cache.k[:2].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_write_negative_counts_of_many_tokens(gpu, dtype):
+    """A negative count means no rows, down to -2^31, also for the tokens behind a workgroup's first."""
+    B, S, HK, D, page = 6, 70, 2, 64, 16  # 32 tokens a workgroup
+    cache = PagedKV.empty(B * 8, page, HK, D, dtype=dtype, track=True, device=gpu)
+    cache.weights.fill_(3.0)
+    want = arrays(cache)
+    k = torch.randn(B, S, HK, D, device=gpu).to(torch.bfloat16)
+    table = torch.arange(B * 8, dtype=torch.int32, device=gpu).view(B, 8)
+    start = torch.full((B,), 5, dtype=torch.int32, device=gpu)
+    low = -2 ** 31
+    cache.write(k, k, table, start, torch.tensor([low, low + 1, low + 31, low + 33, -1, -70], dtype=torch.int32, device=gpu))
+    for name, x in arrays(cache).items():
+        assert np.array_equal(x, want[name]), name
+
+
 def test_captured_cut_of_long_sequences(gpu):
     """Units that several workgroups share, cut in a captured graph: every replay equals the eager call."""
     page, HK, n, keep = 64, 2, 12000, 1000

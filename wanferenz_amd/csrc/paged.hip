@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedView c, WriteArgs
   uint8_t* const dst = side ? c.v : c.k;
   const uint32_t per = uint32_t(c.heads) * LPR;  // 16-byte pieces of a token
   for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
-    const int count = a.count ? min(a.count[b], a.S) : a.S;
+    const int count = a.count ? min(max(a.count[b], 0), a.S) : a.S;  // not negative: i0 is taken off it
     const int tokens = min(count - i0, a.block);
     if (tokens <= 0) continue;
     const int start = a.start[b];
