@@ -56,23 +56,22 @@ def attend(cache, q, table, lens, scale, sink=None):
 
 
 def evict_pairs(weights, positions, n, keep, first, recent, present=None):
-    """One head's (holes, movers) among its n slots: lists of slots, paired in order."""
+    """One head's (holes, movers) among its n slots: lists of slots, paired in order.  Slots that are not
+    present are neither kept nor filled, so as many stay as are present below keep."""
     if n <= keep:
         return [], []
-    present = [True] * n if present is None else present
-    last = max((int(positions[t]) for t in range(n) if present[t]), default=0)
+    slots = [t for t in range(n) if present is None or present[t]]
+    last = max((int(positions[t]) for t in slots), default=0)
 
     def key(t):
-        if not present[t]:
-            return (0, 0.0)
         if positions[t] < first or positions[t] > last - recent:
             return (2, 0.0)
         w = float(weights[t])
         return (0, 0.0) if np.isnan(w) else (1, w)
 
-    order = sorted(range(n), key=lambda t: (-key(t)[0], -key(t)[1], t))
-    kept = set(order[:keep])
-    return [t for t in range(keep) if t not in kept], [t for t in range(keep, n) if t in kept]
+    order = sorted(slots, key=lambda t: (-key(t)[0], -key(t)[1], t))
+    kept = set(order[:sum(t < keep for t in slots)])
+    return [t for t in slots if t < keep and t not in kept], [t for t in slots if t >= keep and t in kept]
 
 
 def evict(cache, table, lens, keep, first=0, recent=0):
@@ -88,7 +87,8 @@ def evict(cache, table, lens, keep, first=0, recent=0):
             w = [cache["weights"][p, h, r] if p >= 0 else 0.0 for p, r in at]
             pos = [cache["positions"][p, h, r] if p >= 0 else 0 for p, r in at]
             holes, movers = evict_pairs(w, pos, n, keep, first, recent, present)
-            moved = [(at[a], at[c]) for a, c in zip(holes, movers) if at[a][0] >= 0 and at[c][0] >= 0]
+            assert len(holes) == len(movers)
+            moved = [(at[a], at[c]) for a, c in zip(holes, movers)]
             for x in cache.values():
                 for (tp, tr), (fp, fr) in moved:
                     x[tp, h, tr] = x[fp, h, fr]

@@ -440,6 +440,40 @@ def test_evict_long(gpu, n, keep):
     assert torch.equal(flat(low), (after & 0x7FFF).to(torch.int16))
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("slots", [0, 9000])
+def test_evict_keeps_protected_slots_beside_missing_pages(gpu, slots, inplace):
+    """What ``first`` and ``recent`` protect stays below the new length wherever pages are missing, as long as the
+    pages below keep hold as many; no page below keep at all leaves everything where it is.  A page's slots of
+    NaN weight count, and are the first to go."""
+    lens, page, keep, first, recent = [300, 200, 120, 97], 16, 96, 6, 20
+    cache, _, _, table = make(gpu, 33, lens, HK=2, D=64, page=page, track=True, width=max(19, -(-slots // page)))
+    for b, n in enumerate(lens):
+        for t in range(n):
+            cache.positions[table[b, t // page], :, t % page] = (7 * t + 3) % n if b else t
+    cache.weights[table[1, 3]] = float("nan")
+    table[0, 1], table[0, 4] = -1, cache.pages
+    table[1, 2], table[1, 9] = -1, -1
+    table[2, :6] = -1
+    want = arrays(cache)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    ref = op.evict(want, table, lens, keep, first, recent)
+    got = cache.evict(torch.from_numpy(table).to(gpu), n, keep, first=first, recent=recent, out=n if inplace else None)
+    assert np.array_equal(got.cpu().numpy(), ref)
+    after = arrays(cache)
+    for name, x in after.items():
+        assert np.array_equal(x, want[name], equal_nan=name == "weights"), name
+    pos = after["positions"]
+    held = [[set(pos[table[b, t // page], h, t % page] for t in range(keep) if 0 <= table[b, t // page] < cache.pages)
+             for h in range(2)] for b in range(4)]
+    for h in range(2):
+        assert set(range(first)) | set(range(300 - recent, 300)) <= held[0][h]
+        gone = {(7 * t + 3) % 200 for t in [*range(32, 48), *range(144, 160)]}
+        newest = max(p for p in range(200) if p not in gone)
+        assert {p for p in [*range(first), *range(newest - recent + 1, newest + 1)] if p not in gone} <= held[1][h]
+        assert not held[2][h]
+
+
 # ---------------------------------------------------------------- together ----
 
 

@@ -174,3 +174,13 @@ def test_plain_evict_keeps_the_heaviest():
     assert op.evict_pairs([1] * 6, [9, 8, 7, 6, 5, 4], 6, 3, 0, 1) == ([], [])
     assert op.evict_pairs([float("nan"), 0, 0], [0, 1, 2], 3, 2, 0, 0) == ([0], [2])
     assert op.evict_pairs(w, pos, 4, 4, 0, 0) == ([], [])
+
+
+def test_plain_evict_leaves_missing_pages_out():
+    """A missing slot below keep takes no kept slot with it: as many stay as have a place, protected ones first."""
+    w = [1.0] * 8
+    missing = [False, False, True, True, True, True, True, True]  # two of the four places have no page
+    assert op.evict_pairs(w, list(range(8)), 8, 4, 0, 2, missing) == ([2, 3], [6, 7])
+    missing = [True, True, False, True, True, True, True, False]
+    assert op.evict_pairs([5, 1, 9, 2, 3, 4, 6, 9], list(range(8)), 8, 4, 1, 0, missing) == ([1, 3], [5, 6])
+    assert op.evict_pairs(w, list(range(8)), 8, 4, 4, 0, [False] * 4 + [True] * 4) == ([], [])

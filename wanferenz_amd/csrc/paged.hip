@@ -124,11 +124,12 @@ constexpr int kEvictTally = 1028;        // words of a chunk's sums over the las
 constexpr int kNoPosition = -0x7FFFFFFF - 1;
 
 // A slot's place in the order of what stays, as an unsigned number: the float's bits, ordered
-// like the values (NaN lowest), a protected slot above them all.
+// like the values (NaN lowest, 1), a protected slot above them all.  Slots without a page have 0: they are
+// neither kept nor filled, so as many slots stay as have a page below keep.
 __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
   if (safe) return 0xFFFFFFFFu;
   const uint32_t u = __float_as_uint(w);
-  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 1u;
   const uint32_t k = u == 0x80000000u ? 0u : u;  // -0 and 0 weigh the same
   return (k & 0x80000000u) ? ~k : k | 0x80000000u;
 }
@@ -148,7 +149,7 @@ struct EvictArgs {
   int32_t* holes;   // [unit][moves]
   int32_t* movers;
   EvictUnit* unit;  // shared units only, as the rest
-  int32_t* newest;  // [unit][chunk]
+  int2* newest;     // [unit][chunk]: its newest position, its slots below keep that have a page
   uint32_t* tally;  // [unit][chunk][kEvictTally]
   uint32_t* keys;   // [unit][capacity]
   int64_t moves, capacity;
@@ -216,6 +217,15 @@ __device__ __forceinline__ void evict_add(uint32_t* hist, int bin, bool in, bool
   if (in && !same) atomicAdd(&hist[bin], high ? 1u << 16 : 1u);
 }
 
+// A wave's slots below keep that have a page.
+template <int R>
+__device__ __forceinline__ int evict_places(const int64_t (&at)[R], int t0, int keep) {
+  int have = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) have += __popcll(__ballot(at[i] >= 0 && t0 + 64 * i < keep));
+  return have;
+}
+
 // The bin, from the top, in which the need-th key lies, and how many of its keys are needed.  Called
 // by a whole workgroup; the bins are not changed until everyone has read them.  -> whether all are needed
 template <int THREADS>
@@ -265,13 +275,13 @@ __device__ __forceinline__ bool evict_under(uint32_t k, uint32_t prefix, int d) 
 
 // A wave's counts of its R rounds: kept slots above the threshold and ties, below keep and past it.
 template <int R>
-__device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, int n, int per, int keep, uint32_t top,
+__device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, int per, int keep, uint32_t top,
                                             int (&sum)[4]) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (i >= per) break;
     const int t = t0 + 64 * i;
-    const bool in = t < n, low = t < keep, gt = in && key[i] > top, tie = in && key[i] == top;
+    const bool low = t < keep, gt = key[i] > top, tie = key[i] != 0 && key[i] == top;
     sum[0] += __popcll(__ballot(gt && low));
     sum[1] += __popcll(__ballot(tie && low));
     sum[2] += __popcll(__ballot(gt && !low));
@@ -280,27 +290,29 @@ __device__ __forceinline__ void evict_count(const uint32_t (&key)[R], int t0, in
 }
 
 // A wave's part of the lists: hole(i, r) and mover(i, r) take the i-th of the unit, which is in round r of
-// this lane.  `before`: evict_count's sums of the slots before the wave's, `all`: of the unit.  Of the
-// ties the lowest `need` stay, so those below keep go first.  -> the unit's pairs
+// this lane.  `before`: evict_count's sums of the slots before the wave's, `all`: of the unit, `have`:
+// evict_places of the slots before the wave's.  Of the ties the lowest `need` stay, so those below keep go
+// first.  -> the unit's pairs
 template <int R, typename Hole, typename Mover>
-__device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&key)[R], int t0, int n, int per,
-                                          uint32_t top, int need, const int (&before)[4], const int (&all)[4],
+__device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&key)[R], int t0, int per, uint32_t top,
+                                          int need, const int (&before)[4], const int (&all)[4], int have,
                                           Hole&& put_hole, Mover&& put_mover) {
   const int lane = threadIdx.x & 63;
   const uint64_t below = (1ull << lane) - 1;
   const int high = max(0, need - all[1]);  // ties past keep that stay
   const int pairs = int(min(int64_t(all[2] + min(all[3], high)), a.moves));
   int ties = before[1] + before[3];
-  int ih = min(t0 - lane, a.keep) - before[0] - min(before[1], need);  // dropped slots below keep
+  int ih = have - before[0] - min(before[1], need);  // dropped slots below keep
   int im = before[2] + min(before[3], high);                          // kept slots past it
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (i >= per) break;
     const int t = t0 + 64 * i;
-    const uint64_t tie = __ballot(t < n && key[i] == top);
-    const bool kept = t < n && (key[i] > top || (key[i] == top && ties + __popcll(tie & below) < need));
+    const bool in = key[i] != 0;
+    const uint64_t tie = __ballot(in && key[i] == top);
+    const bool kept = key[i] > top || (in && key[i] == top && ties + __popcll(tie & below) < need);
     ties += __popcll(tie);
-    const bool hole = t < n && !kept && t < a.keep, mover = kept && t >= a.keep;
+    const bool hole = in && !kept && t < a.keep, mover = kept && t >= a.keep;
     const uint64_t bh = __ballot(hole), bm = __ballot(mover);
     const int x = ih + __popcll(bh & below), y = im + __popcll(bm & below);
     if (hole && x < pairs) put_hole(x, i);
@@ -322,7 +334,7 @@ template <bool MOVE>
 __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictArgs a, int row_bytes) {
   constexpr int R = kEvictSmall / kEvictThreads, NW = kEvictThreads / 64;
   __shared__ uint32_t s_hist[3][kEvictBins];
-  __shared__ int s_last[NW];
+  __shared__ int s_last[NW], s_have[NW];
   __shared__ __align__(16) uint2 s_count[NW];
   const int u = blockIdx.x, b = u / a.c.heads, h = u - b * a.c.heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -345,22 +357,30 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
 #pragma unroll
   for (int i = 0; i < R; ++i) last = max(last, p[i]);
   last = wave_max(last);
-  if (lane == 0) s_last[wave] = last;
+  const int places = evict_places<R>(at, t0, a.keep);
+  if (lane == 0) {
+    s_last[wave] = last;
+    s_have[wave] = places;
+  }
   __syncthreads();
+  int need = 0, have = 0;  // the unit's places, and those before the wave's slots
 #pragma unroll
-  for (int i = 0; i < NW; ++i) last = max(last, s_last[i]);
+  for (int i = 0; i < NW; ++i) {
+    last = max(last, s_last[i]);
+    have = i == wave ? need : have;
+    need += s_have[i];
+  }
   const int64_t old = int64_t(last) - a.recent;  // positions above it are protected
   uint32_t key[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) key[i] = at[i] < 0 ? 0u : evict_key(w[i], p[i] < a.first || int64_t(p[i]) > old);
   uint32_t top = 0;
-  int need = a.keep;
 #pragma unroll
   for (int d = 0; d < 3; ++d) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (i >= per) break;
-      evict_add(s_hist[d], evict_digit(key[i], d), t0 + 64 * i < end && evict_under(key[i], top, d), false);
+      evict_add(s_hist[d], evict_digit(key[i], d), key[i] != 0 && evict_under(key[i], top, d), false);
     }
     __syncthreads();
     int bin;
@@ -369,7 +389,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
     if (whole) break;  // the bin's keys all stay: the threshold is its lowest, the digits below 0
   }
   int sum[4] = {0, 0, 0, 0};
-  evict_count<R>(key, t0, end, per, a.keep, top, sum);
+  evict_count<R>(key, t0, per, a.keep, top, sum);
   // two counts a word: they add up to kEvictSmall at most
   if (lane == 0) s_count[wave] = make_uint2(uint32_t(sum[0]) << 16 | uint32_t(sum[1]), uint32_t(sum[2]) << 16 | uint32_t(sum[3]));
   __syncthreads();
@@ -386,7 +406,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
     // the pairs' rows stay in LDS, in the histograms' place
     int64_t* const holes = reinterpret_cast<int64_t*>(&s_hist[0][0]);
     int64_t* const movers = holes + kEvictPairs;
-    const int pairs = evict_list<R>(a, key, t0, end, per, top, need, before, all, [&](int i, int r) { holes[i] = at[r]; },
+    const int pairs = evict_list<R>(a, key, t0, per, top, need, before, all, have, [&](int i, int r) { holes[i] = at[r]; },
                                     [&](int i, int r) { movers[i] = at[r]; });
     __syncthreads();
     const int lpr = row_bytes / 16;
@@ -394,7 +414,8 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
   } else {
     int32_t* const holes = a.holes + u * a.moves;
     int32_t* const movers = a.movers + u * a.moves;
-    const int pairs = evict_list<R>(a, key, t0, end, per, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
+    const int pairs = evict_list<R>(a, key, t0, per, top, need, before, all, have,
+                                    [&](int i, int r) { holes[i] = t0 + 64 * r; },
                                     [&](int i, int r) { movers[i] = t0 + 64 * r; });
     if (tid == 0) a.counts[u] = pairs;
   }
@@ -404,7 +425,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
 // units took it 87 us, 65535 of one 160): a workgroup per chunk of kEvictChunk slots, a launch for
 // each time that the workgroups have to meet.  Every launch costs its 4 us whatever it does, so a chunk
 // is what one workgroup of four waves does in that time: 26 us in all for both sizes with 1024 slots,
-// 48 with 4096.  STEP 0: the chunk's newest position, and the unit's
+// 48 with 4096.  STEP 0: the chunk's newest position and places, and the unit's
 // histograms cleared.  1: keys and the first digit's histogram.  2, 3: the second's and third's, the
 // third with the chunk's own: tally[j] = its keys of at least the first two digits' threshold followed
 // by j, those below keep in the low 16 bits and those past it in the high.  4: the threshold, what the other chunks
@@ -417,7 +438,7 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
   const int32_t* const trow = a.table + int64_t(b) * a.width;
   const int n = evict_len(a, b);
   EvictUnit& st = a.unit[u];
-  int32_t* const newest = a.newest + int64_t(u) * nb;
+  int2* const newest = a.newest + int64_t(u) * nb;
   uint32_t* const tally = a.tally + int64_t(u) * nb * kEvictTally;
   uint32_t* const keys = a.keys + u * a.capacity;
   if constexpr (STEP == 0)
@@ -431,7 +452,7 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
   if (chunk >= chunks) return;
   const int t0 = chunk * kEvictChunk + wave * (64 * R) + lane;
   const int end = min(n, t0 - lane + 64 * R);
-  __shared__ int s_wave[4][NW];
+  __shared__ int s_wave[5][NW];
   uint32_t key[R];
   if constexpr (STEP <= 1) {
     int64_t at[R];
@@ -443,14 +464,22 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
 #pragma unroll
       for (int i = 0; i < R; ++i) last = max(last, p[i]);
       last = wave_max(last);
-      if (lane == 0) s_wave[0][wave] = last;
+      const int places = evict_places<R>(at, t0, a.keep);
+      if (lane == 0) {
+        s_wave[0][wave] = last;
+        s_wave[1][wave] = places;
+      }
       __syncthreads();
       last = wave_max(s_wave[0][lane & (NW - 1)]);
-      if (tid == 0) newest[chunk] = last;
+      if (tid == 0) {
+        int have = 0;
+        for (int i = 0; i < NW; ++i) have += s_wave[1][i];
+        newest[chunk] = make_int2(last, have);
+      }
       return;
     }
     int last = kNoPosition;
-    for (int i = lane; i < chunks; i += 64) last = max(last, newest[i]);
+    for (int i = lane; i < chunks; i += 64) last = max(last, newest[i].x);
     const int64_t old = int64_t(wave_max(last)) - a.recent;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -463,7 +492,11 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
   }
   // the threshold's digits so far; the launch before wrote what is read here
   uint32_t top = 0;
-  int need = a.keep;
+  int need = 0;
+  if constexpr (STEP == 2) {
+    for (int i = lane; i < chunks; i += 64) need += newest[i].y;
+    need = wave_sum(need);
+  }
   if constexpr (STEP > 2) {
     top = uint32_t(st.known[STEP - 3][0]);
     need = st.known[STEP - 3][1];
@@ -484,7 +517,7 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; ++i)
-      evict_add(s_hist, evict_digit(key[i], d), t0 + 64 * i < end && evict_under(key[i], top, d), false);
+      evict_add(s_hist, evict_digit(key[i], d), key[i] != 0 && evict_under(key[i], top, d), false);
     __syncthreads();
     for (int i = tid; i < kEvictBins; i += kEvictChunkThreads)
       if (s_hist[i]) atomicAdd(&st.hist[d][i], s_hist[i]);  // integers: the order does not matter
@@ -499,8 +532,8 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int t = t0 + 64 * i;
-      const bool in = t < end, gt = in && key[i] >> 10 > top >> 10;
-      evict_add(s_hist, evict_digit(key[i], 2), in && evict_under(key[i], top, 2), t >= a.keep);
+      const bool gt = key[i] >> 10 > top >> 10;
+      evict_add(s_hist, evict_digit(key[i], 2), key[i] != 0 && evict_under(key[i], top, 2), t >= a.keep);
       more += uint32_t(__popcll(__ballot(gt && t < a.keep))) + (uint32_t(__popcll(__ballot(gt && t >= a.keep))) << 16);
     }
     if (lane == 0) s_wave[0][wave] = int(more);
@@ -536,11 +569,17 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
   }
   if constexpr (STEP == 4) {
     int sum[4] = {0, 0, 0, 0};
-    evict_count<R>(key, t0, end, R, a.keep, top, sum);
-    if (lane == 0)
+    evict_count<R>(key, t0, R, a.keep, top, sum);
+    int have = 0;  // the places of the wave, then of those before it
+#pragma unroll
+    for (int i = 0; i < R; ++i) have += __popcll(__ballot(key[i] != 0 && t0 + 64 * i < a.keep));
+    if (lane == 0) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) s_wave[j][wave] = sum[j];
+      s_wave[4][wave] = have;
+    }
     __syncthreads();
+    have = 0;
     int before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
     const int bin = evict_digit(top, 2);
     for (int i = lane; i < chunks; i += 64) {
@@ -552,7 +591,10 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
         all[j] += x[j];
         before[j] += i < chunk ? x[j] : 0;
       }
+      have += i < chunk ? newest[i].y : 0;
     }
+    have = wave_sum(have);
+    for (int i = 0; i < wave; ++i) have += s_wave[4][i];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       all[j] = wave_sum(all[j]);
@@ -561,7 +603,8 @@ __global__ __launch_bounds__(kEvictChunkThreads) void paged_evict_chunk_kernel(E
     }
     int32_t* const holes = a.holes + u * a.moves;
     int32_t* const movers = a.movers + u * a.moves;
-    const int pairs = evict_list<R>(a, key, t0, end, R, top, need, before, all, [&](int i, int r) { holes[i] = t0 + 64 * r; },
+    const int pairs = evict_list<R>(a, key, t0, R, top, need, before, all, have,
+                                    [&](int i, int r) { holes[i] = t0 + 64 * r; },
                                     [&](int i, int r) { movers[i] = t0 + 64 * r; });
     if (chunk == 0 && tid == 0) a.counts[u] = pairs;
   }
@@ -599,7 +642,7 @@ static EvictSizes evict_sizes(const wz_paged_kv* c, int64_t B, int64_t width, in
   if (capacity > kEvictSmall) {
     z.chunks = (capacity + kEvictChunk - 1) / kEvictChunk;
     z.unit = z.units * int64_t(sizeof(EvictUnit));
-    z.newest = (4 * z.units * z.chunks + 15) / 16 * 16;
+    z.newest = (8 * z.units * z.chunks + 15) / 16 * 16;
     z.tally = 4 * kEvictTally * z.units * z.chunks;
     z.keys = 4 * z.units * capacity;
   }
@@ -701,7 +744,7 @@ extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, in
   a.lens = lens;
   a.new_lens = new_lens;
   a.unit = reinterpret_cast<EvictUnit*>(take(z.unit));
-  a.newest = reinterpret_cast<int32_t*>(take(z.newest));
+  a.newest = reinterpret_cast<int2*>(take(z.newest));
   a.tally = reinterpret_cast<uint32_t*>(take(z.tally));
   a.keys = reinterpret_cast<uint32_t*>(take(z.keys));
   a.counts = reinterpret_cast<int32_t*>(take(z.counts));

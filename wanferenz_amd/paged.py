@@ -236,7 +236,8 @@ class PagedKV:
         slots of positions below ``first``, the ``recent`` newest positions and then the slots of the highest
         weight stay (equal weights: the lower slot; NaN: the lowest).  The i-th dropped slot below ``keep`` takes
         over the i-th kept slot from ``keep`` on, with its rows, scales, weight and position, so nothing else
-        moves and the pages past ``keep`` are free; slot order is no longer token order.  Sequences within the
+        moves and the pages past ``keep`` are free; slot order is no longer token order.  Slots that the table has
+        no page for are neither kept nor filled: as many stay as have a page below ``keep``.  Sequences within the
         budget are left as they are.  -> min(lens, keep) int32 [b], in ``out`` if given (``lens`` itself may be)."""
         keep, first, recent = int(keep), int(first), int(recent)
         if self.weights is None:
