@@ -421,7 +421,7 @@ int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q
  * the i-th dropped slot below `keep` takes over the i-th kept slot from `keep` on, with
  * its K, V, scales, weight and position.  Slots whose page is missing are neither kept nor
  * filled: as many slots stay as have a page below keep.  new_lens[b] = min(lens[b], keep) (may
- * be lens itself); sequences within the budget are left as they are.  first + recent <= keep. */
+ * be lens itself, and overlaps it in no other way); sequences within the budget are left as they are.  first + recent <= keep. */
 int64_t wz_paged_evict_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t table_width, int64_t keep);
 int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, int64_t table_width, const int32_t* lens,
                    int32_t* new_lens, int64_t B, int64_t keep, int64_t first, int64_t recent, void* workspace,

@@ -176,6 +176,15 @@ def test_plain_evict_keeps_the_heaviest():
     assert op.evict_pairs(w, pos, 4, 4, 0, 0) == ([], [])
 
 
+def test_evict_refuses_lengths_that_overlap_at_an_offset():
+    """new_lens may be lens, or apart from it: shifted by less than the batch it would be read half written."""
+    c = cache(**TRACK)
+    for new in (4096 - 8, 4096 - 4, 4096 + 4, 4096 + 8):
+        assert evict(c, lens=4096, new=new, B=3) == -1 and "overlaps lens" in err()
+    for new in (4096 - 12, 4096, 4096 + 12):
+        assert evict(c, lens=4096, new=new, B=3) == -3 and "needed" in err()
+
+
 def test_plain_evict_leaves_missing_pages_out():
     """A missing slot below keep takes no kept slot with it: as many stay as have a place, protected ones first."""
     w = [1.0] * 8

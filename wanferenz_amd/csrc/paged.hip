@@ -725,6 +725,10 @@ extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, in
                      (long long)keep, (long long)first, (long long)recent);
   if (B == 0) return WZ_OK;
   if (!lens || !new_lens || (table_width > 0 && !table)) return set_error(WZ_EINVAL, "paged_evict: null pointer");
+  // other workgroups read lens while new_lens is written: the same array is looked after, a shifted one is not
+  if (const uintptr_t l = reinterpret_cast<uintptr_t>(lens), o = reinterpret_cast<uintptr_t>(new_lens);
+      l != o && (l < o ? o - l : l - o) < 4 * uintptr_t(B))
+    return set_error(WZ_EINVAL, "paged_evict: new_lens overlaps lens (it may be lens itself)");
   const int64_t need = wz_paged_evict_workspace_bytes(cache, B, table_width, keep);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(WZ_ESPACE, "paged_evict: workspace of %lld bytes, %lld needed",

@@ -238,7 +238,8 @@ class PagedKV:
         over the i-th kept slot from ``keep`` on, with its rows, scales, weight and position, so nothing else
         moves and the pages past ``keep`` are free; slot order is no longer token order.  Slots that the table has
         no page for are neither kept nor filled: as many stay as have a page below ``keep``.  Sequences within the
-        budget are left as they are.  -> min(lens, keep) int32 [b], in ``out`` if given (``lens`` itself may be)."""
+        budget are left as they are.  -> min(lens, keep) int32 [b], in ``out`` if given (``lens`` itself may be, another view that
+        overlaps it may not)."""
         keep, first, recent = int(keep), int(first), int(recent)
         if self.weights is None:
             raise ValueError("PagedKV.evict: the cache is not tracked (weights and positions)")
