@@ -176,6 +176,16 @@ def test_plain_evict_keeps_the_heaviest():
     assert op.evict_pairs(w, pos, 4, 4, 0, 0) == ([], [])
 
 
+def test_partials_of_odd_rows_lie_on_16_bytes():
+    """A worker has two partials of m and l (rounded up to 16 bytes together) and O [rows, 64], and one record
+    of 16 bytes; the number of workers is the same for 1, 2 and 3 rows a KV head."""
+    c = cache()
+    need = [N.lib().wz_paged_attn_workspace_bytes(ctypes.byref(c), 1, 1, 2 * rows, 3, 0) for rows in (1, 2, 3)]
+    slots = [16 + 4 * 64, 16 + 4 * 2 * 64, 32 + 4 * 3 * 64]
+    workers = need[1] // (2 * slots[1] + 16)
+    assert need == [workers * (2 * s + 16) for s in slots]
+
+
 def test_evict_refuses_lengths_that_overlap_at_an_offset():
     """new_lens may be lens, or apart from it: shifted by less than the batch it would be read half written."""
     c = cache(**TRACK)

@@ -58,7 +58,7 @@ struct PagedAttnArgs {
   const int32_t* table;
   const int32_t* lens;
   uint16_t* o;
-  float* part;    // 2 W slots of m[rows], l[rows] and O[rows][D]
+  float* part;    // 2 W slots of m[rows], l[rows] and O[rows][D] (paged_head, paged_slot)
   PagedCut* cut;  // a unit where by_unit, else the cut unit that begins in a worker's share
   float* ml;      // accumulate: per unit and row the final maximum and 1 / sum
   float* scores;  // accumulate: y [B, heads, R, capacity]
@@ -66,6 +66,11 @@ struct PagedAttnArgs {
   int64_t capacity;  // slots of the table, width * page
   float scale2;      // softmax scale * log2(e)
 };
+
+// Floats of a partial before its O, and in all.  O is stored and read 16 bytes at a time, so with odd rows
+// two floats are left out before it.
+__host__ __device__ __forceinline__ int paged_head(int rows) { return (2 * rows + 3) & ~3; }
+__host__ __device__ __forceinline__ int64_t paged_slot(int rows, int D) { return paged_head(rows) + int64_t(rows) * D; }
 
 static inline int64_t paged_units(const PagedAttnArgs& a) {
   const int R = a.S * (a.H / a.c.heads);
@@ -649,7 +654,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
       l_run[rt] += __shfl_xor(l_run[rt], 32, 64);
     }
     {
-      float* const part = a.part + (2 * int64_t(w) + (g0 == 0 ? 1 : 0)) * (int64_t(a.rows) * (D + 2));
+      float* const part = a.part + (2 * int64_t(w) + (g0 == 0 ? 1 : 0)) * paged_slot(a.rows, D);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int rl = rh * C::WROWS + 16 * rt + nl, r = rg * ROWS + rl;
@@ -683,7 +688,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            *reinterpret_cast<v4f*>(part + 2 * a.rows + rl * D + 16 * nt + 4 * g) = acc[rt][nt];
+            *reinterpret_cast<v4f*>(part + paged_head(a.rows) + rl * D + 16 * nt + 4 * g) = acc[rt][nt];
         }
       }
     }
@@ -710,12 +715,12 @@ __device__ __forceinline__ void paged_join(const PagedAttnArgs& a, int unit, int
   const int ch = tid % CH, gr = tid / CH;
   const int rl = WIDE ? rows : rows * GR + gr, r = rg * a.unit_rows + rl;
   if (rl >= a.rows || r >= R) return;  // WIDE: the whole workgroup
-  const int64_t slot = int64_t(a.rows) * (D + 2);
+  const int64_t slot = paged_slot(a.rows, D);
   const float* const part = a.part + rl;
   auto at = [&](int j) { return part + (2 * (int64_t(cut.w) + j) + (j == 0 ? 1 : 0)) * slot; };
   const int head = hk * grp + r % grp;
   const float sk = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-  const int off = 2 * a.rows + rl * (D - 1) + 4 * ch;
+  const int off = paged_head(a.rows) + rl * (D - 1) + 4 * ch;
   float M = sk, den = 0.0f;
   v4f o = v4f{0.f, 0.f, 0.f, 0.f};
   float Me;
@@ -805,7 +810,7 @@ __device__ __forceinline__ void paged_weigh(const PagedAttnArgs& a, int bh, int 
         m = ml[2 * r];
         inv = ml[2 * r + 1];
       } else {
-        const int64_t slot = int64_t(a.rows) * (D + 2);
+        const int64_t slot = paged_slot(a.rows, D);
         const float* const part = a.part + r;
         auto at = [&](int j) { return part + (2 * (int64_t(cut.w) + j) + (j == 0 ? 1 : 0)) * slot; };
         const float sk = a.sink ? a.sink[hk * grp + r % grp] * kLog2e : -INFINITY;

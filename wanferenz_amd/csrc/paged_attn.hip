@@ -28,7 +28,7 @@ static PagedAttnSizes paged_attn_sizes(const wz_paged_kv* c, int64_t B, int64_t 
   a.H = int(H);
   int workers = 0;
   const int64_t rows = paged_attn_any(c->head_dim, a, true, &workers, nullptr);
-  z.part = (2 * workers * rows * (c->head_dim + 2) + 3) / 4 * 4;
+  z.part = 2 * workers * paged_slot(int(rows), c->head_dim);
   z.cut = workers * int64_t(sizeof(PagedCut) / sizeof(float));
   if (accumulate) {
     z.ml = (2 * B * c->kv_heads * R + 3) / 4 * 4;

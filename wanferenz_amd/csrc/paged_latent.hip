@@ -489,7 +489,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
                                                                  f32x2_to_bf16x2(acc[ht][nt][2] * iv, acc[ht][nt][3] * iv));
       }
     } else {
-      float* const part = a.part + (2 * int64_t(w) + (g0 == 0 ? 1 : 0)) * (int64_t(a.rows) * (D + 2));
+      float* const part = a.part + (2 * int64_t(w) + (g0 == 0 ? 1 : 0)) * paged_slot(a.rows, D);
       if (wave == 0 && lane < ROWS && row0 + lane < R) {
         part[lane] = m_run;
         part[a.rows + lane] = l;
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
         if (row0 + rl >= R) continue;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-          *reinterpret_cast<v4f*>(part + 2 * a.rows + rl * D + 16 * NT * wave + 16 * nt + 4 * g) = acc[ht][nt];
+          *reinterpret_cast<v4f*>(part + paged_head(a.rows) + rl * D + 16 * NT * wave + 16 * nt + 4 * g) = acc[ht][nt];
       }
     }
     meet();  // the buffers are free for the next part's tiles
