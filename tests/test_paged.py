@@ -176,6 +176,20 @@ def test_plain_evict_keeps_the_heaviest():
     assert op.evict_pairs(w, pos, 4, 4, 0, 0) == ([], [])
 
 
+def test_evict_sizes_that_do_not_fit_64_bits_are_refused():
+    """B kv_heads and B kv_heads slots are not multiplied out before B is checked."""
+    L = N.lib()
+    c = cache(heads=4, **TRACK)
+    for B in (16384, 2 ** 61, 2 ** 62, 2 ** 62 + 1, 2 ** 63 - 1):
+        assert evict(c, B=B) == -1 and "65535" in err(), B
+        assert L.wz_paged_evict_workspace_bytes(ctypes.byref(c), B, 3, 8) == 0
+    assert evict(c, B=16383) == -3
+    assert L.wz_paged_evict_workspace_bytes(ctypes.byref(c), 16383, 3, 8) == 4 * 65532 + 8 * 65532 * 8
+    for B, width, keep in ((1, 2 ** 62, 8), (1, -1, 8), (1, 3, -1), (1, 3, 2 ** 40), (0, 3, 8), (-1, 3, 8)):
+        assert L.wz_paged_evict_workspace_bytes(ctypes.byref(c), B, width, keep) == 0
+    assert L.wz_paged_evict_workspace_bytes(None, 1, 3, 8) == 0
+
+
 def test_partials_of_odd_rows_lie_on_16_bytes():
     """A worker has two partials of m and l (rounded up to 16 bytes together) and O [rows, 64], and one record
     of 16 bytes; the number of workers is the same for 1, 2 and 3 rows a KV head."""

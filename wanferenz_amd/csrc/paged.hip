@@ -118,6 +118,7 @@ constexpr int kEvictSmall = 8192;        // slots that one workgroup holds
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictChunk = 1024;        // slots of a workgroup where several share a unit
 constexpr int kEvictChunkThreads = 256;
+constexpr int64_t kEvictUnits = 65535;   // of a call: the grid's second dimension
 constexpr int64_t kEvictFused = 65536;   // bytes of K a unit's one workgroup moves itself,
 constexpr int kEvictPairs = 1024;        // in up to as many rows
 constexpr int kEvictTally = 1028;        // words of a chunk's sums over the last digit
@@ -707,7 +708,9 @@ extern "C" int wz_paged_kv_write(const wz_paged_kv* cache, const void* k_bf16, c
 extern "C" int64_t wz_paged_evict_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t table_width,
                                                   int64_t keep) {
   using namespace wz;
-  if (!cache || B <= 0 || table_width < 0 || keep < 0 || cache->page_size <= 0 || cache->kv_heads <= 0) return 0;
+  PagedView view;
+  if (paged_view("paged_evict", cache, table_width, &view) != WZ_OK) return 0;
+  if (B <= 0 || B > kEvictUnits / view.heads || keep < 0 || keep > 0x7FFFFFFFLL) return 0;
   return evict_sizes(cache, B, table_width, keep).total;
 }
 
@@ -718,8 +721,9 @@ extern "C" int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, in
   PagedView c;
   if (int rc = paged_view("paged_evict", cache, table_width, &c)) return rc;
   if (!c.weights) return set_error(WZ_EINVAL, "paged_evict: the cache is not tracked (weights and positions)");
-  if (B < 0 || B * c.heads > 65535)
-    return set_error(WZ_EINVAL, "paged_evict: %lld sequences of %d heads (65535 in all)", (long long)B, c.heads);
+  if (B < 0 || B > kEvictUnits / c.heads)
+    return set_error(WZ_EINVAL, "paged_evict: %lld sequences of %d heads (%lld in all)", (long long)B, c.heads,
+                     (long long)kEvictUnits);
   if (keep < 0 || first < 0 || recent < 0 || keep > 0x7FFFFFFFLL || first > keep || recent > keep - first)
     return set_error(WZ_EINVAL, "paged_evict: keep %lld, first %lld, recent %lld (first + recent <= keep)",
                      (long long)keep, (long long)first, (long long)recent);
