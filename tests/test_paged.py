@@ -176,6 +176,13 @@ def test_plain_evict_keeps_the_heaviest():
     assert op.evict_pairs(w, pos, 4, 4, 0, 0) == ([], [])
 
 
+def test_write_refuses_more_tokens_than_a_grid_has():
+    """Some 2^24 workgroups of 32 tokens each (2 heads of 64), of one each (64 heads)."""
+    assert write(cache(), S=2 ** 29) == -1 and "1 x 536870912 tokens" in err()
+    assert write(cache(), S=2 ** 31 - 1) == -1 and "tokens" in err()
+    assert write(cache(heads=64), S=2 ** 24) == -1 and "1 x 16777216 tokens" in err()
+
+
 def test_evict_sizes_that_do_not_fit_64_bits_are_refused():
     """B kv_heads and B kv_heads slots are not multiplied out before B is checked."""
     L = N.lib()

@@ -684,11 +684,12 @@ extern "C" int wz_paged_kv_write(const wz_paged_kv* cache, const void* k_bf16, c
   a.width = int(table_width);
   a.S = int(S);
   a.B = int(B);
-  if (B > (int64_t(1) << 40) / (S * c.heads))
-    return set_error(WZ_EINVAL, "paged_kv_write: %lld x %lld tokens", (long long)B, (long long)S);
   const int D = cache->head_dim;
   a.block = std::max(1, 256 * kWriteLoads / (c.heads * (D / 8)));
-  const dim3 grid(unsigned((S + a.block - 1) / a.block), unsigned(std::min<int64_t>(B, 65535)),
+  const int64_t blocks = (S + a.block - 1) / a.block;  // of 256 threads: a grid's side stays below 2^32
+  if (B > (int64_t(1) << 40) / (S * c.heads) || blocks > 0xFFFFFF)
+    return set_error(WZ_EINVAL, "paged_kv_write: %lld x %lld tokens", (long long)B, (long long)S);
+  const dim3 grid(unsigned(blocks), unsigned(std::min<int64_t>(B, 65535)),
                   c.shared ? 1u : 2u);
 #define WZ_PAGED_WRITE(DD)                                                                                    \
   do {                                                                                                        \
