@@ -407,7 +407,8 @@ int wz_paged_kv_write(const wz_paged_kv* cache, const void* k_bf16, const int64_
  * head_dim] bf16 (q_strides as above), H a multiple of kv_heads, query head h reading KV
  * head h / (H / kv_heads); attn_sink [H] float32 or NULL; o dense bf16, not over q.  accumulate adds to
  * each slot's weight the attention that the rows of its KV head give it, in a fixed
- * order (a tracked cache with 16-byte aligned weights, one call at a time).  lens beyond the table are cut to it. */
+ * order (a tracked cache with 16-byte aligned weights, one call at a time).  lens beyond the table are cut to it.
+ * The workspace's size is that of the current device, which the call has to run on. */
 int64_t wz_paged_attn_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t S, int64_t H, int64_t table_width,
                                       int accumulate);
 int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q_strides, const float* attn_sink,

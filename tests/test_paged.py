@@ -176,6 +176,34 @@ def test_plain_evict_keeps_the_heaviest():
     assert op.evict_pairs(w, pos, 4, 4, 0, 0) == ([], [])
 
 
+def test_workspace_is_sized_on_the_cache_s_device(monkeypatch):
+    """The partials' number goes by the device that is current in the library: the cache's own is made current."""
+    seen = []
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            seen.append(("in", self.device))
+
+        def __exit__(self, *_):
+            seen.append(("out", self.device))
+
+    class Lib:
+        @staticmethod
+        def wz_paged_attn_workspace_bytes(ref, b, s, h, width, acc):
+            seen.append((b, s, h, width, acc))
+            return 64
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(N, "lib", Lib)
+    cache = object.__new__(PagedKV)
+    cache.device, cache._ref = torch.device("cuda", 5), None
+    assert cache.attend_workspace_bytes(2, 1, 8, 3, True) == 64
+    assert seen == [("in", cache.device), (2, 1, 8, 3, 1), ("out", cache.device)]
+
+
 def test_write_refuses_more_tokens_than_a_grid_has():
     """Some 2^24 workgroups of 32 tokens each (2 heads of 64), of one each (64 heads)."""
     assert write(cache(), S=2 ** 29) == -1 and "1 x 536870912 tokens" in err()

@@ -229,7 +229,8 @@ class PagedKV:
     def attend_workspace_bytes(self, b, s, h, table_width, accumulate=False) -> int:
         """Device bytes of an ``attend`` call's partial results (and, accumulating, of its scores:
         4 b s h table_width page_size bytes)."""
-        return int(N.lib().wz_paged_attn_workspace_bytes(self._ref, b, s, h, table_width, int(accumulate)))
+        with torch.cuda.device(self.device):  # partials are counted by the compute units of the cache's device
+            return int(N.lib().wz_paged_attn_workspace_bytes(self._ref, b, s, h, table_width, int(accumulate)))
 
     def evict(self, table, lens, keep, first=0, recent=0, out=None, workspace=None):
         """Cuts every sequence of a tracked cache to ``keep`` slots, in place and for each KV head by itself: the
