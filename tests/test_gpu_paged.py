@@ -800,3 +800,85 @@ def test_refusals_with_device_tensors(gpu):
         plain.attend(q, tab, n, 0.1, accumulate=True)
     for name, x in arrays(cache).items():
         assert np.array_equal(x, want[name], equal_nan=name == "weights"), name
+
+
+@pytest.mark.parametrize("HK,D,shared", [(2, 64, False), (1, 128, False), (1, 512, True)])
+def test_write_of_rows_that_are_not_finite(gpu, HK, D, shared):
+    """An e4m3 row follows act_quant's arithmetic: with an infinity its scale is inf and the infinity's code NaN,
+    with a NaN all of it is NaN, a row of tiny values has the floor's scale; other rows are not touched by it."""
+    cache = PagedKV.empty(4, 16, HK, D, dtype=E4M3, shared=shared, track=True, device=gpu)
+    x = torch.randn(1, 9, HK, D, generator=torch.Generator().manual_seed(D)).to(torch.bfloat16)
+    inf, nan = float("inf"), float("nan")
+    x[0, 1, 0, D - 1], x[0, 3, 0, 0], x[0, 4, HK - 1, 9] = inf, -inf, nan
+    x[0, 5, 0, 3], x[0, 5, 0, 4] = inf, nan
+    x[0, 6] = 3.3e38
+    x[0, 7] *= 1e-38
+    x[0, 8] = 0
+    one = lambda n: torch.tensor([n], dtype=torch.int32, device=gpu)  # noqa: E731
+    cache.write(x.to(gpu), None if shared else x.to(gpu), one(3)[None], one(2))
+    code, s = quantise(x)
+    for pool, scale in ((cache.k, cache.k_scale),) + (() if shared else ((cache.v, cache.v_scale),)):
+        got, want = pool[3, :, 2:11].cpu().float(), code[0].transpose(0, 1).float()
+        assert torch.equal(scale[3, :, 2:11].cpu().nan_to_num(-1), s[0].t().nan_to_num(-1))
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+        assert torch.isnan(got).any(-1).sum(0).tolist() == [0, 1, 0, 1, 1, 1, 0, 0, 0]
+        assert not pool[:3].view(torch.uint8).any() and not pool[3, :, :2].view(torch.uint8).any()
+
+
+def test_calls_with_workspace_and_out_allocate_nothing(gpu):
+    """Contiguous int32 tables and lengths, aligned rows, out and workspace given: no device memory is asked for."""
+    B, HK, H, D, page = 3, 2, 8, 128, 16
+    cache = PagedKV.empty(3 * 600, page, HK, D, track=True, device=gpu)
+    for width in (20, 600):  # eviction by one workgroup a unit, and by several
+        table = torch.arange(B * width, dtype=torch.int32, device=gpu).view(B, width)
+        lens = torch.tensor([100, 250, 9], dtype=torch.int32, device=gpu)
+        rows = torch.randn(B, 2, (H + 2 * HK) * D, device=gpu).to(torch.bfloat16)
+        q, k, v = (t.unflatten(-1, (-1, D)) for t in rows.split([H * D, HK * D, HK * D], -1))
+        o, new, sink = torch.empty(B, 2, H, D, dtype=torch.bfloat16, device=gpu), torch.empty_like(lens), torch.zeros(H, device=gpu)
+        ws = torch.empty(max(cache.attend_workspace_bytes(B, 2, H, width, True), cache.evict_workspace_bytes(B, width, 64)),
+                         dtype=torch.uint8, device=gpu)
+
+        def calls():
+            cache.write(k, v, table, lens, position=lens)
+            cache.attend(q, table, lens, 0.1, sink, accumulate=True, out=o, workspace=ws)
+            cache.attend(q, table, lens, 0.1, out=o, workspace=ws)
+            cache.evict(table, lens, 64, 2, 8, out=new, workspace=ws)
+
+        calls()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_stats(gpu)["allocation.all.allocated"]
+        calls()
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_stats(gpu)["allocation.all.allocated"] == before
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("HK,g,D,shared", [(2, 4, 64, False), (1, 16, 512, True)])
+def test_a_wide_table_changes_nothing(gpu, HK, g, D, shared, dtype):
+    """The loop of write, attend and evict with a table far wider than its sequences (the cut then goes by
+    chunks, the workspaces grow): bit for bit that of a narrow table."""
+    B, page, keep, steps = 3, 16, 80, 12
+    narrow = PagedKV.empty(B * 8, page, HK, D, dtype=dtype, shared=shared, track=True, device=gpu)
+    wide = PagedKV.empty(B * 8, page, HK, D, dtype=dtype, shared=shared, track=True, device=gpu)
+    tables = [torch.arange(B * 8, dtype=torch.int32, device=gpu).view(B, 8).flip(1).contiguous()]
+    tables.append(torch.cat([tables[0], torch.full((B, 700), -1, dtype=torch.int32, device=gpu)], 1))
+    n = [torch.zeros(B, dtype=torch.int32, device=gpu) for _ in range(2)]
+    pos = torch.zeros(B, dtype=torch.int32, device=gpu)
+    gen = torch.Generator(device=gpu).manual_seed(D)
+    for step in range(steps):
+        s = 70 if step == 0 else 2
+        k = torch.randn(B, s, HK, D, device=gpu, generator=gen).to(torch.bfloat16)
+        q = torch.randn(B, min(s, 2), HK * g, D, device=gpu, generator=gen).to(torch.bfloat16)
+        count = torch.tensor([s, s // 2, s], dtype=torch.int32, device=gpu)
+        out = []
+        for i, (c, t) in enumerate(zip((narrow, wide), tables)):
+            c.write(k, None if shared else k.flip(3).contiguous(), t, n[i], count=count, position=pos)
+            n[i] = n[i] + count
+            out.append(c.attend(q, t, n[i], D ** -0.5, accumulate=True))
+            n[i] = c.evict(t, n[i], keep, first=2, recent=10)
+        pos = pos + count
+        assert torch.equal(*out) and torch.equal(*n)
+        for name, x in arrays(narrow).items():
+            assert np.array_equal(x, arrays(wide)[name], equal_nan=name == "weights"), (step, name)
+    assert n[0].tolist() == [keep, 46, keep] and pos.tolist() == [92, 46, 92]
