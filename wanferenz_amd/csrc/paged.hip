@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedView c, WriteArgs
     const int start = a.start[b];
     const int32_t* const trow = a.table + int64_t(b) * a.width;
     const uint16_t* const src = a.src[side] + b * a.sb[side] + i0 * a.ss[side];
-    const uint32_t pieces = uint32_t(tokens) * per;  // up to 16 x 1024 x 64
+    const uint32_t pieces = uint32_t(tokens) * per;  // 512 at most, or one token's 1024 x 64
     for (uint32_t p0 = 0; p0 < pieces; p0 += 256 * N) {
       v4i x[N];
       int64_t at[N];
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedView c, WriteArgs
 // ---- evict ----
 
 constexpr int kEvictBins = 2048;         // keys are taken 11, 11 and 10 bits at a time
-constexpr int kEvictSmall = 8192;        // slots that one workgroup holds
+constexpr int kEvictSmall = 8192;        // slots of a table that one workgroup a unit goes through
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictChunk = 1024;        // slots of a workgroup where several share a unit
 constexpr int kEvictChunkThreads = 256;
@@ -206,8 +206,8 @@ __device__ __forceinline__ int wave_sum(int x) {
 
 // Counts a wave's keys (the lanes with `in`) in their bins, in a word's upper half where `high`.  The lanes
 // that share the first one's bin add up first: equal weights, as a prompt's zeros are, would meet in one
-// word of LDS, an addition after the other (32 units of 8000 zeros 27.6 us, so 16.6; random weights 16.8 and
-// 16.4, of 4160 slots 14.3 and 15.0).
+// word of LDS, an addition after the other (32 units of 8000 zeros 33.6 us, so 18.9, 128 of 4160 23.6 and 16.3;
+// of random weights 16.2 to 17.2 and 18.2, 13.8 and 14.3).
 __device__ __forceinline__ void evict_add(uint32_t* hist, int bin, bool in, bool high) {
   const uint64_t some = __ballot(in);
   if (!some) return;
@@ -324,13 +324,14 @@ __device__ __forceinline__ int evict_list(const EvictArgs& a, const uint32_t (&k
   return pairs;
 }
 
-// A unit (sequence, head) of up to kEvictSmall slots: the keep-th largest key by three digits, then the
+// A unit (sequence, head) of a table of up to kEvictSmall slots (the lengths are on the device, so the table's
+// width decides, whatever a sequence holds): the keep-th largest key by three digits, then the
 // holes below keep and the kept slots from keep on, in slot order.  Every wave has a range of
 // consecutive slots, 64 a round with the keys in registers, so the ranks need one exchange between the
 // waves.  MOVE: few pairs are moved here, which saves the second launch.  Its chain of dependent steps
-// bounds it: 128 units of 4160 slots cut to 4096 take 15.8 us, 13.7 and a move of 6.5 without MOVE, and 35 as chunks;
-// without the rounds past a unit's own 14.4.  16 rounds a thread, for 16384 slots, cost the short ones more than the long
-// ones gain: 4160 slots 18.8 us against 13.8, 12000 23.5 against 24 as chunks.
+// bounds it: 128 units of 4160 slots cut to 4096 take 14.2 to 14.9 us, 12.9 and a move of 5.2 without MOVE, and 32 to 36
+// and a move of 6 as chunks.  16 rounds a thread, for 16384 slots, cost the short ones more than the long ones gain: 4160
+// slots 19.3 to 20.4 us, 12000 slots of 32 units 25.8 against 28 to 31 as chunks.
 template <bool MOVE>
 __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictArgs a, int row_bytes) {
   constexpr int R = kEvictSmall / kEvictThreads, NW = kEvictThreads / 64;
@@ -422,9 +423,10 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_small_kernel(EvictA
   }
 }
 
-// The same for longer units, which one compute unit's instruction rate would bound (32767 slots of 16
-// units took it 87 us, 65535 of one 160): a workgroup per chunk of kEvictChunk slots, a launch for
-// each time that the workgroups have to meet.  Every launch costs its 4 us whatever it does, so a chunk
+// The same for units of wider tables, which one compute unit's instruction rate would bound (32767 slots of 16
+// units took it 87 us, 65535 of one 160): a workgroup per chunk of kEvictChunk slots of the table, a launch for
+// each time that the workgroups have to meet.  Chunks past a sequence's length end at once, but they are launched
+// five times: the 128 units of 4160 slots take 76 us and a move of 9.6 in a table of 131072 slots.  Every launch costs its 4 us whatever it does, so a chunk
 // is what one workgroup of four waves does in that time: 26 us in all for both sizes with 1024 slots,
 // 48 with 4096.  STEP 0: the chunk's newest position and places, and the unit's
 // histograms cleared.  1: keys and the first digit's histogram.  2, 3: the second's and third's, the

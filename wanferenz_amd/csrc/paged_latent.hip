@@ -12,7 +12,7 @@
 //     with the m of the tiles before and flags a row that needs a new one; only then a second barrier
 //     follows, after the maxima have met, O is rescaled and P written again;
 //   * O^T[512, rows] += V^T P^T: wave w has columns 64 w .. +64 of every row.
-// 4 x 65536 latents (269 MB, 34 GF) take 68 to 75 us by card, 3.6 to 4 TB/s, and the join of the 131 KB partials 8.  A
+// 4 x 65536 latents (269 MB, 34 GF) take 68 to 81 us by card, 3.3 to 4 TB/s, and the join of the 131 KB partials 8.  A
 // copy without the products takes 56 and one without the loads 58: a tile's chain from K to O is 3.6 us long, of which
 // the matrix instructions are a fifth and LDS reads (K twice, V, Q's last chunks and P, 260 KB) a quarter, and one
 // tile is in flight behind it.  With 16 heads 16 x 16000 latents (262 MB) take 52, 5.1 TB/s.

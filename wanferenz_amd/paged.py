@@ -16,8 +16,9 @@ A decode loop::
     o = cache.attend(q, table, lens + 1, scale, accumulate=True)
     lens = cache.evict(table, lens + 1, keep=4096, first=4, recent=1024)
 
-Every call runs on the current stream of the cache's device, allocates only its outputs and
-(unless given) its workspace, never synchronises, and can be captured in a graph.  The operators
+Every call runs on the current stream of the cache's device, allocates only its outputs, (unless
+given) its workspace and copies of tables and lengths that are not contiguous and of rows that are not
+16-byte aligned, never synchronises, and can be captured in a graph.  The operators
 are for serving: they have no gradients.
 """
 
