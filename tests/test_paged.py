@@ -225,6 +225,15 @@ def test_evict_sizes_that_do_not_fit_64_bits_are_refused():
     assert L.wz_paged_evict_workspace_bytes(None, 1, 3, 8) == 0
 
 
+def test_evict_is_sized_before_its_pools_exist():
+    """The workspace goes by the shape: pointers that are not there yet change nothing."""
+    L = N.lib()
+    for width in (3, 1000):
+        full, bare = cache(**TRACK), cache(k=None, v=None)
+        need = L.wz_paged_evict_workspace_bytes(ctypes.byref(full), 2, width, 8)
+        assert need > 0 and L.wz_paged_evict_workspace_bytes(ctypes.byref(bare), 2, width, 8) == need
+
+
 def test_partials_of_odd_rows_lie_on_16_bytes():
     """A worker has two partials of m and l (rounded up to 16 bytes together) and O [rows, 64], and one record
     of 16 bytes; the number of workers is the same for 1, 2 and 3 rows a KV head."""

@@ -711,9 +711,10 @@ extern "C" int wz_paged_kv_write(const wz_paged_kv* cache, const void* k_bf16, c
 extern "C" int64_t wz_paged_evict_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t table_width,
                                                   int64_t keep) {
   using namespace wz;
-  PagedView view;
-  if (paged_view("paged_evict", cache, table_width, &view) != WZ_OK) return 0;
-  if (B <= 0 || B > kEvictUnits / view.heads || keep < 0 || keep > 0x7FFFFFFFLL) return 0;
+  // the shape alone: a caller may ask before its pools exist
+  if (!cache || cache->page_size <= 0 || cache->kv_heads <= 0 || cache->kv_heads > 1024) return 0;
+  if (table_width < 0 || table_width > (int64_t(1) << 30) / cache->page_size) return 0;
+  if (B <= 0 || B > kEvictUnits / cache->kv_heads || keep < 0 || keep > 0x7FFFFFFFLL) return 0;
   return evict_sizes(cache, B, table_width, keep).total;
 }
 
