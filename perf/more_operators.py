@@ -12,7 +12,7 @@ Kinds of case:
   append  q, k and v, views of a fused projection's rows: q and k normed for each head and rotated, k and v
           written into their pages (bf16 or e4m3)
   tree    q [B, S, H, D], the S drafted tokens of a tree, against the cached prefix and their own ancestors
-  sample  one token a row of logits by temperature, top-k, top-p and min-p from a given uniform number
+  sample  one token a row of logits by temperature, min-p, top-k and top-p from a given uniform number
   accept  the walk down the tree along the sampled tokens, and its rows moved to the prefix's end
 """
 
@@ -363,10 +363,9 @@ def _plain_sample(st):
     z = order.values.double()
     w = torch.exp((z - z[:, :1]) / torch.where(t == 0, 1.0, t))
     place = torch.arange(V, device=x.device)
-    w = torch.where(((k <= 0) | (place < k)) & ((t != 0) | (place == 0)), w, 0.0)
+    w = torch.where((w >= m) & ((k <= 0) | (place < k)) & ((t != 0) | (place == 0)), w, 0.0)
     total = torch.cumsum(w, 1)
-    before = total - w
-    w = torch.where(((place == 0) | (p >= 1.0) | (before < p * total[:, -1:])) & (w >= m), w, 0.0)
+    w = torch.where((place == 0) | (p >= 1.0) | (total - w < p * total[:, -1:]), w, 0.0)
     total = torch.cumsum(w, 1)
     at = (total <= st["u"].double()[:, None] * total[:, -1:]).sum(1, keepdim=True)
     at = torch.minimum(at, (w > 0).sum(1, keepdim=True) - 1)
@@ -560,9 +559,9 @@ def _exact_sample(st):
         w = np.exp((row[order] - row[order[0]]) / t[r])
         keep = len(w) if k[r] <= 0 else min(len(w), int(k[r]))
         w = w[:keep]
+        w = w[w >= m[r]]
         if p[r] < 1.0:
             w = w[:max(1, int(np.searchsorted(np.cumsum(w), p[r] * np.cumsum(w)[-1], side="left")) + 1)]
-        w = w[w >= m[r]]
         acc = np.cumsum(w)
         at = min(int(np.searchsorted(acc, u[r] * acc[-1], side="right")), len(w) - 1)
         token[r], prob[r] = order[at], w[at] / acc[-1]
