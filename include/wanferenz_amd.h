@@ -416,6 +416,49 @@ int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q
                   int64_t H, float softmax_scale, int accumulate, void* workspace, int64_t workspace_bytes,
                   hipStream_t stream);
 
+/* New tokens of a projection on their way into the cache: every head's row of q and k becomes
+ * x / sqrt(mean(x^2) + eps) * norm (float32 [head_dim]; NULL: as it is), then its dims
+ * [offset, offset + rotary) are turned by the token's position, pairs (a, b) to
+ * (a c - b s, a s + b c) with (c, s) = freqs[position][pair] (float32 [turns, rotary / 2, 2],
+ * cos and sin: torch.view_as_real of freqs_cis; a position outside [0, turns) turns by
+ * NaN).  A pair is dims 2 i and 2 i + 1 of the rotary part (the reference's rotation,
+ * architecture.py:611-672), or with `halves` i and i + rotary / 2.  All of it in
+ * 32 bits, rounded once.  q goes to q_out [B, S, H, head_dim] bf16 (dense; q itself where q is
+ * dense, else over no input), k and v into their pages as wz_paged_kv_write puts them
+ * (an e4m3 row is quantised from the 32-bit values), v as it is.  position: [B], the first
+ * token's (token i has position[b] + i), or with position_each [B, S], every token's; NULL:
+ * the slots.  A tracked slot gets its token's position.  For i >= count[b] q_out is 0 and
+ * nothing is written.  rotary and offset are multiples of 16 (rotary 0: no rotation);
+ * norms, freqs and rows 16-byte aligned. */
+int wz_paged_append(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q_strides, const void* k_bf16,
+                    const int64_t* k_strides, const void* v_bf16, const int64_t* v_strides, void* q_out_bf16, int64_t H,
+                    const float* q_norm, const float* k_norm, float eps, const float* freqs, int64_t turns,
+                    int64_t rotary, int halves, int64_t offset, const int32_t* table, int64_t table_width,
+                    const int32_t* start, const int32_t* count, const int32_t* position, int position_each, int64_t B,
+                    int64_t S, hipStream_t stream);
+
+/* Attention of a tree of S drafted tokens a sequence (1..64, already written) over the cached
+ * tokens: node i of sequence b is slot lens[b] - count[b] + i (count NULL: S), and sees the slots
+ * before the tree, itself, and the nodes above it: parent [B, S] holds each node's
+ * parent, in any order; a parent outside [0, count[b]) is none, so the node hangs on the
+ * prefix.  Nodes i >= count[b] get 0.  The rest is wz_paged_attn's. */
+int64_t wz_paged_tree_attn_workspace_bytes(const wz_paged_kv* cache, int64_t B, int64_t S, int64_t H,
+                                           int64_t table_width);
+int wz_paged_tree_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q_strides, const float* attn_sink,
+                       const int32_t* table, int64_t table_width, const int32_t* lens, const int32_t* parent,
+                       const int32_t* count, void* o_bf16, int64_t B, int64_t S, int64_t H, float softmax_scale,
+                       void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* The accepted path of a verified tree, S nodes a sequence (0..64), node i in slot start[b] + i: node 0
+ * is accepted, and from an accepted node on its lowest child behind it (parent[b][c] = node, c > node,
+ * c < count[b]; count NULL: S) with drafted[b][c] = sampled[b][node].  The m accepted nodes' rows
+ * (scales, weights, positions) move in order to the slots from start[b] on; a row without a page at either
+ * end stays.  lens[b] = start[b] + m; path [B, S] the accepted nodes, tokens [B, S] what was sampled
+ * at them (the last one is the next tree's root), both -1 from m on.  Outputs overlap no input. */
+int wz_paged_accept(const wz_paged_kv* cache, const int32_t* drafted, const int32_t* parent, const int32_t* sampled,
+                    const int32_t* table, int64_t table_width, const int32_t* start, const int32_t* count,
+                    int32_t* lens, int32_t* tokens, int32_t* path, int64_t B, int64_t S, hipStream_t stream);
+
 /* Cuts every sequence of a tracked cache to `keep` slots, in place: for each KV head the
  * slots with positions below `first`, the `recent` newest positions and then those of the
  * highest weight stay (NaN counts as the lowest, equal weights go by the lower slot);
@@ -427,6 +470,20 @@ int64_t wz_paged_evict_workspace_bytes(const wz_paged_kv* cache, int64_t B, int6
 int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, int64_t table_width, const int32_t* lens,
                    int32_t* new_lens, int64_t B, int64_t keep, int64_t first, int64_t recent, void* workspace,
                    int64_t workspace_bytes, hipStream_t stream);
+
+/* One token for each of n rows of V logits (float32, or bf16 with logits_bf16; rows row_stride
+ * elements apart), from uniform[row] in [0, 1).  A row's tokens stand in order of their logits, the highest first,
+ * equal ones by index; w = exp((logit - highest) / temperature).  Kept are those with w >= min_p, of them
+ * the top_k first (0 or less: all), and of those the fewest first ones whose w add up to top_p of all (1 or more:
+ * all; one at least).  The token is the first one in order whose cumulated w exceeds uniform times the kept sum;
+ * probs[row] = w over that sum.  temperature <= 0 takes the first token, probability 1.  NaN and -inf are never
+ * taken (a row of nothing else: token -1, probability 0), +inf takes all the weight.  A
+ * weight below 2^-42 of the row's largest counts as nothing.  temperature, top_k, top_p and
+ * min_p are device arrays [n], or NULL for the value beside them. */
+int wz_sample(const void* logits, int logits_bf16, int64_t row_stride, const float* uniform, const float* temperature,
+              float temperature_all, const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+              const float* min_p, float min_p_all, int32_t* tokens, float* probs, int64_t n, int64_t V,
+              hipStream_t stream);
 
 /* The FP8 wire format of a pipeline-stage boundary — _pack_t / _unpack_t
  * (serving/chain.py:208-222): per row scale = bf16(clamp(amax/448, 1e-8, bf16 max)),

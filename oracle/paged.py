@@ -93,3 +93,71 @@ def evict(cache, table, lens, keep, first=0, recent=0):
                 for (tp, tr), (fp, fr) in moved:
                     x[tp, h, tr] = x[fp, h, fr]
     return np.array(out, dtype=np.int32)
+
+
+def tree_sight(parent, nodes):
+    """Row i: the set of nodes that node i of a tree sees, itself and those above it."""
+    out = []
+    for i in range(nodes):
+        seen, at = set(), i
+        while 0 <= at < nodes and at not in seen:
+            seen.add(at)
+            at = int(parent[at])
+        out.append(seen)
+    return out
+
+
+def attend_tree(cache, q, table, lens, parent, scale, sink=None, count=None):
+    """attend for trees of drafted tokens -> (o, abs, None, reach), as attend's."""
+    k, v = cache["k"], cache.get("v", cache["k"])
+    P, HK, page, D = k.shape
+    B, S, H, _ = q.shape
+    o, mag, reach = np.zeros((B, S, H, D)), np.zeros((B, S, H, D)), 0.0
+    for b in range(B):
+        n = int(min(max(int(lens[b]), 0), table.shape[1] * page))
+        nodes = S if count is None else min(max(int(count[b]), 0), S)
+        at = slot_places(table[b], P, page, range(n))
+        for i, sight in enumerate(tree_sight(parent[b], nodes)):
+            seen = [x for t, x in enumerate(at) if x[0] >= 0 and (t < n - nodes or t - (n - nodes) in sight)]
+            if not seen:
+                continue
+            pid, row = np.array([x[0] for x in seen]), np.array([x[1] for x in seen])
+            for h in range(H):
+                kk, vv = k[pid, h // (H // HK), row], v[pid, h // (H // HK), row]
+                with np.errstate(all="ignore"):
+                    s = (kk @ q[b, i, h]) * scale
+                    reach = max(reach, float(np.nanmax(np.abs(kk) @ np.abs(q[b, i, h]) * scale)))
+                    m = max(float(s.max()), -np.inf if sink is None else float(sink[h]))
+                    if m == -np.inf:
+                        continue
+                    e = np.exp(s - m)
+                    p = e / (e.sum() + (0.0 if sink is None else np.exp(float(sink[h]) - m)))
+                    o[b, i, h], mag[b, i, h] = p @ vv, p @ np.abs(vv)
+    return o, mag, None, reach
+
+
+def turned(x, norm, eps, turns, halves, leading):
+    """Rows x [.., D] float64, normed by `norm` (None: as they are) and rotated by `turns` [.., R / 2] complex."""
+    x = np.array(x, dtype=np.float64)
+    if norm is not None:
+        x = x / np.sqrt(np.mean(x * x, axis=-1, keepdims=True) + eps) * norm
+    R, D = 2 * turns.shape[-1], x.shape[-1]
+    lo = 0 if leading else D - R
+    pair = np.arange(R // 2)
+    i = lo + (pair if halves else 2 * pair)
+    j = i + (R // 2 if halves else 1)
+    z = (x[..., i] + 1j * x[..., j]) * turns
+    x[..., i], x[..., j] = z.real, z.imag
+    return x
+
+
+def accept(drafted, parent, sampled, nodes):
+    """One tree's accepted nodes, in order."""
+    path = [0] if nodes > 0 else []
+    while path:
+        on = [c for c in range(path[-1] + 1, nodes)
+              if parent[c] == path[-1] and drafted[c] == sampled[path[-1]]]
+        if not on:
+            break
+        path.append(on[0])
+    return path

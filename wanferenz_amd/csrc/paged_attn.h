@@ -43,6 +43,7 @@ constexpr int kPagedTile = 32;           // tokens of a wave's tile
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kPagedLazy = 8.0f;       // the running maximum moves when a tile exceeds it by more
 constexpr int kPagedMaxS = 16;
+constexpr int kPagedMaxNodes = 64;       // of a tree: a lane each, a bit each
 constexpr int kPagedStart = 3;           // a worker's start of a unit, in tiles (paged_cost)
 
 // A unit's parts: np of them (1: nothing to join, 0: no unit), of worker w and those after it.
@@ -62,6 +63,8 @@ struct PagedAttnArgs {
   PagedCut* cut;  // a unit where by_unit, else the cut unit that begins in a worker's share
   float* ml;      // accumulate: per unit and row the final maximum and 1 / sum
   float* scores;  // accumulate: y [B, heads, R, capacity]
+  const int32_t* parent;  // trees: [B, S]
+  const int32_t* count;   // trees: nodes of each sequence, or null: S
   int width, B, S, H, W, rows, unit_rows, by_unit;  // rows: of a partial, min(R, unit_rows)
   int64_t capacity;  // slots of the table, width * page
   float scale2;      // softmax scale * log2(e)
@@ -80,6 +83,32 @@ static inline int64_t paged_units(const PagedAttnArgs& a) {
 // Tokens of a sequence, and its granules.
 __device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
   return int(min(int64_t(max(a.lens[b], 0)), a.capacity));
+}
+
+// Nodes of a sequence's tree.
+__device__ __forceinline__ int paged_nodes(const PagedAttnArgs& a, int b) {
+  return a.count ? min(max(a.count[b], 0), a.S) : a.S;
+}
+
+// A tree's visibility: bit j of lane i's mask says that node i sees node j, itself or one above it.  Each of six rounds
+// doubles the steps up that a mask covers, so the order of the nodes does not matter, and a parent that is no node of the
+// tree ends the way up.
+__device__ __forceinline__ uint64_t paged_tree_masks(const PagedAttnArgs& a, int b, int nodes, int lane) {
+  uint64_t seen = lane < nodes ? 1ull << lane : 0ull;
+  int up = lane < nodes ? a.parent[int64_t(b) * a.S + lane] : -1;
+  up = uint32_t(up) < uint32_t(nodes) ? up : -1;
+  for (int i = 0; i < 6; ++i) {
+    const uint32_t lo = __shfl(uint32_t(seen), up & 63, 64), hi = __shfl(uint32_t(seen >> 32), up & 63, 64);
+    const int next = __shfl(up, up & 63, 64);
+    if (up >= 0) {
+      seen |= uint64_t(hi) << 32 | lo;
+      up = next;
+    }
+  }
+  return seen;
+}
+__device__ __forceinline__ uint64_t paged_tree_mask(uint64_t masks, int node) {
+  return uint64_t(uint32_t(__shfl(uint32_t(masks >> 32), node, 64))) << 32 | uint32_t(__shfl(uint32_t(masks), node, 64));
 }
 
 // What a unit of n tokens counts for: its granules of G, and START more for the time in which a worker
@@ -283,7 +312,8 @@ struct PagedCfg {
   static_assert(PER_CU >= 1 && SIDE / 1024 % RH == 0, "a worker fits, and its waves share a tile's loads evenly");
 };
 
-template <int D, bool FP8, bool SHARED, int RT, int RH>
+// TREE: the new tokens are the nodes of a tree, which see the prefix, themselves and the nodes above them.
+template <int D, bool FP8, bool SHARED, int RT, int RH, bool TREE>
 __global__ __launch_bounds__(64 * RH, (PagedCfg<D, FP8, SHARED, RT, RH>::EU))
 void paged_attn_kernel(PagedAttnArgs a) {
   using C = PagedCfg<D, FP8, SHARED, RT, RH>;
@@ -345,7 +375,9 @@ void paged_attn_kernel(PagedAttnArgs a) {
     const int t0 = g0 * kPagedTile, tm = min(g1 * kPagedTile, n);
     // The last S - 1 tokens, from n0 on, are seen by some rows only.  The others' p is 0 there, which keeps
     // a finite value out of them; a token whose V is not finite is added by itself after the tiles.
-    const int n0 = n - a.S + 1;
+    const int nodes = TREE ? __builtin_amdgcn_readfirstlane(paged_nodes(a, b)) : 0;
+    const int n0 = TREE ? n - nodes : n - a.S + 1;  // a tree's first token need not be above the others
+    const uint64_t masks = TREE && tm > n0 ? paged_tree_masks(a, b, nodes, lane) : 0ull;
     int odd0 = 0, odd1 = 0;  // those tokens
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
       a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
@@ -452,7 +484,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
       uint8_t* const vt = SHARED ? kt : kt + C::SIDE;
       uint32_t valid = __builtin_amdgcn_readfirstlane(s_valid[stage]);
       const int t = t0 + kPagedTile * k;
-      const bool last = a.S > 1 && t + kPagedTile > n0;
+      const bool last = (TREE || a.S > 1) && t + kPagedTile > n0;
       if (last) {
         const uint32_t some = valid & ~((1u << max(n0 - t, 0)) - 1u);  // tokens that some rows see
         bool odd = false;
@@ -530,10 +562,19 @@ void paged_attn_kernel(PagedAttnArgs a) {
             if (!((valid >> (16 * (i >> 2) + 4 * g + (i & 3))) & 1)) y[i] = -INFINITY;
         }
         if (last) {
-          const int sees = n0 + min(row0 + 16 * rt + nl, R - 1) / grp - t;  // tokens of the tile that the row sees
+          if constexpr (TREE) {
+            const uint64_t mask = paged_tree_mask(masks, min(row0 + 16 * rt + nl, R - 1) / grp);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (16 * (i >> 2) + 4 * g + (i & 3) >= sees) y[i] = -INFINITY;
+            for (int i = 0; i < 8; ++i) {
+              const int node = t + 16 * (i >> 2) + 4 * g + (i & 3) - n0;
+              if (node >= 0 && !((mask >> (node & 63)) & 1)) y[i] = -INFINITY;
+            }
+          } else {
+            const int sees = n0 + min(row0 + 16 * rt + nl, R - 1) / grp - t;  // tokens of the tile that the row sees
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (16 * (i >> 2) + 4 * g + (i & 3) >= sees) y[i] = -INFINITY;
+          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, y[i]);
@@ -624,7 +665,8 @@ void paged_attn_kernel(PagedAttnArgs a) {
           const float dot =
               paged_dot<D, FP8>(a.q + b * a.qb + (rq / grp) * a.qs + (hk * grp + rq % grp) * a.qh, kr, g);
           const int r = row0 + 16 * rt + nl;
-          const bool sees = r < R && t < n - (a.S - 1 - r / grp);
+          const uint64_t mask = TREE ? paged_tree_mask(masks, rq / grp) >> ((t - n0) & 63) : 0ull;
+          const bool sees = r < R && (TREE ? mask & 1 : t < n - (a.S - 1 - r / grp));
           const float y = FP8 ? dot * ksc * a.scale2 : dot * a.scale2;
           if (a.scores && r < R && g == 0)
             a.scores[((int64_t(b) * a.c.heads + hk) * R + r) * a.capacity + t] = y;
@@ -668,6 +710,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
             const float Me = M == -INFINITY ? 0.0f : M;
             f = m_run[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[rt] - Me);
             den = den * f + __builtin_amdgcn_exp2f(sk - Me);
+          }
+          if (TREE && s >= nodes) {  // no node's row
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) acc[rt][nt] = v4f{0.f, 0.f, 0.f, 0.f};
+            den = 0.0f;
           }
           const float inv = den == 0.0f ? 0.0f : f / den;
           uint16_t* const orow = a.o + ((int64_t(b) * a.S + s) * a.H + head) * D + 4 * g;
@@ -768,6 +815,10 @@ __device__ __forceinline__ void paged_join(const PagedAttnArgs& a, int unit, int
     }
   }
   if (a.sink) den += __builtin_amdgcn_exp2f(sk - Me);
+  if (a.parent && r / grp >= paged_nodes(a, b)) {  // no node's row
+    o = v4f{0.f, 0.f, 0.f, 0.f};
+    den = 0.0f;
+  }
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
   uint16_t* const orow = a.o + ((int64_t(b) * a.S + r / grp) * a.H + head) * D;
   *reinterpret_cast<uint2*>(orow + 4 * ch) =
@@ -911,7 +962,7 @@ int paged_attn_join(const PagedAttnArgs& a, hipStream_t stream) {
 
 // The kernel of R rows a KV head: 16, 32 or 64 rows a unit.  With 4 rows 16 x 8000 tokens take 94.5 / 97.6 / 121.7 us with
 // each, 48 x 9001 e4m3 tokens of 128 with 8 rows 167 / 214 / 400.
-template <int D, bool FP8, bool SHARED, int RT, int RH>
+template <int D, bool FP8, bool SHARED, int RT, int RH, bool TREE>
 int paged_attn_launch_rt(PagedAttnArgs a, bool ask, int* workers, hipStream_t stream) {
   using C = PagedCfg<D, FP8, SHARED, RT, RH>;
   static_assert(C::LDS <= 160 * 1024, "a workgroup's LDS");
@@ -925,37 +976,40 @@ int paged_attn_launch_rt(PagedAttnArgs a, bool ask, int* workers, hipStream_t st
   }
   a.by_unit = paged_units(a) <= a.W;
   static LdsGrant grant;
-  auto* const kernel = paged_attn_kernel<D, FP8, SHARED, RT, RH>;
+  auto* const kernel = paged_attn_kernel<D, FP8, SHARED, RT, RH, TREE>;
   if (int rc = allow_lds("paged_attn", kernel, C::LDS, grant)) return rc;
   WZ_LAUNCH("paged_attn", stream, kernel, dim3{unsigned(a.W)}, dim3(64 * RH), C::LDS, a);
   if (int rc = check_launch("paged_attn")) return rc;
   return paged_attn_join<D>(a, stream);
 }
 
-template <int D, bool FP8, bool SHARED>
+template <int D, bool FP8, bool SHARED, bool TREE>
 int paged_attn_launch_d(const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
   const int R = a.S * (a.H / a.c.heads);
-  if (R <= 16) return paged_attn_launch_rt<D, FP8, SHARED, 1, 1>(a, ask, workers, stream);
-  if (R <= 32) return paged_attn_launch_rt<D, FP8, SHARED, 2, 1>(a, ask, workers, stream);
-  return paged_attn_launch_rt<D, FP8, SHARED, 2, 2>(a, ask, workers, stream);
+  if (R <= 16) return paged_attn_launch_rt<D, FP8, SHARED, 1, 1, TREE>(a, ask, workers, stream);
+  if (R <= 32) return paged_attn_launch_rt<D, FP8, SHARED, 2, 1, TREE>(a, ask, workers, stream);
+  return paged_attn_launch_rt<D, FP8, SHARED, 2, 2, TREE>(a, ask, workers, stream);
 }
 
 int paged_latent(bool fp8, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
 
 // Launches, or with `ask` -> the rows of a partial, and *workers.
-template <bool FP8>
+template <bool FP8, bool TREE>
 int paged_attn_launch(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
   if (a.c.shared) {
-    if (D == 128) return paged_attn_launch_d<128, FP8, true>(a, ask, workers, stream);
-    if (D == 256) return paged_attn_launch_d<256, FP8, true>(a, ask, workers, stream);
+    if (D == 128) return paged_attn_launch_d<128, FP8, true, TREE>(a, ask, workers, stream);
+    if (D == 256) return paged_attn_launch_d<256, FP8, true, TREE>(a, ask, workers, stream);
     return paged_latent(FP8, a, ask, workers, stream);
   }
-  if (D == 64) return paged_attn_launch_d<64, FP8, false>(a, ask, workers, stream);
-  if (D == 128) return paged_attn_launch_d<128, FP8, false>(a, ask, workers, stream);
-  return paged_attn_launch_d<256, FP8, false>(a, ask, workers, stream);
+  if (D == 64) return paged_attn_launch_d<64, FP8, false, TREE>(a, ask, workers, stream);
+  if (D == 128) return paged_attn_launch_d<128, FP8, false, TREE>(a, ask, workers, stream);
+  return paged_attn_launch_d<256, FP8, false, TREE>(a, ask, workers, stream);
 }
 
+// The kernels are compiled by four sources: for one to 16 new tokens in a row and for trees, of bf16 and of e4m3 rows.
 int paged_attn_bf16(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
 int paged_attn_e4m3(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
+int paged_tree_bf16(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
+int paged_tree_e4m3(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream);
 
 }  // namespace wz

@@ -3,6 +3,6 @@
 
 namespace wz {
 int paged_attn_e4m3(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
-  return paged_attn_launch<true>(D, a, ask, workers, stream);
+  return paged_attn_launch<true, false>(D, a, ask, workers, stream);
 }
 }  // namespace wz

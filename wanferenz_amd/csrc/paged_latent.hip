@@ -35,7 +35,7 @@ struct LatentCfg {
 
 // EXTRA: several new tokens, or weights to accumulate; without their code 64 rows just fit the registers (4 x 65536
 // latents 73.4 us, with it 76.9).
-template <bool FP8, int HT, bool EXTRA>
+template <bool FP8, int HT, bool EXTRA, bool TREE>
 __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(PagedAttnArgs a) {
   using C = LatentCfg<FP8>;
   using L = PagedRow<C::RB>;
@@ -102,7 +102,10 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
     const bool whole = g0 == 0 && g1 == cost - kLatentStart;
     const int hk = u / RG, rg = u - hk * RG, row0 = rg * ROWS;
     const int t0 = g0 * T, tm = min(g1 * T, n);
-    const int n0 = n - a.S + 1;  // from here on a token is seen by some rows only, as in paged_attn_kernel
+    // from n0 on a token is seen by some rows only, as in paged_attn_kernel
+    const int nodes = TREE ? __builtin_amdgcn_readfirstlane(paged_nodes(a, b)) : 0;
+    const int n0 = TREE ? n - nodes : n - a.S + 1;
+    const uint64_t masks = TREE && tm > n0 ? paged_tree_masks(a, b, nodes, lane) : 0ull;
     int odd0 = 0, odd1 = 0;
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
       a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       uint8_t* const ks = kb[buf];
       uint64_t valid = uint64_t(paged_uniform(*reinterpret_cast<const int64_t*>(s_valid[buf])));
       const int tk = t0 + T * k;
-      const bool last = EXTRA && a.S > 1 && tk + T > n0;
+      const bool last = EXTRA && (TREE || a.S > 1) && tk + T > n0;
       if (last) {
         const uint64_t some = valid & ~((1ull << max(n0 - tk, 0)) - 1ull);  // tokens that some rows see
         bool odd = false;  // every wave looks at all of them, and comes to the same
@@ -288,10 +291,20 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
             y[h][i] = (valid >> (16 * rt + 4 * g + i)) & 1 ? s : -INFINITY;
           }
           if (last) {
-            const int sees = n0 + min(row0 + 16 * (ht0 + h) + nl, R - 1) / grp - tk;  // tokens that the row sees
+            const int s = min(row0 + 16 * (ht0 + h) + nl, R - 1) / grp;
+            if constexpr (TREE) {
+              const uint64_t mask = paged_tree_mask(masks, s);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (16 * rt + 4 * g + i >= sees) y[h][i] = -INFINITY;
+              for (int i = 0; i < 4; ++i) {
+                const int node = tk + 16 * rt + 4 * g + i - n0;
+                if (node >= 0 && !((mask >> (node & 63)) & 1)) y[h][i] = -INFINITY;
+              }
+            } else {
+              const int sees = n0 + s - tk;  // tokens that the row sees
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (16 * rt + 4 * g + i >= sees) y[h][i] = -INFINITY;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = fmaxf(top, y[h][i]);
@@ -425,7 +438,8 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       }
       meet();
       const int r = row0 + lane;
-      const bool sees = lane < ROWS && r < R && t < n - (a.S - 1 - r / grp);
+      const uint64_t mask = TREE ? paged_tree_mask(masks, min(r, R - 1) / grp) >> ((t - n0) & 63) : 0ull;
+      const bool sees = lane < ROWS && r < R && (TREE ? mask & 1 : t < n - (a.S - 1 - r / grp));
       const float yy = s_y[lane < ROWS ? lane : 0];
       const float m_new = sees ? fmaxf(m_run, yy) : m_run, m = m_new == -INFINITY ? 0.0f : m_new;
       const float resc = !sees ? 1.0f : m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m);
@@ -470,7 +484,8 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
         f = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - Me);
         den = den * f + __builtin_amdgcn_exp2f(sk - Me);
       }
-      const float inv = den == 0.0f ? 0.0f : f / den;
+      const bool dead = TREE && rr / grp >= nodes;  // no node's row
+      const float inv = den == 0.0f || dead ? 0.0f : f / den;
       if (a.ml && wave == 0 && lane < ROWS && row0 + lane < R) {
         float* const e = a.ml + 2 * ((int64_t(b) * a.c.heads + hk) * R + row0 + lane);
         e[0] = M == -INFINITY ? 0.0f : M;
@@ -481,6 +496,10 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
         const float iv = __shfl(inv, 16 * ht + nl, 64);
         const int r = row0 + 16 * ht + nl;
         if (r >= R) continue;
+        if (TREE && r / grp >= nodes) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[ht][nt] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
         uint16_t* const orow =
             a.o + ((int64_t(b) * a.S + r / grp) * a.H + hk * grp + r % grp) * D + 16 * NT * wave + 4 * g;
 #pragma unroll
@@ -519,10 +538,12 @@ static int latent_launch(PagedAttnArgs a, bool ask, int* workers, hipStream_t st
     return a.rows;
   }
   a.by_unit = paged_units(a) <= a.W;
-  if (a.S > 1 || a.scores)
-    WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, true>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
+  if (a.parent)
+    WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, true, true>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
+  else if (a.S > 1 || a.scores)
+    WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, true, false>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
   else
-    WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, false>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
+    WZ_LAUNCH("paged_attn", stream, (paged_latent_kernel<FP8, HT, false, false>), dim3{unsigned(a.W)}, dim3(64 * kLatentWaves), 0, a);
   if (int rc = check_launch("paged_attn")) return rc;
   return paged_attn_join<kLatentD>(a, stream);
 }

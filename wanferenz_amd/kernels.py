@@ -575,6 +575,57 @@ def sparse_attn_workspace_bytes(b, s, h, d, topk) -> int:
     return int(N.lib().wz_sparse_attn_workspace_bytes(b, s, h, d, topk))
 
 
+def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """One token a row: logits [n, V] float32 or bf16 (rows dense, any stride between them), ``uniform`` [n] float32 in
+    [0, 1), one random number a row -> (tokens int32 [n], probs float32 [n]), in ``out`` if given.
+
+    A row's tokens stand in order of their logits, the highest first, equal ones by index, and w = exp((logit -
+    highest) / temperature).  Kept are those with w >= ``min_p``, of them the ``top_k`` first (0: all), and of those the
+    fewest first ones whose w add up to ``top_p`` of all.  The token is the first in order whose cumulated w exceeds
+    ``uniform`` times the kept sum, so a smaller number gives a likelier token; its probability is its w over that
+    sum.  Temperature 0 takes the first token.  NaN and -inf are never taken: a row of nothing else gives token -1,
+    probability 0.  A weight below 2^-42 of the row's largest counts as nothing.
+
+    Each of the four is one number for all rows, or a tensor [n] on the logits' device (float32, ``top_k`` int32; not read
+    by the host).  The reference's tail takes the highest logit (temperature 0)."""
+    what = "sample"
+    _require_cuda(logits, uniform)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"{what}: logits must be [n, V], got {list(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{what}: float32 or bf16 logits expected (got {logits.dtype})")
+    n, V = logits.shape
+    dev = logits.device
+
+    def rows(name, t, dtype):
+        if t.shape != (n,) or t.dtype != dtype or t.device != dev:
+            raise ValueError(f"{what}: {name} must be {dtype} [{n}] on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+        return t if t.is_contiguous() else t.contiguous()
+
+    uniform = rows("uniform", uniform, torch.float32)
+    args = []
+    for name, x, dtype, most in (("temperature", temperature, torch.float32, None), ("top_k", top_k, torch.int32, None),
+                                 ("top_p", top_p, torch.float32, 1), ("min_p", min_p, torch.float32, 1)):
+        if isinstance(x, torch.Tensor):
+            x = rows(name, x, dtype)
+            args += [x, 0]
+            continue
+        if not x >= 0 or (most is not None and x > most):
+            raise ValueError(f"{what}: {name} = {x} (0 or more{'' if most is None else ', 1 or less'})")
+        args += [None, min(int(x), 2**31 - 1) if dtype == torch.int32 else float(x)]
+    if logits.stride(1) != 1 or (n > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+    elif rows("out[0]", out[0], torch.int32) is not out[0] or rows("out[1]", out[1], torch.float32) is not out[1]:
+        raise ValueError(f"{what}: out must be contiguous")
+    with torch.cuda.device(dev):
+        N.call("wz_sample", N.ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0) if n > 1 else V,
+               N.ptr(uniform), *[N.ptr(x) if i % 2 == 0 else x for i, x in enumerate(args)], N.ptr(out[0]), N.ptr(out[1]),
+               n, V, N.stream_handle(dev))
+    return out
+
+
 def wire_pack(t):
     """_pack_t (serving/chain.py:208-217): bf16 [..., D] -> (e4m3 [..., D], bf16 scale [...])."""
     assert t.is_contiguous()

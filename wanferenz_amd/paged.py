@@ -94,7 +94,8 @@ class PagedKV:
         self._desc = d
         self._ref = ctypes.byref(d)
         lib = N.lib()
-        self._entry = {n: getattr(lib, n) for n in ("wz_paged_kv_write", "wz_paged_attn", "wz_paged_evict")}
+        self._entry = {n: getattr(lib, n) for n in ("wz_paged_kv_write", "wz_paged_append", "wz_paged_attn",
+                                                    "wz_paged_tree_attn", "wz_paged_accept", "wz_paged_evict")}
         self._sizes = {}
 
     @classmethod
@@ -130,6 +131,20 @@ class PagedKV:
         if t.device != self.device:
             raise ValueError(f"{what}: table is on {t.device}, the cache on {self.device}")
         return t if t.is_contiguous() else t.contiguous()
+
+    def _nodes(self, what, name, t, b, s):
+        if t.dtype != torch.int32 or t.shape != (b, s):
+            raise ValueError(f"{what}: {name} must be int32 {[b, s]}, got {t.dtype} {list(t.shape)}")
+        if t.device != self.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, the cache on {self.device}")
+        return t if t.is_contiguous() else t.contiguous()
+
+    def _out(self, what, out, shape):
+        if out is None:
+            return torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        if out.shape != shape or out.dtype != torch.bfloat16 or out.device != self.device or not out.is_contiguous():
+            raise ValueError(f"{what}: out must be contiguous bf16 {list(shape)} on {self.device}")
+        return out
 
     def _rows(self, what, name, t):
         """t as bf16 rows [.., .., .., D] that the kernels read in place: dense in their last dimension
@@ -193,6 +208,63 @@ class PagedKV:
         self._call("wz_paged_kv_write", k.data_ptr(), ks, N.ptr(v), vs, table.data_ptr(), table.shape[1],
                    start.data_ptr(), N.ptr(count), N.ptr(position), b, s)
 
+    def append(self, q, k, v, table, start, freqs_cis=None, count=None, position=None, q_norm=None, k_norm=None, eps=1e-6,
+               halves=False, leading=False, out=None):
+        """``write`` with the norms and the rotation on the way: q [b, s, h, head_dim], k and v as ``write`` takes them,
+        all views of a fused projection's rows if need be.  Each head's row of q and k is normed, x / sqrt(mean(x^2) +
+        ``eps``) * ``q_norm`` or ``k_norm`` (float32 [head_dim]; without it the row stays as it is), and turned by its
+        token's position; k and v go into their pages.  -> the turned q [b, s, h, head_dim] bf16 (``out`` if given, which
+        may be q itself where q is contiguous, and overlaps the inputs in no other way).
+
+        ``freqs_cis`` complex64 [positions, r / 2]: the reference's table (architecture.py:611-672), r a multiple of 16
+        up to head_dim; without it nothing is turned.  The r last dims of a row are turned, or the first with
+        ``leading``; a pair is two neighbouring dims, as the reference's, or with ``halves`` dims i and i + r / 2.
+        ``position``: [b], the first new token's position (its slot without it), or [b, s], every token's, as a tree's
+        depths need; a tracked slot keeps it.  A position outside the table turns by NaN.  Tokens i >= ``count[b]`` are
+        not written, their q is 0.  All of it is computed in 32 bits and rounded once."""
+        what = "PagedKV.append"
+        if q.dim() != 4 or q.shape[3] != self.head_dim:
+            raise ValueError(f"{what}: q must be [b, s, h, {self.head_dim}], got {list(q.shape)}")
+        b, s, h, d = q.shape
+        if k.shape != (b, s, self.kv_heads, d):
+            raise ValueError(f"{what}: k must be {[b, s, self.kv_heads, d]}, got {list(k.shape)}")
+        if (v is None) != (self.v is None):
+            raise ValueError(f"{what}: v is given where the cache has a v")
+        if v is not None and v.shape != k.shape:
+            raise ValueError(f"{what}: v {list(v.shape)} does not match k {list(k.shape)}")
+        table = self._table(what, table, b)
+        start = self._ints(what, "start", start, b)
+        if count is not None:
+            count = self._ints(what, "count", count, b)
+        each = position is not None and position.dim() == 2
+        if each:
+            position = self._nodes(what, "position", position, b, s)
+        elif position is not None:
+            position = self._ints(what, "position", position, b)
+        turns = rotary = 0
+        if freqs_cis is not None:
+            if freqs_cis.dtype != torch.complex64 or freqs_cis.dim() != 2 or freqs_cis.device != self.device:
+                raise ValueError(f"{what}: freqs_cis must be complex64 [positions, r / 2] on {self.device}, got "
+                                 f"{freqs_cis.dtype} {list(freqs_cis.shape)} on {freqs_cis.device}")
+            if not freqs_cis.is_contiguous():
+                raise ValueError(f"{what}: freqs_cis must be contiguous")
+            if freqs_cis.is_conj():
+                raise ValueError(f"{what}: freqs_cis is a conjugated view: resolve_conj() it once")
+            turns, rotary = freqs_cis.shape[0], 2 * freqs_cis.shape[1]
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None and (w.shape != (d,) or w.dtype != torch.float32 or w.device != self.device
+                                  or not w.is_contiguous()):
+                raise ValueError(f"{what}: {name} must be contiguous float32 [{d}] on {self.device}")
+        out = self._out(what, out, (b, s, h, d))
+        q, qs = self._rows(what, "q", q)
+        k, ks = self._rows(what, "k", k)
+        v, vs = (None, None) if v is None else self._rows(what, "v", v)
+        self._call("wz_paged_append", q.data_ptr(), qs, k.data_ptr(), ks, N.ptr(v), vs, out.data_ptr(), h, N.ptr(q_norm),
+                   N.ptr(k_norm), float(eps), N.ptr(freqs_cis), turns, rotary, int(halves),
+                   0 if leading else d - rotary, table.data_ptr(), table.shape[1], start.data_ptr(), N.ptr(count),
+                   N.ptr(position), int(each), b, s)
+        return out
+
     def attend(self, q, table, lens, softmax_scale, attn_sink=None, accumulate=False, out=None, workspace=None):
         """Attention of the s newest tokens of every sequence (1 to 16, already written) over its cached tokens:
         q [b, s, h, head_dim] bf16, ``lens`` [b] the tokens cached, the s new ones among them.  Query i of a
@@ -232,6 +304,73 @@ class PagedKV:
         4 b s h table_width page_size bytes)."""
         with torch.cuda.device(self.device):  # partials are counted by the compute units of the cache's device
             return int(N.lib().wz_paged_attn_workspace_bytes(self._ref, b, s, h, table_width, int(accumulate)))
+
+    def attend_tree(self, q, table, lens, parent, softmax_scale, attn_sink=None, count=None, out=None, workspace=None):
+        """``attend`` for a tree of s drafted tokens a sequence (1 to 64, already written): node i is the slot ``lens[b] -
+        s + i`` and sees the slots before the tree, itself and the nodes above it.  ``parent`` [b, s] int32: each node's
+        parent, in any order; one outside [0, s) is none, and the node hangs on the prefix.  ``count`` [b] int32: the
+        nodes of each sequence of a padded batch (its tree begins at ``lens[b] - count[b]``); the rows behind them are
+        0.  ``out`` may not overlap q; ``workspace``: of ``attend_tree_workspace_bytes``."""
+        what = "PagedKV.attend_tree"
+        if q.dim() != 4 or q.shape[3] != self.head_dim:
+            raise ValueError(f"{what}: q must be [b, s, h, {self.head_dim}], got {list(q.shape)}")
+        b, s, h, d = q.shape
+        table = self._table(what, table, b)
+        lens = self._ints(what, "lens", lens, b)
+        parent = self._nodes(what, "parent", parent, b, s)
+        if count is not None:
+            count = self._ints(what, "count", count, b)
+        sink = None
+        if attn_sink is not None:
+            if attn_sink.shape != (h,) or attn_sink.dtype != torch.float32 or attn_sink.device != self.device:
+                raise ValueError(f"{what}: attn_sink must be float32 [{h}] on {self.device}")
+            sink = attn_sink.contiguous()
+        q, qs = self._rows(what, "q", q)
+        out = self._out(what, out, (b, s, h, d))
+        width = table.shape[1]
+        workspace = self._space(what, workspace, self.attend_tree_workspace_bytes, b, s, h, width)
+        self._call("wz_paged_tree_attn", q.data_ptr(), qs, N.ptr(sink), table.data_ptr(), width, lens.data_ptr(),
+                   parent.data_ptr(), N.ptr(count), out.data_ptr(), b, s, h, float(softmax_scale), workspace.data_ptr(),
+                   workspace.numel())
+        return out
+
+    def attend_tree_workspace_bytes(self, b, s, h, table_width) -> int:
+        """Device bytes of an ``attend_tree`` call's partial results."""
+        with torch.cuda.device(self.device):
+            return int(N.lib().wz_paged_tree_attn_workspace_bytes(self._ref, b, s, h, table_width))
+
+    def accept(self, drafted, parent, sampled, table, start, count=None, out=None):
+        """The accepted path of a verified tree of s nodes a sequence (up to 64), node i in slot ``start[b] + i``: node 0
+        (the last token that is known) is accepted, and from an accepted node on its lowest child behind it whose
+        ``drafted`` token is the one ``sampled`` at the node.  Parents come before their children here; a node that does
+        not is never reached.  The accepted nodes' rows move, in order, to the slots from ``start[b]`` on, with their
+        scales, weights and positions; the other nodes' slots are free.  drafted, parent, sampled int32 [b, s];
+        ``count`` [b]: the nodes of each sequence of a padded batch (0: nothing is accepted).
+
+        -> (lens [b], tokens [b, s], path [b, s]) int32 (``out`` if given: three such tensors, over no input):
+        ``start`` and the accepted nodes; what was sampled at them, the last of it the next tree's node 0; and the
+        nodes; both -1 behind them.  A model's layers give the same path: call it on each layer's cache."""
+        what = "PagedKV.accept"
+        if drafted.dim() != 2:
+            raise ValueError(f"{what}: drafted must be int32 [b, s], got {list(drafted.shape)}")
+        b, s = drafted.shape
+        drafted = self._nodes(what, "drafted", drafted, b, s)
+        parent = self._nodes(what, "parent", parent, b, s)
+        sampled = self._nodes(what, "sampled", sampled, b, s)
+        table = self._table(what, table, b)
+        start = self._ints(what, "start", start, b)
+        if count is not None:
+            count = self._ints(what, "count", count, b)
+        if out is None:
+            flat = torch.empty(b * (1 + 2 * s), dtype=torch.int32, device=self.device)
+            out = flat[:b], flat[b:b + b * s].view(b, s), flat[b + b * s:].view(b, s)
+        elif (self._ints(what, "out[0]", out[0], b) is not out[0] or self._nodes(what, "out[1]", out[1], b, s) is not out[1]
+              or self._nodes(what, "out[2]", out[2], b, s) is not out[2]):
+            raise ValueError(f"{what}: out must be contiguous")
+        self._call("wz_paged_accept", drafted.data_ptr(), parent.data_ptr(), sampled.data_ptr(), table.data_ptr(),
+                   table.shape[1], start.data_ptr(), N.ptr(count), out[0].data_ptr(), out[1].data_ptr(),
+                   out[2].data_ptr(), b, s)
+        return out
 
     def evict(self, table, lens, keep, first=0, recent=0, out=None, workspace=None):
         """Cuts every sequence of a tracked cache to ``keep`` slots, in place and for each KV head by itself: the
