@@ -479,11 +479,13 @@ int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, int64_t table
  * probs[row] = w over that sum.  temperature <= 0 takes the first token, probability 1.  NaN and -inf are never
  * taken (a row of nothing else: token -1, probability 0), +inf takes all the weight.  A
  * weight below 2^-42 of the row's largest counts as nothing.  temperature, top_k, top_p and
- * min_p are device arrays [n], or NULL for the value beside them. */
+ * min_p are device arrays [n], or NULL for the value beside them.  Few rows are shared by several workgroups each, with
+ * a workspace (its size is that of the current device; 0: none is needed; one call at a time uses it). */
+int64_t wz_sample_workspace_bytes(int64_t n, int64_t V);
 int wz_sample(const void* logits, int logits_bf16, int64_t row_stride, const float* uniform, const float* temperature,
               float temperature_all, const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
               const float* min_p, float min_p_all, int32_t* tokens, float* probs, int64_t n, int64_t V,
-              hipStream_t stream);
+              void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /* The FP8 wire format of a pipeline-stage boundary — _pack_t / _unpack_t
  * (serving/chain.py:208-222): per row scale = bf16(clamp(amax/448, 1e-8, bf16 max)),

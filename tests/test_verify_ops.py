@@ -32,8 +32,9 @@ def accept(c, d=4096, p=8192, s=12288, table=16384, width=3, start=20480, count=
     return N.lib().wz_paged_accept(ctypes.byref(c), d, p, s, table, width, start, count, lens, tokens, path, B, S, None)
 
 
-def sample(logits=16, bf16=0, stride=100, u=4, tokens=4, probs=4, n=1, V=100):
-    return N.lib().wz_sample(logits, bf16, stride, u, None, 1.0, None, 0, None, 1.0, None, 0.0, tokens, probs, n, V, None)
+def sample(logits=16, bf16=0, stride=100, u=4, tokens=4, probs=4, n=1, V=100, ws=None, wsb=0):
+    return N.lib().wz_sample(logits, bf16, stride, u, None, 1.0, None, 0, None, 1.0, None, 0.0, tokens, probs, n, V, ws, wsb,
+                             None)
 
 
 @pytest.mark.parametrize("call", [append, tree, accept])
@@ -100,6 +101,13 @@ def test_sample_refusals():
         assert sample(**{name: None}) == -1 and "null" in err(), name
     assert sample(logits=18) == -1 and sample(logits=17, bf16=1) == -1 and "aligned" in err()
     assert sample(n=0, u=None) == 0
+    # few long rows are shared by workgroups, many are not; a larger batch's workspace need not serve a smaller one
+    need = N.lib().wz_sample_workspace_bytes
+    assert need(1, 131072) > need(1, 5000) > 0 and need(512, 131072) == 0 and need(1, 4096) == 0
+    assert need(0, 100) == 0 and need(1, 0) == 0 and need(-1, 100) == 0 and need(1, 2 ** 21 + 1) == 0
+    assert sample(V=131072, stride=131072) == -3 and "workspace of 0 bytes" in err()
+    assert sample(V=131072, stride=131072, ws=16, wsb=100) == -3 and "workspace of 100 bytes" in err()
+    assert sample(V=131072, stride=131072, ws=8, wsb=1 << 30) == -1 and "16-byte" in err()
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         kernels.sample(torch.zeros(1, 5), torch.zeros(1))
 

@@ -69,7 +69,9 @@ SIGNATURES = {
     "wz_paged_accept": (_I, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _P]),
     "wz_paged_evict_workspace_bytes": (_I64, [_P, _I64, _I64, _I64]),
     "wz_paged_evict": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P]),
-    "wz_sample": (_I, [_P, _I, _I64, _P, _P, _F, _P, ctypes.c_int32, _P, _F, _P, _F, _P, _P, _I64, _I64, _P]),
+    "wz_sample": (_I, [_P, _I, _I64, _P, _P, _F, _P, ctypes.c_int32, _P, _F, _P, _F, _P, _P, _I64, _I64, _P, _I64,
+                       _P]),
+    "wz_sample_workspace_bytes": (_I64, [_I64, _I64]),
     "wz_fp8_wire_unpack": (_I, [_P, _P, _P, _I64, _I64, _P]),
     "wz_synth_fill": (_I, [_P, _I64, ctypes.c_uint64, _I64, _I, ctypes.c_double, ctypes.c_double, _P]),
     "wz_prof_begin": (_I, [_I]),

@@ -575,7 +575,7 @@ def sparse_attn_workspace_bytes(b, s, h, d, topk) -> int:
     return int(N.lib().wz_sparse_attn_workspace_bytes(b, s, h, d, topk))
 
 
-def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, workspace=None):
     """One token a row: logits [n, V] float32 or bf16 (rows dense, any stride between them), ``uniform`` [n] float32 in
     [0, 1), one random number a row -> (tokens int32 [n], probs float32 [n]), in ``out`` if given.
 
@@ -587,7 +587,9 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=
     probability 0.  A weight below 2^-42 of the row's largest counts as nothing.
 
     Each of the four is one number for all rows, or a tensor [n] on the logits' device (float32, ``top_k`` int32; not read
-    by the host).  The reference's tail takes the highest logit (temperature 0)."""
+    by the host).  The reference's tail takes the highest logit (temperature 0).  ``workspace``: a uint8 tensor of
+    ``sample_workspace_bytes``, for calls that must not allocate (with ``out``); calls that overlap in time need one
+    each."""
     what = "sample"
     _require_cuda(logits, uniform)
     if logits.dim() != 2 or logits.shape[1] < 1:
@@ -620,10 +622,20 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=
     elif rows("out[0]", out[0], torch.int32) is not out[0] or rows("out[1]", out[1], torch.float32) is not out[1]:
         raise ValueError(f"{what}: out must be contiguous")
     with torch.cuda.device(dev):
+        if workspace is None:
+            need = sample_workspace_bytes(n, V)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor on {dev}")
         N.call("wz_sample", N.ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0) if n > 1 else V,
                N.ptr(uniform), *[N.ptr(x) if i % 2 == 0 else x for i, x in enumerate(args)], N.ptr(out[0]), N.ptr(out[1]),
-               n, V, N.stream_handle(dev))
+               n, V, N.ptr(workspace), 0 if workspace is None else workspace.numel(), N.stream_handle(dev))
     return out
+
+
+def sample_workspace_bytes(n, V) -> int:
+    """Device bytes that a sample call of n rows of V logits shares among its workgroups, on the current device (0: none)."""
+    return int(N.lib().wz_sample_workspace_bytes(n, V))
 
 
 def wire_pack(t):
