@@ -9,7 +9,9 @@
 //   * the loads fill a ring of NS tiles in LDS directly; a wave has T / NW rows of a tile, which lie in one page;
 //   * one barrier a tile: a tile that a wave's loads have brought is there for all behind it, and the tile before it is free;
 //   * p = 2^(y - m) as in paged_attn_kernel, m moved only when a tile's maximum exceeds it by more than 8.
-// Units, shares, partials and the join are paged_attn_kernel's.
+// Units, shares, partials and the join are paged_attn_kernel's, but that units without a row of a sequence's own nodes are none.
+// 8 trees of 64 nodes over 8191 tokens, 64 heads on 8 of 128 (268 MB, 137 GF) 164 us, 840 TFLOP/s, the matrix units busy
+// two fifths of it, the vector units as long; a product of 8192^3 by the library does 1218.
 #pragma once
 
 #include <cfloat>
@@ -28,20 +30,17 @@ struct WideCfg {
   static constexpr int SIDE = kWideTile * RB;
   static constexpr int STAGE = SIDE * (SHARED ? 1 : 2);
   static constexpr int SCALES = FP8 ? 8 * kWideTile : 0;  // a tile's K and V scales
-  // A wave loads RPW rows of each side, or (HALF) where they are less than a load 16 of one.
-  static constexpr bool HALF = kWideTile / NW * RB < 1024;
-  static constexpr int RPW = HALF ? 16 : kWideTile / NW;
-  static constexpr int LPS = RPW * RB / 1024;  // loads of them
-  static constexpr int LOADS = LPS * (SHARED || HALF ? 1 : 2) + (FP8 ? 1 : 0);
+  static constexpr int RPW = kWideTile / NW;      // rows that a wave loads of each side
+  static constexpr int LPS = RPW * RB / 1024;     // loads of them
+  static constexpr int LOADS = LPS * (SHARED ? 1 : 2) + (FP8 ? 1 : 0);
   static constexpr int ROWS = 32 * NW;
-  static constexpr int PER_CU = NW == 8 ? 1 : 2;
+  static constexpr int PER_CU = 8 / NW;                   // two waves a SIMD
   static constexpr int FIT = 150 * 1024 / PER_CU / (STAGE + SCALES);
   static constexpr int NS = FIT < 6 ? FIT : 6;
   static constexpr int RING = NS * (STAGE + SCALES);
   static constexpr int LDS = RING + NS * 8;  // valid masks
   static_assert(LPS * 1024 == RPW * RB && LPS >= 1 && NS >= 2 && NS * LOADS < 64, "whole loads, counted by the waits");
   static_assert(RPW <= 16 && RPW >= 8, "a wave's rows lie in one page, and fill bytes of the mask");
-  static_assert(!HALF || (!SHARED && NW == 8), "four waves a side");
 };
 
 // 16-byte chunk c of row r at slot c ^ swz(r).  The fragments' 16-byte reads take one chunk of 32 rows, the transposing ones four
@@ -67,6 +66,62 @@ __device__ __forceinline__ float wide_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Units of a sequence that hold rows of its nodes, and all of their cost; paged_total and paged_find over them.
+template <int ROWS>
+__device__ __forceinline__ int wide_live(const PagedAttnArgs& a, int b) {
+  return a.c.heads * ((paged_nodes(a, b) * (a.H / a.c.heads) + ROWS - 1) / ROWS);
+}
+template <int ROWS>
+__device__ __forceinline__ int wide_cost(const PagedAttnArgs& a, int b) {
+  return b < a.B ? paged_cost<kWideTile, kPagedStart>(paged_len(a, b)) * wide_live<ROWS>(a, b) : 0;
+}
+template <int ROWS>
+__device__ __forceinline__ int wide_total(const PagedAttnArgs& a) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) sum += wide_cost<ROWS>(a, b0 + lane);
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  return __builtin_amdgcn_readfirstlane(sum);
+}
+template <int ROWS>
+__device__ __forceinline__ void wide_find(const PagedAttnArgs& a, int x, int* seq, int* before) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int g = wide_cost<ROWS>(a, b0 + lane);
+    int inc = g;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += y;
+    }
+    const uint64_t past = __ballot(sum + inc > x);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      *seq = b0 + l;
+      *before = __builtin_amdgcn_readlane(sum + inc - g, l);
+      return;
+    }
+    sum += __builtin_amdgcn_readlane(inc, 63);
+  }
+  *seq = a.B - 1;  // not reached: x is below the total
+  *before = sum;
+}
+
+// The rows that are no node's, of the sequences w, w + a.W, ...: zeros, and no parts of the units that hold nothing else.
+template <int ROWS>
+__device__ __forceinline__ void wide_empty(const PagedAttnArgs& a, int w, int RG, int D) {
+  const int grp = a.H / a.c.heads, upb = a.c.heads * RG;
+  for (int b = w; b < a.B; b += a.W) {
+    const int nodes = paged_len(a, b) > 0 ? paged_nodes(a, b) : 0, live = (nodes * grp + ROWS - 1) / ROWS;
+    const int64_t node = int64_t(a.H) * (D / 8), end = (int64_t(b) + 1) * a.S * node;
+    for (int64_t i = (int64_t(b) * a.S + nodes) * node + threadIdx.x; i < end; i += blockDim.x)
+      *reinterpret_cast<v4i*>(a.o + i * 8) = v4i{0, 0, 0, 0};
+    if (a.by_unit)
+      for (int u = threadIdx.x; u < upb; u += blockDim.x)
+        if (u % RG >= live) a.cut[int64_t(b) * upb + u] = PagedCut{b, u, 0, 0};
+  }
+}
+
 template <int D, bool FP8, bool SHARED, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a) {
   using C = WideCfg<D, FP8, SHARED, NW>;
@@ -81,18 +136,17 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
 
   const int grp = a.H / a.c.heads, R = a.S * grp, RG = (R + ROWS - 1) / ROWS, upb = a.c.heads * RG;
   const int w = blockIdx.x;
-  const PagedShares shares(paged_total<T, kPagedStart>(a, upb), a.W);
+  wide_empty<ROWS>(a, w, RG, D);
+  const PagedShares shares(wide_total<ROWS>(a), a.W);
   if (!a.by_unit && tid == 0) a.cut[w] = PagedCut{0, 0, 0, 0};
-  if (w >= shares.workers) {
-    paged_empty(a, w, upb, D, 64 * NW);
-    return;
-  }
+  if (w >= shares.workers) return;
   int x = shares.begin(w);
   const int x_end = shares.begin(w + 1);
   int b, before;  // sequence, and the granules before it
-  paged_find<T, kPagedStart>(a, upb, x, &b, &before);
+  wide_find<ROWS>(a, x, &b, &before);
   int n = __builtin_amdgcn_readfirstlane(paged_len(a, b)), cost = paged_cost<T, kPagedStart>(n);
-  int u = (x - before) / cost, ubeg = before + u * cost;  // unit of the sequence, and where it begins
+  int live = __builtin_amdgcn_readfirstlane(wide_live<ROWS>(a, b));
+  int u = (x - before) / cost, ubeg = before + u * cost;  // of the sequence's live units, and where it begins
   const int ps = a.c.shift, page = a.c.page;
   // the largest of the raw products is the largest of the scaled ones too: a negative scale turns Q's signs
   const float scale2 = a.scale2 == 0.0f ? FLT_MIN : fabsf(a.scale2);  // (masked products are -inf times it)
@@ -102,16 +156,20 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
     ubeg += cost;
     if (ubeg >= x_end) return false;
     x = ubeg;
-    if (++u == upb) {
+    if (++u == live) {
       do {
         ++b;
         n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-      } while (n == 0);
+        live = __builtin_amdgcn_readfirstlane(wide_live<ROWS>(a, b));
+      } while (n == 0 || live == 0);
       cost = paged_cost<T, kPagedStart>(n);
       u = 0;
     }
     return true;
   };
+  // Of the two waves of a SIMD one goes first: its exponentials then run beside the other's products.  Taking turns they would do
+  // the same at the same time.
+  if (wave >= 4) __builtin_amdgcn_s_setprio(1);
   for (bool more = true; more; more = next()) {
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));  // the lane's coordinates, made anew for each part
@@ -120,23 +178,23 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
     const int g0 = max(x - ubeg - kPagedStart, 0), g1 = min(x_end - ubeg, cost) - kPagedStart;
     if (g1 <= 0) continue;
     const bool whole = g0 == 0 && g1 == cost - kPagedStart;
-    const int hk = u / RG, rg = u - hk * RG;
+    const int lrg = live / a.c.heads, hk = u / lrg, rg = u - hk * lrg;
     const int row0 = rg * ROWS + 32 * wave;  // this wave's first row
-    const bool busy = row0 < R;
     const int t0 = g0 * T, tm = min(g1 * T, n);
     // the tree's tokens, from n0 on, are seen by some rows only (as in paged_attn_kernel)
     const int nodes = __builtin_amdgcn_readfirstlane(paged_nodes(a, b)), n0 = n - nodes;
+    const bool busy = row0 < nodes * grp;  // or the wave has no row of the sequence's nodes
     const uint64_t masks = tm > n0 ? paged_tree_masks(a, b, nodes, lane) : 0ull;
     const int rq = min(row0 + nl, R - 1);  // this lane's row
     int odd0 = 0, odd1 = 0;
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
-      a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
-          PagedCut{b, u, whole ? 1 : shares.owner(ubeg + cost - 1) - w + 1, w};
+      a.cut[a.by_unit ? int64_t(b) * upb + hk * RG + rg : w] =
+          PagedCut{b, hk * RG + rg, whole ? 1 : shares.owner(ubeg + cost - 1) - w + 1, w};
     const int32_t* const trow = a.table + int64_t(b) * a.width;
 
     // ---- loads ----
     const int nk = (tm - t0 + T - 1) / T;
-    const int wrow = C::RPW * (C::HALF ? wave & 3 : wave);  // this wave's first row of a tile's loads
+    const int wrow = C::RPW * wave;  // this wave's first row of a tile's loads
     int ids = -1, ids_base = 0;  // lane e: the page of this wave's rows of tile base + e
     auto fetch_ids = [&](int k0) {
       ids_base = k0;
@@ -152,7 +210,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
       const uint32_t valid = id < 0 ? 0u : tm - t >= C::RPW ? (1u << C::RPW) - 1u : (1u << max(tm - t, 0)) - 1u;
       if (lane == 0) {
         if constexpr (C::RPW == 8) s_valid[8 * stage + wave] = uint8_t(valid);
-        else *reinterpret_cast<uint16_t*>(s_valid + 8 * stage + wrow / 8) = uint16_t(valid);  // (HALF: both sides' waves)
+        else *reinterpret_cast<uint16_t*>(s_valid + 8 * stage + wrow / 8) = uint16_t(valid);
       }
       const int64_t row = (int64_t(max(id, 0)) * a.c.heads + hk) * page + (t & (page - 1));
       const int rin = lane / CH, slot = lane % CH;
@@ -165,17 +223,11 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
           paged_load16(pool + (row + r) * RB, voff, dst + j * 1024);
         }
       };
-      if constexpr (C::HALF) {
-        load(wave < 4 ? a.c.k : a.c.v, wave >> 2);
-      } else {
-        load(a.c.k, 0);
-        if constexpr (!SHARED) load(a.c.v, 1);
-      }
-      if constexpr (FP8) {  // K's with the first RPW lanes, V's with the next (HALF: this wave's side's)
-        const uint32_t at = C::HALF ? (wave >> 2) * T + wrow : 2 * wrow;
-        const uint32_t sdst = __builtin_amdgcn_readfirstlane(scales_lds + stage * C::SCALES + 4 * at);
-        const bool second = C::HALF ? wave >= 4 : lane >= C::RPW;
-        if (lane < (C::HALF ? 1 : 2) * C::RPW) paged_load4((second ? a.c.vs : a.c.ks) + row + lane % C::RPW, sdst);
+      load(a.c.k, 0);
+      if constexpr (!SHARED) load(a.c.v, 1);
+      if constexpr (FP8) {  // K's with the first RPW lanes, V's with the next
+        const uint32_t sdst = __builtin_amdgcn_readfirstlane(scales_lds + stage * C::SCALES + 8 * wrow);
+        if (lane < 2 * C::RPW) paged_load4((lane >= C::RPW ? a.c.vs : a.c.ks) + row + lane % C::RPW, sdst);
       }
     };
     if (nk > 0) fetch_ids(0);
@@ -215,9 +267,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
       const float* const sc = reinterpret_cast<const float*>(scales + stage * C::SCALES);
       uint64_t valid = uint64_t(paged_uniform(*reinterpret_cast<const int64_t*>(s_valid + 8 * stage)));
       const int tk = t0 + T * k;
-      auto scale_at = [&](int t, int side) {  // where token t's scale stands
-        return C::HALF ? side * T + t : t / C::RPW * 2 * C::RPW + side * C::RPW + t % C::RPW;
-      };
+      // where token t's scale stands
+      auto scale_at = [](int t, int side) { return t / C::RPW * 2 * C::RPW + side * C::RPW + t % C::RPW; };
       const bool last = tk + T > n0;
       if (last) {
         const uint64_t some = valid & ~((1ull << max(n0 - tk, 0)) - 1ull);  // tokens that some rows see
@@ -245,31 +296,39 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
       if (!busy) continue;
 
       // ---- S^T: s[tt][i] = q . k of row n, token 32 tt + 8 (i >> 2) + 4 h + (i & 3) ----
-      pv16f s[2];
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        s[tt] = pv16f(0.0f);
-        const uint8_t* const krow = kt + (32 * tt + nl) * RB;
+      // Fragments are read kAhead steps ahead of their products: left to the compiler each read stood right before its product.
+      constexpr int kAhead = 3;
+      pv16f s[2] = {pv16f(0.0f), pv16f(0.0f)};
+      {
+        constexpr int STEPS = FP8 ? KC / 2 : KC;  // reads of a row
+        const uint8_t* const krow = kt + nl * RB;
         const int sw = wide_swz<RB>(nl);
-        if constexpr (!FP8) {
+        v4i kf[kAhead + 1];
+        auto kload = [&](int j) {  // j = 2 step + tt
+          kf[j % (kAhead + 1)] = *reinterpret_cast<const v4i*>(krow + 32 * (j & 1) * RB + (((2 * (j >> 1) + h) ^ sw) << 4));
+        };
 #pragma unroll
-          for (int cc = 0; cc < KC; ++cc)
-            s[tt] = wide_mfma(*reinterpret_cast<const pv8s*>(krow + (((2 * cc + h) ^ sw) << 4)), qf[cc], s[tt]);
-        } else {
+        for (int j = 0; j < kAhead; ++j) kload(j);
 #pragma unroll
-          for (int cp = 0; cp < KC / 2; ++cp) {
-            const v4i kc = *reinterpret_cast<const v4i*>(krow + (((2 * cp + h) ^ sw) << 4));
-            s[tt] = wide_mfma(paged_widen(kc[0], kc[1]), qf[2 * cp], s[tt]);
-            s[tt] = wide_mfma(paged_widen(kc[2], kc[3]), qf[2 * cp + 1], s[tt]);
+        for (int j = 0; j < 2 * STEPS; ++j) {
+          if (j + kAhead < 2 * STEPS) kload(j + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+          const v4i kc = kf[j % (kAhead + 1)];
+          if constexpr (!FP8) {
+            s[j & 1] = wide_mfma(__builtin_bit_cast(pv8s, kc), qf[j >> 1], s[j & 1]);
+          } else {
+            s[j & 1] = wide_mfma(paged_widen(kc[0], kc[1]), qf[2 * (j >> 1)], s[j & 1]);
+            s[j & 1] = wide_mfma(paged_widen(kc[2], kc[3]), qf[2 * (j >> 1) + 1], s[j & 1]);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (FP8) {
+      }
+      if constexpr (FP8) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const v4f ks = *reinterpret_cast<const v4f*>(sc + scale_at(32 * tt + 8 * j + 4 * h, 0));
+        for (int j = 0; j < 8; ++j) {
+          const v4f ks = *reinterpret_cast<const v4f*>(sc + scale_at(8 * j + 4 * h, 0));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[tt][4 * j + i] *= ks[i];
-          }
+          for (int i = 0; i < 4; ++i) s[j >> 2][4 * (j & 3) + i] *= ks[i];
         }
       }
       // ---- softmax ----
@@ -328,26 +387,34 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
       }
       // ---- O^T += V^T P^T, 16 tokens at a time ----
       const int l16 = lane & 15, side = (lane >> 4) & 1;  // column 16 side + l16 of 32
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          pv8s vf;
-          if constexpr (!FP8) {
-            const int row = 16 * q + 4 * h + (l16 >> 2), c = 4 * nt + 2 * side + ((l16 >> 1) & 1);
-            const pv4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_pv4s*)(vt + row * RB + ((c ^ wide_swz<RB>(row)) << 4) + (l16 & 1) * 8));
-            const pv4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_pv4s*)(vt + (row + 8) * RB + ((c ^ wide_swz<RB>(row + 8)) << 4) + (l16 & 1) * 8));
-            vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          } else {
-            const int row = 16 * q + 4 * h + ((l16 >> 1) & 3) + 8 * (l16 >> 3), c = 2 * nt + side;
-            const pv2i c8 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (lds_pv2i*)(vt + row * RB + ((c ^ wide_swz<RB>(row)) << 4) + (l16 & 1) * 8));
-            vf = paged_widen(c8[0], c8[1]);
-          }
-          acc[nt] = wide_mfma(vf, pf[q], acc[nt]);
+      v4i vf[kAhead + 1];
+      auto vload = [&](int j) {  // j = NT q + nt
+        const int q = j / NT, nt = j % NT;
+        v4i& f = vf[j % (kAhead + 1)];
+        if constexpr (!FP8) {
+          const int row = 4 * h + (l16 >> 2), c = 4 * nt + 2 * side + ((l16 >> 1) & 1);  // 16 rows on the swizzle is the same
+          const pv4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_pv4s*)(vt + (16 * q + row) * RB + ((c ^ wide_swz<RB>(row)) << 4) + (l16 & 1) * 8));
+          const pv4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_pv4s*)(vt + (16 * q + row + 8) * RB + ((c ^ wide_swz<RB>(row + 8)) << 4) + (l16 & 1) * 8));
+          f = __builtin_bit_cast(v4i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+          const int row = 4 * h + ((l16 >> 1) & 3) + 8 * (l16 >> 3), c = 2 * nt + side;
+          const pv2i c8 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (lds_pv2i*)(vt + (16 * q + row) * RB + ((c ^ wide_swz<RB>(row)) << 4) + (l16 & 1) * 8));
+          f[0] = c8[0];
+          f[1] = c8[1];
         }
+      };
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) vload(j);
+#pragma unroll
+      for (int j = 0; j < 4 * NT; ++j) {
+        if (j + kAhead < 4 * NT) vload(j + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+        const v4i f = vf[j % (kAhead + 1)];
+        acc[j % NT] = wide_mfma(FP8 ? paged_widen(f[0], f[1]) : __builtin_bit_cast(pv8s, f), pf[j / NT], acc[j % NT]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 
@@ -389,7 +456,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
     // ---- the part's end ----
     l_run = wide_sum(l_run);
     const int r = row0 + nl;
-    if (r < R) {
+    if (r < nodes * grp) {  // the rest is zeros already (the join writes them again)
       if (whole) {
         const int head = hk * grp + r % grp, node = r / grp;
         float den = l_run, f = 1.0f;
@@ -398,16 +465,15 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
           f = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - Me);
           den = den * f + __builtin_amdgcn_exp2f(sk - Me);
         }
-        const bool dead = node >= nodes;  // no node's row
         const float inv = den == 0.0f ? 0.0f : f / den;
         uint16_t* const orow = a.o + ((int64_t(b) * a.S + node) * a.H + head) * D + 4 * h;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint2 o = make_uint2(f32x2_to_bf16x2(acc[nt][4 * j] * inv, acc[nt][4 * j + 1] * inv),
-                                       f32x2_to_bf16x2(acc[nt][4 * j + 2] * inv, acc[nt][4 * j + 3] * inv));
-            *reinterpret_cast<uint2*>(orow + 32 * nt + 8 * j) = dead ? make_uint2(0, 0) : o;
+            *reinterpret_cast<uint2*>(orow + 32 * nt + 8 * j) =
+                make_uint2(f32x2_to_bf16x2(acc[nt][4 * j] * inv, acc[nt][4 * j + 1] * inv),
+                           f32x2_to_bf16x2(acc[nt][4 * j + 2] * inv, acc[nt][4 * j + 3] * inv));
           }
       } else {
         float* const part = a.part + (2 * int64_t(w) + (g0 == 0 ? 1 : 0)) * paged_slot(a.rows, D);
@@ -426,7 +492,6 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_wide_kernel(PagedAttnArgs a)
     }
     meet();  // the ring is free for the next part's tiles
   }
-  paged_empty(a, w, upb, D, 64 * NW);
 }
 
 template <int D, bool FP8, bool SHARED, int NW>
@@ -450,12 +515,14 @@ int paged_wide_launch(PagedAttnArgs a, bool ask, int* workers, hipStream_t strea
   return paged_attn_join<D>(a, stream);
 }
 
-// Rows beyond 64: 4 waves, beyond 128: 8.
+// Rows beyond 64: workers of 4 waves, beyond 128 rows of 128 of 8, which read the cache half as often (8 x 8191 tokens, 512 rows:
+// 164 us against 188).  Heads of 64 stay with 4: a tile's time there is one wave's way through it, and two workers a compute unit
+// go theirs side by side (24 x 1125 .. 9001 e4m3 tokens, 8 to 192 rows: 65 us against 99).
 template <int D, bool FP8, bool SHARED>
 int paged_wide(const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
-  const int R = a.S * (a.H / a.c.heads);
-  if (R <= 128) return paged_wide_launch<D, FP8, SHARED, 4>(a, ask, workers, stream);
-  return paged_wide_launch<D, FP8, SHARED, 8>(a, ask, workers, stream);
+  if constexpr (D == 128)
+    if (a.S * (a.H / a.c.heads) > 128) return paged_wide_launch<D, FP8, SHARED, 8>(a, ask, workers, stream);
+  return paged_wide_launch<D, FP8, SHARED, 4>(a, ask, workers, stream);
 }
 
 template <bool FP8>
