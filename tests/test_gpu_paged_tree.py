@@ -204,3 +204,96 @@ def test_refusals_workspace_and_outputs(gpu):
     with pytest.raises(Exception, match="S=65"):
         z = torch.zeros(2, 65, HK * g, D, dtype=torch.bfloat16, device=gpu)
         cache.attend_tree(z, tab, n, torch.zeros(2, 65, dtype=torch.int32, device=gpu), 1.0, workspace=ws)
+
+
+WIDE = [  # HK, g, S, D, shared: 65 rows and more a KV head
+    (1, 5, 13, 64, False), (2, 8, 24, 64, False), (1, 7, 40, 64, False), (1, 4, 32, 128, False), (2, 3, 43, 128, False),
+    (1, 8, 64, 128, False), (1, 2, 40, 128, True), (1, 9, 30, 128, True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("HK,g,S,D,shared", WIDE)
+def test_many_rows_of_padded_trees(gpu, HK, g, S, D, shared, dtype):
+    """Trees of every size from none to S, so that waves and whole units have no node's row, over prefixes at the tiles'
+    borders and one that many workgroups share; pages that end inside a tile; a sink."""
+    count = [S, 0, 1, S // 3, S - 1, S, 2 * S, -1, S // 2]
+    pre = [0, 70, 63, 64, 128, 3000, 17, 30, 700]
+    lens = [min(max(c, 0), S) + p for c, p in zip(count, pre)]
+    cache, vals, tab, table = make(gpu, S + g, lens, HK=HK, D=D, page=16 if S % 2 else 32, dtype=dtype, shared=shared)
+    q, qd = queries(gpu, S, len(lens), S, HK * g, D, scale=1.5, strided=True)
+    parent = trees(S, len(lens), S, "forest")
+    sink = torch.linspace(-2, 3, HK * g)
+    out = torch.full((len(lens), S, HK * g, D), float("nan"), dtype=torch.bfloat16, device=gpu)
+    o = run(gpu, cache, tab, lens, parent, q, D ** -0.5, attn_sink=sink.to(gpu), count=count, out=out)
+    check(o, op.attend_tree(vals, qd, table, lens, parent, D ** -0.5, sink.double().numpy(), count=count), D)
+    for b, c in enumerate(count):
+        assert (o[b, min(max(c, 0), S):] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("HK,g,S,D,shared", WIDE)
+@pytest.mark.parametrize("n", [0, 50, 900])
+def test_many_rows_take_nothing_from_branches_they_do_not_see(gpu, n, HK, g, S, D, shared, dtype):
+    """NaN in the K of one node and the V of others, over two tiles of the tree: rows without them above stay as they were."""
+    lens = [S + n, S + n + 37]
+    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared)
+    q, qd = queries(gpu, 4, 2, S, HK * g, D)
+    parent = trees(3, 2, S)
+    ref = op.attend_tree(vals, qd, table, lens, parent, D ** -0.5)
+    bad = {1: cache.k, S // 2: cache.k if shared else cache.v, S - 2: cache.k if shared else cache.v}
+    for b, m in enumerate(lens):
+        for node, pool in bad.items():
+            t = m - S + node
+            row = pool[table[b, t // 16], :, t % 16]
+            row.view(torch.uint8 if dtype == E4M3 else torch.int16).fill_(0x7F if dtype == E4M3 else 0x7FC0)
+    o = run(gpu, cache, tab, lens, parent, q, D ** -0.5)
+    for b in range(2):
+        dirty = [i for i, seen in enumerate(op.tree_sight(parent[b], S)) if seen & set(bad)]
+        clean = [i for i in range(S) if i not in dirty]
+        check(o[b:b + 1, clean], tuple(x[b:b + 1, clean] if i < 2 else x for i, x in enumerate(ref)), D)
+        assert torch.isnan(o[b, dirty]).all()
+
+
+@pytest.mark.parametrize("HK,g,S,D,shared", [(1, 5, 13, 64, False), (1, 4, 32, 128, False), (1, 8, 40, 128, False)])
+def test_many_rows_of_more_units_than_workers(gpu, HK, g, S, D, shared):
+    B = 560
+    lens = [S + (7 * b) % 90 for b in range(B)]
+    cache, vals, tab, table = make(gpu, 21, lens, HK=HK, D=D, page=16)
+    q, qd = queries(gpu, 21, B, S, HK * g, D)
+    parent = trees(21, B, S)
+    o = run(gpu, cache, tab, lens, parent, q, D ** -0.5)
+    some = [0, 1, 255, 256, 300, 511, 512, 559]
+    pick = lambda x: np.ascontiguousarray(x[some])  # noqa: E731
+    ref = op.attend_tree(vals, pick(qd), pick(table), [lens[b] for b in some], pick(parent), D ** -0.5)
+    check(o[some], ref, D)
+    assert torch.isfinite(o).all()
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 3.0])
+@pytest.mark.parametrize("g,S,D", [(4, 3, 64), (8, 20, 64), (8, 30, 128)])
+def test_scales_of_any_sign(gpu, g, S, D, scale):
+    lens = [S + 5, S + 200]
+    cache, vals, tab, table = make(gpu, 31, lens, HK=1, D=D, page=16)
+    q, qd = queries(gpu, 31, 2, S, g, D)
+    parent = trees(31, 2, S)
+    o = run(gpu, cache, tab, lens, parent, q, scale)
+    ref = op.attend_tree(vals, qd, table, lens, parent, scale)
+    check(o, (*ref[:3], abs(ref[3]) if scale >= 0 else float(np.abs(op.attend_tree(vals, -qd, table, lens, parent, -scale)[3]))), D)
+
+
+@pytest.mark.parametrize("g,S,D", [(8, 24, 64), (8, 12, 128), (8, 40, 128)])
+def test_many_rows_whose_maximum_moves(gpu, g, S, D):
+    """K that grows along the sequence, so that the maximum moves far at many tiles."""
+    lens = [S + 900, S + 333]
+    cache, vals, tab, table = make(gpu, 5, lens, HK=1, D=D, page=32)
+    grow = torch.ones(cache.pages, 1, 32, 1)
+    for b, n in enumerate(lens):
+        for p in range(-(-n // 32)):
+            grow[table[b, p]] = 2.0 ** (p // 4)
+    k = (torch.from_numpy(vals["k"]) * grow).to(torch.bfloat16)
+    cache.k.copy_(torch.where(torch.isnan(cache.k.cpu()), cache.k.cpu(), k).to(gpu))
+    vals["k"] = k.double().numpy()
+    q, qd = queries(gpu, 6, 2, S, g, D)
+    parent = trees(6, 2, S)
+    o = run(gpu, cache, tab, lens, parent, q, 0.3)
+    check(o, op.attend_tree(vals, qd, table, lens, parent, 0.3), D)

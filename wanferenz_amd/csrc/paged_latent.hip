@@ -105,7 +105,6 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
     // from n0 on a token is seen by some rows only, as in paged_attn_kernel
     const int nodes = TREE ? __builtin_amdgcn_readfirstlane(paged_nodes(a, b)) : 0;
     const int n0 = TREE ? n - nodes : n - a.S + 1;
-    const uint64_t masks = TREE && tm > n0 ? paged_tree_masks(a, b, nodes, lane) : 0ull;
     int odd0 = 0, odd1 = 0;
     if (g0 == 0 && tid == 0 && (a.by_unit || !whole))
       a.cut[a.by_unit ? int64_t(b) * upb + u : w] =
@@ -292,8 +291,8 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
           }
           if (last) {
             const int s = min(row0 + 16 * (ht0 + h) + nl, R - 1) / grp;
-            if constexpr (TREE) {
-              const uint64_t mask = paged_tree_mask(masks, s);
+            if constexpr (TREE) {  // (the masks are made where they are used: held all along they cost a register too many)
+              const uint64_t mask = paged_tree_mask(paged_tree_masks(a, b, nodes, ln), s);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int node = tk + 16 * rt + 4 * g + i - n0;
@@ -438,7 +437,8 @@ __global__ __launch_bounds__(64 * kLatentWaves, 2) void paged_latent_kernel(Page
       }
       meet();
       const int r = row0 + lane;
-      const uint64_t mask = TREE ? paged_tree_mask(masks, min(r, R - 1) / grp) >> ((t - n0) & 63) : 0ull;
+      const uint64_t mask =
+          TREE ? paged_tree_mask(paged_tree_masks(a, b, nodes, lane), min(r, R - 1) / grp) >> ((t - n0) & 63) : 0ull;
       const bool sees = lane < ROWS && r < R && (TREE ? mask & 1 : t < n - (a.S - 1 - r / grp));
       const float yy = s_y[lane < ROWS ? lane : 0];
       const float m_new = sees ? fmaxf(m_run, yy) : m_run, m = m_new == -INFINITY ? 0.0f : m_new;

@@ -605,32 +605,47 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=
         return t if t.is_contiguous() else t.contiguous()
 
     uniform = rows("uniform", uniform, torch.float32)
-    args = []
-    for name, x, dtype, most in (("temperature", temperature, torch.float32, None), ("top_k", top_k, torch.int32, None),
-                                 ("top_p", top_p, torch.float32, 1), ("min_p", min_p, torch.float32, 1)):
+
+    def value(name, x, dtype, most):  # (device pointer, value)
         if isinstance(x, torch.Tensor):
-            x = rows(name, x, dtype)
-            args += [x, 0]
-            continue
-        if not x >= 0 or (most is not None and x > most):
-            raise ValueError(f"{what}: {name} = {x} (0 or more{'' if most is None else ', 1 or less'})")
-        args += [None, min(int(x), 2**31 - 1) if dtype == torch.int32 else float(x)]
+            held.append(rows(name, x, dtype))
+            return held[-1].data_ptr(), 0
+        if not 0 <= x <= most:
+            raise ValueError(f"{what}: {name} = {x} (from 0{f' to {most}' if most < inf else ''})")
+        return None, x if dtype == torch.float32 else min(int(x), 2**31 - 1)
+
+    held, inf = [], float("inf")  # copies live until the launch
+    args = (value("temperature", temperature, torch.float32, inf), value("top_k", top_k, torch.int32, inf),
+            value("top_p", top_p, torch.float32, 1), value("min_p", min_p, torch.float32, 1))
     if logits.stride(1) != 1 or (n > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+        out = torch.empty(n, dtype=torch.int32, device=dev), uniform.new_empty((n,))
     elif rows("out[0]", out[0], torch.int32) is not out[0] or rows("out[1]", out[1], torch.float32) is not out[1]:
         raise ValueError(f"{what}: out must be contiguous")
-    with torch.cuda.device(dev):
-        if workspace is None:
-            need = sample_workspace_bytes(n, V)
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
-            raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor on {dev}")
-        N.call("wz_sample", N.ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0) if n > 1 else V,
-               N.ptr(uniform), *[N.ptr(x) if i % 2 == 0 else x for i, x in enumerate(args)], N.ptr(out[0]), N.ptr(out[1]),
-               n, V, N.ptr(workspace), 0 if workspace is None else workspace.numel(), N.stream_handle(dev))
+    if workspace is not None and (workspace.dtype != torch.uint8 or workspace.device != dev
+                                  or not workspace.is_contiguous()):
+        raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor on {dev}")
+    t, k, p, m = args
+    args = (logits.data_ptr(), int(logits.dtype == torch.bfloat16), logits.stride(0) if n > 1 else V, uniform.data_ptr(),
+            *t, *k, *p, *m, out[0].data_ptr(), out[1].data_ptr(), n, V)
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = _sample_on(dev, workspace, n, V, args)
+    else:
+        with torch.cuda.device(dev):
+            rc = _sample_on(dev, workspace, n, V, args)
+    if rc:
+        N.check(rc, "wz_sample")
     return out
+
+
+def _sample_on(dev, workspace, n, V, args):
+    lib = N.lib()
+    if workspace is None:
+        need = lib.wz_sample_workspace_bytes(n, V)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+    return lib.wz_sample(*args, ws, size, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
 def sample_workspace_bytes(n, V) -> int:

@@ -139,9 +139,9 @@ class PagedKV:
             raise ValueError(f"{what}: {name} is on {t.device}, the cache on {self.device}")
         return t if t.is_contiguous() else t.contiguous()
 
-    def _out(self, what, out, shape):
+    def _out(self, what, q, out, shape):
         if out is None:
-            return torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            return q.new_empty(shape)
         if out.shape != shape or out.dtype != torch.bfloat16 or out.device != self.device or not out.is_contiguous():
             raise ValueError(f"{what}: out must be contiguous bf16 {list(shape)} on {self.device}")
         return out
@@ -255,8 +255,8 @@ class PagedKV:
             if w is not None and (w.shape != (d,) or w.dtype != torch.float32 or w.device != self.device
                                   or not w.is_contiguous()):
                 raise ValueError(f"{what}: {name} must be contiguous float32 [{d}] on {self.device}")
-        out = self._out(what, out, (b, s, h, d))
         q, qs = self._rows(what, "q", q)
+        out = self._out(what, q, out, (b, s, h, d))
         k, ks = self._rows(what, "k", k)
         v, vs = (None, None) if v is None else self._rows(what, "v", v)
         self._call("wz_paged_append", q.data_ptr(), qs, k.data_ptr(), ks, N.ptr(v), vs, out.data_ptr(), h, N.ptr(q_norm),
@@ -326,7 +326,7 @@ class PagedKV:
                 raise ValueError(f"{what}: attn_sink must be float32 [{h}] on {self.device}")
             sink = attn_sink.contiguous()
         q, qs = self._rows(what, "q", q)
-        out = self._out(what, out, (b, s, h, d))
+        out = self._out(what, q, out, (b, s, h, d))
         width = table.shape[1]
         workspace = self._space(what, workspace, self.attend_tree_workspace_bytes, b, s, h, width)
         self._call("wz_paged_tree_attn", q.data_ptr(), qs, N.ptr(sink), table.data_ptr(), width, lens.data_ptr(),
@@ -362,8 +362,8 @@ class PagedKV:
         if count is not None:
             count = self._ints(what, "count", count, b)
         if out is None:
-            flat = torch.empty(b * (1 + 2 * s), dtype=torch.int32, device=self.device)
-            out = flat[:b], flat[b:b + b * s].view(b, s), flat[b + b * s:].view(b, s)
+            new = start.new_empty
+            out = new((b,)), new((b, s)), new((b, s))
         elif (self._ints(what, "out[0]", out[0], b) is not out[0] or self._nodes(what, "out[1]", out[1], b, s) is not out[1]
               or self._nodes(what, "out[2]", out[2], b, s) is not out[2]):
             raise ValueError(f"{what}: out must be contiguous")
