@@ -152,6 +152,16 @@ def test_same_result_in_every_call_and_batch(gpu, n):
             assert one[0][0] == a[0][i] and one[1][0] == a[1][i]
 
 
+@pytest.mark.parametrize("n,V", [(3, 20000), (600, 6000)])
+def test_lists_of_every_length(gpu, n, V):
+    """top-k from 1 to the most that is gathered by its count, where lists are sorted in one way or another."""
+    x, u = heads(11, n, V, torch.float32, gpu)
+    rows = min(n, 8)
+    for k in (1, 2, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1000, 1024):
+        got = kernels.sample(x, u.to(gpu), temperature=3.0, top_k=k)
+        check(x[:rows], u[:rows], [y[:rows] for y in got], 3.0, k)
+
+
 def test_long_rows(gpu):
     """A row of 2^21 logits, and its top half alone."""
     g = torch.Generator().manual_seed(1)

@@ -10,6 +10,7 @@ import torch
 
 from oracle import paged as op
 from oracle import sampling as osm
+from tests.launch_recorder import record
 from tests.test_paged import I3, cache, err
 from wanferenz_amd import _native as N
 from wanferenz_amd import kernels
@@ -171,3 +172,43 @@ def test_plain_sample_filters():
     assert osm.sample(row, 0.99, min_p=0.5)[0] == 3 and osm.sample(row, 0.99, temperature=0)[0] == 1
     assert osm.sample([np.nan, -np.inf], 0.5)[:2] == (-1, 0.0)
     assert osm.sample([np.inf, 3.0, np.inf], 0.6)[:2] == (2, 0.5)
+
+
+# ---- which kernels a call takes, on a recording HIP runtime of 256 compute units ----
+
+P, BIG = 1 << 20, 1 << 40
+
+
+def launches(tmp_path, *call):
+    _, events = record(tmp_path, [call])
+    return [(e["name"].split("(")[0].split("wz::")[1], e["grid"], e["block"], e["bytes"]) for e in events if e["kind"] == "launch"]
+
+
+def raw(c):
+    return bytes(ctypes.string_at(ctypes.byref(c), ctypes.sizeof(c)))
+
+
+@pytest.mark.parametrize("S,g,D,shared,kernel", [
+    (4, 4, 128, False, "paged_attn_kernel<128, false, false, 1, 1, true>"),
+    (16, 4, 128, False, "paged_attn_kernel<128, false, false, 2, 2, true>"),
+    (13, 5, 128, False, "paged_wide_kernel<128, false, false, 4>"), (16, 8, 128, False, "paged_wide_kernel<128, false, false, 4>"),
+    (43, 3, 128, False, "paged_wide_kernel<128, false, false, 8>"), (64, 16, 128, True, "paged_wide_kernel<128, false, true, 8>"),
+    (64, 16, 64, False, "paged_wide_kernel<64, false, false, 4>"), (64, 1, 64, False, "paged_attn_kernel<64, false, false, 2, 2, true>"),
+    (33, 4, 256, False, "paged_attn_kernel<256, false, false, 2, 2, true>"),
+    (8, 64, 512, True, "paged_latent_kernel<false, 4, true, true>")])
+def test_tree_routes(tmp_path, S, g, D, shared, kernel):
+    c = cache(k=P, v=None if shared else P, heads=1, dim=D)
+    got = launches(tmp_path, "wz_paged_tree_attn", raw(c), P, raw(I3(0, 0, D)), None, P, 100, P, P, None, P, 4, S, g, 0.1, P, BIG, None)
+    assert [x[0] for x in got][0] == kernel and "join" in got[1][0] and len(got) == 2
+    assert got[0][3] * max(1, 512 // got[0][2] if "wide" in kernel else 1) <= 160 * 1024
+
+
+@pytest.mark.parametrize("n,V,greedy,names", [
+    (1, 4096, False, ["sample_kernel", "sample_dense_kernel"]), (1, 4097, False, ["sample_top_kernel", "sample_histogram_kernel", "sample_pick_kernel"]),
+    (64, 131072, False, ["sample_top_kernel", "sample_histogram_kernel", "sample_pick_kernel"]),
+    (64, 131072, True, ["sample_top_kernel", "sample_pick_kernel"]), (512, 100003, True, ["sample_kernel"]),
+    (257, 100003, False, ["sample_kernel", "sample_dense_kernel"])])
+def test_sample_routes(tmp_path, n, V, greedy, names):
+    got = launches(tmp_path, "wz_sample", P, 0, V, P, None, 0.0 if greedy else 1.0, None, 0, None, 1.0, None, 0.0, P, P, n, V, P, BIG,
+                   None)
+    assert [x[0].split("<")[0] for x in got] == names

@@ -48,6 +48,8 @@ struct alignas(16) SampleSpace {
   uint32_t count[kSampleBins];
   SampleBins bins;
   uint32_t listed, done;  // tokens in the list, workgroups that have put in what they have
+  float top;              // the row's largest logit, and its first place
+  int32_t first;
 };
 
 struct SampleArgs {
@@ -251,10 +253,13 @@ __device__ __forceinline__ T sample_scan(T x, T* s_wave, T* total) {
   return sample_over_waves(x, in, s_wave, total);
 }
 
+constexpr int kSampleRanked = 512;  // tokens of a list that are sorted by counting; no more than a workgroup's threads
+
 struct SampleShared {
   uint32_t count[kSampleBins];  // of each bin, then of the bins before it
   u64 mass[kSampleBins];
   u64 list[kSampleList];        // key << 32 | ~index: descending is the row's order
+  int rank[kSampleRanked];
   u64 wave64[16];
   float wavef[16];
   uint32_t wave32[16];
@@ -306,17 +311,24 @@ __device__ __forceinline__ void sample_prefix(SampleShared& s, uint32_t* tokens,
   __syncthreads();
 }
 
-// Sorts the list, descending.  A short one by each token's rank, which its thread counts.  Else to a power of two of places
-// (zeros behind), a pair of places a thread: pairs up to 64 apart stay with one wave, which waits for nobody.
-constexpr int kSampleRanked = 128;
+// Sorts the list, descending.  A short one by each token's rank: the threads that have the same token count in a part of the list
+// each (200 tokens 2 us; sorted 9).  Else to a power of two of places (zeros behind), a pair of places a thread: pairs up to
+// 64 apart stay with one wave, which waits for nobody.
 __device__ __forceinline__ void sample_sort(SampleShared& s, int n) {
   if (n <= kSampleRanked) {
-    const u64 x = s.list[min(int(threadIdx.x), n - 1) & (kSampleList - 1)];
+    int places = 64;
+    while (places < n) places <<= 1;
+    const int parts = blockDim.x / places, i = threadIdx.x & (places - 1), part = threadIdx.x / places;
+    const int share = (n + parts - 1) / parts, j1 = min((part + 1) * share, n);
+    const u64 x = s.list[max(min(i, n - 1), 0)];
     int rank = 0;
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) rank += s.list[i] > x;
+    for (int j = part * share; j < j1; ++j) rank += s.list[j] > x;
+    if (part == 0) s.rank[i] = 0;
     __syncthreads();
-    if (int(threadIdx.x) < n) s.list[rank] = x;
+    if (i < n && rank) atomicAdd(&s.rank[i], rank);
+    __syncthreads();
+    if (int(threadIdx.x) < n) s.list[s.rank[i]] = x;
     __syncthreads();
     return;
   }
@@ -777,7 +789,8 @@ __device__ __forceinline__ float sample_row_top(const SampleArgs& a, int64_t row
   int at = 0x7FFFFFFF;
   for (int c = lane; c < a.chunks; c += 64) {
     const float x = a.top[row * a.chunks + c];
-    at = x > top ? a.first[row * a.chunks + c] : at;
+    const int i = a.first[row * a.chunks + c];
+    at = x > top ? i : at;
     top = fmaxf(top, x);
   }
 #pragma unroll 1
@@ -799,11 +812,15 @@ __global__ __launch_bounds__(kSampleShare, 8) void sample_histogram_kernel(Sampl
   const SampleRow r = sample_row(a, row);
   int first;
   const float top = sample_row_top(a, row, &first);
+  SampleSpace& z = a.space[row];
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    z.top = top;
+    z.first = first;
+  }
   if (!is_finite_f32(top) || !(r.t > 0.0f)) return;
   const SampleScale sc(top, r, s.table);
   sample_clear(s);
   sample_histogram<BF16>(a, row, begin, end, r, sc, s);
-  SampleSpace& z = a.space[row];
   for (int i = threadIdx.x; i < kSampleBins; i += blockDim.x) {
     if (s.count[i]) atomicAdd(&z.count[i], s.count[i]);
     if (s.mass[i]) atomicAdd(&z.mass[i], s.mass[i]);
@@ -836,9 +853,12 @@ __global__ __launch_bounds__(kSampleShare, 4) void sample_pick_kernel(SampleArgs
   __shared__ SampleShared s;
   const int64_t row = blockIdx.y;
   const int begin = blockIdx.x * a.chunk, end = min(begin + a.chunk, a.V);
+  SampleSpace& z = a.space[row];
   const SampleRow r = sample_row(a, row);
-  int first;
-  const float top = sample_row_top(a, row, &first);
+  const SampleBins g = z.bins;  // (of no meaning where the histogram's launch had nothing to do)
+  float top = z.top;
+  int first = z.first;
+  if (!a.t && !(a.t1 > 0.0f)) top = sample_row_top(a, row, &first);  // there was none
   if (top == -INFINITY || !(r.t > 0.0f)) {
     if (blockIdx.x == 0) sample_plain(a, row, r, top, first);
     return;
@@ -850,8 +870,6 @@ __global__ __launch_bounds__(kSampleShare, 4) void sample_pick_kernel(SampleArgs
     if (blockIdx.x == 0) sample_dense<BF16>(a, row, r, sc, s);
     return;
   }
-  SampleSpace& z = a.space[row];
-  const SampleBins g = z.bins;
   sample_gather<BF16>(a, row, begin, end, r, sc, g, s);
   const int mine = int(s.listed);
   if (threadIdx.x == 0 && mine > 0)
