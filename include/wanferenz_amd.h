@@ -420,8 +420,8 @@ int wz_paged_attn(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q
  * x / sqrt(mean(x^2) + eps) * norm (float32 [head_dim]; NULL: as it is), then its dims
  * [offset, offset + rotary) are turned by the token's position, pairs (a, b) to
  * (a c - b s, a s + b c) with (c, s) = freqs[position][pair] (float32 [turns, rotary / 2, 2],
- * cos and sin: torch.view_as_real of freqs_cis; a position outside [0, turns) turns by
- * NaN).  A pair is dims 2 i and 2 i + 1 of the rotary part (the reference's rotation,
+ * cos and sin: torch.view_as_real of freqs_cis, turns >= 1; a position outside [0, turns)
+ * turns by NaN).  A pair is dims 2 i and 2 i + 1 of the rotary part (the reference's rotation,
  * architecture.py:611-672), or with `halves` i and i + rotary / 2.  All of it in
  * 32 bits, rounded once.  q goes to q_out [B, S, H, head_dim] bf16 (dense; q itself where q is
  * dense, else over no input), k and v into their pages as wz_paged_kv_write puts them

@@ -39,7 +39,7 @@ def heads(seed, n, V, dtype, gpu):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [1, 2, 3, 7, 64, 1000, 4097, 50001])
+@pytest.mark.parametrize("V", [1, 2, 3, 7, 64, 1000, 4097, 32768, 50001])
 @pytest.mark.parametrize("t,k,p,m", [(1.0, 0, 1.0, 0.0), (0.7, 50, 0.9, 0.0), (1.3, 0, 0.95, 0.0), (0.9, 0, 1.0, 0.05),
                                      (1.0, 1, 1.0, 0.0), (0.0, 5, 0.5, 0.1), (1.1, 2000, 0.8, 0.01), (0.5, 1024, 1.0, 0.0),
                                      (2.0, 1025, 0.99, 0.0)])
@@ -105,6 +105,33 @@ def test_values_that_are_not_finite(gpu):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_rows_that_are_not_finite(gpu, dtype):
+    """Rows that several workgroups share: nothing to choose from, an infinity or many, ties of the largest over all
+    parts of a row, a NaN beside each."""
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(9, 40001, generator=g)
+    x[0], x[1], x[2] = nan, -inf, nan
+    x[2, 33333] = 1.5
+    x[3, 17000] = inf
+    x[4, ::97] = inf
+    x[5, ::101] = 9.0
+    x[6, ::2] = nan
+    x[7] = -3e38
+    x[8] = 0.0
+    x[3:6, 5] = nan
+    x, u = x.to(dtype), torch.rand(9, generator=g)
+    for args in (dict(), dict(top_k=7), dict(top_p=0.5), dict(min_p=0.2), dict(temperature=0.0), dict(top_k=3000, top_p=0.9)):
+        got = kernels.sample(x.to(gpu), u.to(gpu), **args)
+        check(x, u, got, args.get("temperature", 1.0), args.get("top_k", 0), args.get("top_p", 1.0), args.get("min_p", 0.0))
+        assert got[0].tolist()[:4] == [-1, -1, 33333, 17000]
+    mixed = torch.tensor([1.0, 0, 1, 0, 0, 0, 0, 0, 1])
+    got = kernels.sample(x.to(gpu), u.to(gpu), temperature=mixed.to(gpu))
+    check(x, u, got, mixed)
+    assert got[0].tolist()[4:6] == [0, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_parameters_of_each_row(gpu, dtype):
     n, V = 70, 2003
     x, u = heads(5, n, V, dtype, gpu)
@@ -139,7 +166,7 @@ def test_rows_at_any_stride_and_alignment(gpu, dtype):
 @pytest.mark.parametrize("n", [1, 2, 5, 300])
 def test_same_result_in_every_call_and_batch(gpu, n):
     """A row's token depends on the row alone, and is the same in every call."""
-    V = 33333
+    V = 33333  # shared by several workgroups up to 128 rows
     x, u = heads(3, n, V, torch.float32, gpu)
     u = u.to(gpu)
     first = [kernels.sample(x, u, top_p=p, top_k=k) for p, k in ((0.9, 0), (1.0, 0), (0.9, 40))]
@@ -152,7 +179,7 @@ def test_same_result_in_every_call_and_batch(gpu, n):
             assert one[0][0] == a[0][i] and one[1][0] == a[1][i]
 
 
-@pytest.mark.parametrize("n,V", [(3, 20000), (600, 6000)])
+@pytest.mark.parametrize("n,V", [(3, 40000), (600, 6000)])
 def test_lists_of_every_length(gpu, n, V):
     """top-k from 1 to the most that is gathered by its count, where lists are sorted in one way or another."""
     x, u = heads(11, n, V, torch.float32, gpu)

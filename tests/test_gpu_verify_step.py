@@ -131,7 +131,7 @@ def test_captured_step_replays(gpu, rows):
     """The four calls captured once and replayed with other tokens, trees, lengths and numbers, with eager calls and
     synchronisations between, against the same calls made eagerly."""
     B, S, H, HK, D = (2, 3, 8, 2, 64) if rows == 6 else (30, 20, 8, 2, 64)
-    V = 9000 if rows == 6 else 300  # few long rows are shared by workgroups
+    V = 40000 if rows == 6 else 300  # few long rows are shared by workgroups
     L, E = (Loop(gpu, 7, B, S, H, HK, D, torch.bfloat16, False, V=V) for _ in range(2))
     rng = np.random.default_rng(7)
 
@@ -167,14 +167,14 @@ def test_captured_step_replays(gpu, rows):
 
 def test_two_streams_at_once(gpu):
     """Two loops on streams of their own, without a wait between them, each with its own workspaces, give what they give alone."""
-    loops = [Loop(gpu, 20 + i, 4, 12, 16, 2, 128, torch.bfloat16, False, V=20000) for i in range(2)]
-    alone = [Loop(gpu, 20 + i, 4, 12, 16, 2, 128, torch.bfloat16, False, V=20000) for i in range(2)]
+    loops = [Loop(gpu, 20 + i, 4, 12, 16, 2, 128, torch.bfloat16, False, V=40000) for i in range(2)]
+    alone = [Loop(gpu, 20 + i, 4, 12, 16, 2, 128, torch.bfloat16, False, V=40000) for i in range(2)]
     rng = np.random.default_rng(1)
     args = []
     for _ in range(2):
         parent, depth = trees(rng, 4, 12)
         args.append([torch.tensor(x, dtype=torch.int32, device=gpu) for x in
-                     (rng.integers(0, 20000, (4, 12)), parent, depth, [0, 40, 99, 120])] + [torch.rand(4, 12, device=gpu)])
+                     (rng.integers(0, 40000, (4, 12)), parent, depth, [0, 40, 99, 120])] + [torch.rand(4, 12, device=gpu)])
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     got = []
@@ -192,19 +192,19 @@ def test_two_streams_at_once(gpu):
 
 
 def test_calls_with_workspace_and_out_allocate_nothing(gpu):
-    L = Loop(gpu, 3, 2, 9, 16, 2, 64, torch.bfloat16, False, V=30000)
+    L = Loop(gpu, 3, 2, 9, 16, 2, 64, torch.bfloat16, False, V=40000)
     rng = np.random.default_rng(3)
     parent, depth = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in trees(rng, 2, 9))
-    tokens = torch.tensor(rng.integers(0, 30000, (2, 9)), dtype=torch.int32, device=gpu)
+    tokens = torch.tensor(rng.integers(0, 40000, (2, 9)), dtype=torch.int32, device=gpu)
     lens = torch.tensor([5, 70], dtype=torch.int32, device=gpu)
     u = torch.rand(18, device=gpu)
-    logits = torch.randn(18, 30000, device=gpu)
+    logits = torch.randn(18, 40000, device=gpu)
     q, k, v = L.split(tokens)
     pos, total = lens[:, None] + depth, lens + 9
     out = torch.empty(2, 9, 16, 64, dtype=torch.bfloat16, device=gpu)
     heard = torch.empty_like(out)
     ws = torch.empty(L.cache.attend_tree_workspace_bytes(2, 9, 16, L.table.shape[1]), dtype=torch.uint8, device=gpu)
-    sw = torch.empty(kernels.sample_workspace_bytes(18, 30000), dtype=torch.uint8, device=gpu)
+    sw = torch.empty(kernels.sample_workspace_bytes(18, 40000), dtype=torch.uint8, device=gpu)
     so = torch.empty(18, dtype=torch.int32, device=gpu), torch.empty(18, device=gpu)
     ao = lens.clone(), tokens.clone(), tokens.clone()
     torch.cuda.synchronize()
@@ -223,6 +223,6 @@ def test_calls_with_workspace_and_out_allocate_nothing(gpu):
     # what a smaller call left in the workspace does not count
     want = kernels.sample(logits[:3], u[:3], top_p=0.9)
     kernels.sample(logits, u, temperature=0.0, workspace=sw)
-    ws3 = sw if sw.numel() >= kernels.sample_workspace_bytes(3, 30000) else None
+    ws3 = sw if sw.numel() >= kernels.sample_workspace_bytes(3, 40000) else None
     got = kernels.sample(logits[:3], u[:3], top_p=0.9, workspace=ws3)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
