@@ -31,6 +31,8 @@ def run(gpu, cache, tab, lens, parent, q, scale, **more):
     return cache.attend_tree(q, tab, i32(lens), torch.from_numpy(parent).to(gpu), scale, **more)
 
 
+MANY = 9000  # pages of a table that a call cannot take for a small one
+
 LAYOUTS = [  # HK, g, D, shared
     (2, 4, 128, False), (8, 1, 128, False), (1, 16, 64, False), (2, 3, 64, False), (2, 5, 256, False),
     (1, 8, 128, True), (1, 5, 256, True), (1, 16, 512, True), (1, 20, 512, True),
@@ -40,10 +42,12 @@ LAYOUTS = [  # HK, g, D, shared
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
 @pytest.mark.parametrize("HK,g,D,shared", LAYOUTS)
 @pytest.mark.parametrize("S", [1, 7, 33])
-def test_layouts(gpu, S, HK, g, D, shared, dtype):
-    """Head layouts and widths, ragged prefixes among them none, trees smaller and larger than a tile."""
+@pytest.mark.parametrize("width", [None, MANY])
+def test_layouts(gpu, width, S, HK, g, D, shared, dtype):
+    """Head layouts and widths, ragged prefixes among them none, trees smaller and larger than a tile; tables as wide as
+    the sequences, whose rows go 16 at a time, and much wider ones, whose rows go together."""
     lens = [S + n for n in (0, 1, 16, 31, 100, 300)]
-    cache, vals, tab, table = make(gpu, D + HK + g, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared)
+    cache, vals, tab, table = make(gpu, D + HK + g, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared, width=width)
     q, qd = queries(gpu, g, len(lens), S, HK * g, D, strided=True)
     parent = trees(S, len(lens), S)
     o = run(gpu, cache, tab, lens, parent, q, D ** -0.5)
@@ -52,12 +56,13 @@ def test_layouts(gpu, S, HK, g, D, shared, dtype):
 
 @pytest.mark.parametrize("kind", ["chain", "star", "random", "forest"])
 @pytest.mark.parametrize("S,page", [(2, 16), (16, 64), (63, 32), (64, 1024)])
-def test_shapes_of_trees(gpu, S, page, kind):
+@pytest.mark.parametrize("width", [None, MANY])
+def test_shapes_of_trees(gpu, width, S, page, kind):
     """Chains, stars, forests whose roots hang on the prefix; more rows than a unit; a sink; lengths at and off the
     tiles' borders; sequences that hold less than their tree."""
     lens = [S, 0, 1, S + 31, 128, 129, 257, 700]
     HK, g, D = 2, 8, 64
-    cache, vals, tab, table = make(gpu, S + page, lens, HK=HK, D=D, page=page)
+    cache, vals, tab, table = make(gpu, S + page, lens, HK=HK, D=D, page=page, width=width)
     q, qd = queries(gpu, S, len(lens), S, HK * g, D, scale=1.5)
     sink = torch.linspace(-3, 4, HK * g)
     parent = trees(S + page, len(lens), S, kind)
@@ -88,11 +93,12 @@ def test_parents_in_any_order_and_rings(gpu):
 
 @pytest.mark.parametrize("HK,g,D,shared,n", [(1, 4, 128, False, 4000), (1, 40, 64, False, 1500), (1, 16, 512, True, 900)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
-def test_padded_batches_over_many_workgroups(gpu, HK, g, D, shared, n, dtype):
+@pytest.mark.parametrize("width", [None, MANY])
+def test_padded_batches_over_many_workgroups(gpu, width, HK, g, D, shared, n, dtype):
     """Sequences with fewer nodes than the batch's, none and more than it; a long one that many workgroups share."""
     S, count = 21, [21, 1, 0, 8, 99, -3]
     lens = [n, 40, 55, 8, 64, 33]
-    cache, vals, tab, table = make(gpu, 11, lens, HK=HK, D=D, page=64, dtype=dtype, shared=shared)
+    cache, vals, tab, table = make(gpu, 11, lens, HK=HK, D=D, page=64, dtype=dtype, shared=shared, width=width)
     q, qd = queries(gpu, 12, len(lens), S, HK * g, D, scale=2.0)
     parent = trees(5, len(lens), S)
     out = torch.full((len(lens), S, HK * g, D), float("nan"), dtype=torch.bfloat16, device=gpu)
@@ -105,10 +111,11 @@ def test_padded_batches_over_many_workgroups(gpu, HK, g, D, shared, n, dtype):
 @pytest.mark.parametrize("HK,g,D,shared", [(2, 2, 64, False), (1, 16, 128, False), (1, 24, 128, False), (2, 8, 256, False),
                                            (1, 6, 128, True), (1, 16, 512, True), (1, 64, 512, True)])
 @pytest.mark.parametrize("n", [6, 40, 600])
-def test_a_node_takes_nothing_from_branches_it_does_not_see(gpu, n, HK, g, D, shared, dtype):
+@pytest.mark.parametrize("width", [None, MANY])
+def test_a_node_takes_nothing_from_branches_it_does_not_see(gpu, width, n, HK, g, D, shared, dtype):
     """NaN in the K of one node and the V of another: every node that has neither above it stays as it was."""
     S, lens = 6, [n, n + 27]
-    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared)
+    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared, width=width)
     q, qd = queries(gpu, 4, 2, S, HK * g, D)
     parent = np.array([[-1, 0, 0, 1, 2, 2], [-1, 0, 0, 1, 2, 2]], dtype=np.int32)
     ref = op.attend_tree(vals, qd, table, lens, parent, D ** -0.5)
@@ -219,7 +226,7 @@ def test_many_rows_of_padded_trees(gpu, HK, g, S, D, shared, dtype):
     count = [S, 0, 1, S // 3, S - 1, S, 2 * S, -1, S // 2]
     pre = [0, 70, 63, 64, 128, 3000, 17, 30, 700]
     lens = [min(max(c, 0), S) + p for c, p in zip(count, pre)]
-    cache, vals, tab, table = make(gpu, S + g, lens, HK=HK, D=D, page=16 if S % 2 else 32, dtype=dtype, shared=shared)
+    cache, vals, tab, table = make(gpu, S + g, lens, HK=HK, D=D, page=16 if S % 2 else 32, dtype=dtype, shared=shared, width=MANY)
     q, qd = queries(gpu, S, len(lens), S, HK * g, D, scale=1.5, strided=True)
     parent = trees(S, len(lens), S, "forest")
     sink = torch.linspace(-2, 3, HK * g)
@@ -236,7 +243,7 @@ def test_many_rows_of_padded_trees(gpu, HK, g, S, D, shared, dtype):
 def test_many_rows_take_nothing_from_branches_they_do_not_see(gpu, n, HK, g, S, D, shared, dtype):
     """NaN in the K of one node and the V of others, over two tiles of the tree: rows without them above stay as they were."""
     lens = [S + n, S + n + 37]
-    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared)
+    cache, vals, tab, table = make(gpu, 13, lens, HK=HK, D=D, page=16, dtype=dtype, shared=shared, width=MANY)
     q, qd = queries(gpu, 4, 2, S, HK * g, D)
     parent = trees(3, 2, S)
     ref = op.attend_tree(vals, qd, table, lens, parent, D ** -0.5)
@@ -258,7 +265,7 @@ def test_many_rows_take_nothing_from_branches_they_do_not_see(gpu, n, HK, g, S, 
 def test_many_rows_of_more_units_than_workers(gpu, HK, g, S, D, shared):
     B = 560
     lens = [S + (7 * b) % 90 for b in range(B)]
-    cache, vals, tab, table = make(gpu, 21, lens, HK=HK, D=D, page=16)
+    cache, vals, tab, table = make(gpu, 21, lens, HK=HK, D=D, page=16, width=400)
     q, qd = queries(gpu, 21, B, S, HK * g, D)
     parent = trees(21, B, S)
     o = run(gpu, cache, tab, lens, parent, q, D ** -0.5)
@@ -273,7 +280,7 @@ def test_many_rows_of_more_units_than_workers(gpu, HK, g, S, D, shared):
 @pytest.mark.parametrize("g,S,D", [(4, 3, 64), (8, 20, 64), (8, 30, 128)])
 def test_scales_of_any_sign(gpu, g, S, D, scale):
     lens = [S + 5, S + 200]
-    cache, vals, tab, table = make(gpu, 31, lens, HK=1, D=D, page=16)
+    cache, vals, tab, table = make(gpu, 31, lens, HK=1, D=D, page=16, width=MANY)
     q, qd = queries(gpu, 31, 2, S, g, D)
     parent = trees(31, 2, S)
     o = run(gpu, cache, tab, lens, parent, q, scale)
@@ -285,7 +292,7 @@ def test_scales_of_any_sign(gpu, g, S, D, scale):
 def test_many_rows_whose_maximum_moves(gpu, g, S, D):
     """K that grows along the sequence, so that the maximum moves far at many tiles."""
     lens = [S + 900, S + 333]
-    cache, vals, tab, table = make(gpu, 5, lens, HK=1, D=D, page=32)
+    cache, vals, tab, table = make(gpu, 5, lens, HK=1, D=D, page=32, width=MANY)
     grow = torch.ones(cache.pages, 1, 32, 1)
     for b, n in enumerate(lens):
         for p in range(-(-n // 32)):

@@ -199,9 +199,22 @@ def raw(c):
     (8, 64, 512, True, "paged_latent_kernel<false, 4, true, true>")])
 def test_tree_routes(tmp_path, S, g, D, shared, kernel):
     c = cache(k=P, v=None if shared else P, heads=1, dim=D)
-    got = launches(tmp_path, "wz_paged_tree_attn", raw(c), P, raw(I3(0, 0, D)), None, P, 100, P, P, None, P, 4, S, g, 0.1, P, BIG, None)
+    got = launches(tmp_path, "wz_paged_tree_attn", raw(c), P, raw(I3(0, 0, D)), None, P, 5000, P, P, None, P, 4, S, g, 0.1, P, BIG, None)
     assert [x[0] for x in got][0] == kernel and "join" in got[1][0] and len(got) == 2
     assert got[0][3] * max(1, 512 // got[0][2] if "wide" in kernel else 1) <= 160 * 1024
+
+
+@pytest.mark.parametrize("width,rows", [(4, 16), (378, 16), (380, 64), (5000, 64)])
+def test_tables_of_few_slots_take_units_of_16_rows(tmp_path, width, rows):
+    """64 rows on 2 KV heads of 4 sequences: 32 units of 16 rows, width / 2 + 3 tiles each, up to 24 a compute unit; the workspace
+    holds the partials of the kernel that runs."""
+    c = cache(k=P, v=P, heads=2, dim=128, page=16)
+    assert (32 * (width // 2 + 3) <= 24 * 256) == (rows == 16)
+    got = launches(tmp_path, "wz_paged_tree_attn", raw(c), P, raw(I3(0, 0, 128)), None, P, width, P, P, None, P, 4, 16, 8, 0.1, P,
+                   BIG, None)
+    assert got[0][0] == f"paged_attn_kernel<128, false, false, {'1, 1' if rows == 16 else '2, 2'}, true>"
+    need = N.lib().wz_paged_tree_attn_workspace_bytes(ctypes.byref(c), 4, 16, 8, width)
+    assert need == got[0][1] * (2 * 4 * (2 * rows + rows * 128) + 16)
 
 
 @pytest.mark.parametrize("n,V,greedy,names", [

@@ -960,6 +960,16 @@ int paged_attn_join(const PagedAttnArgs& a, hipStream_t stream) {
   return check_launch("paged_attn_weigh");
 }
 
+// Whether a tree's units of 16 rows are so few, whatever the lengths that its table can hold, that there are six tiles a worker at
+// most.  The time is a worker's way through its tiles then, and shorter with fewer rows: us with the kernel of the rows / with 16
+// rows a unit (join in both), heads of 128: 1 x 1015 tokens, 64 rows on 8 KV heads 17.4 / 15.9, 1 x 4000 22.9 / 18.9, 8 x 300 26.1 /
+// 19.2, 1 x 1000 with 256 rows 27.1 / 25.4, with 512 rows on 300 24.8 / 22.2; heads of 64: 1 x 3000, 192 rows on 8 20.9 / 20.2, 1 x
+// 6000, 512 rows on one 16.3 / 18.5.
+static inline bool paged_few(const PagedAttnArgs& a) {
+  const int64_t R = a.S * (a.H / a.c.heads);
+  return a.B * int64_t(a.c.heads) * ((R + 15) / 16) * (a.capacity / kPagedTile + kPagedStart) <= 24 * int64_t(cu_count());
+}
+
 // The kernel of R rows a KV head: 16, 32 or 64 rows a unit.  With 4 rows 16 x 8000 tokens take 94.5 / 97.6 / 121.7 us with
 // each, 48 x 9001 e4m3 tokens of 128 with 8 rows 167 / 214 / 400.
 template <int D, bool FP8, bool SHARED, int RT, int RH, bool TREE>
@@ -986,6 +996,8 @@ int paged_attn_launch_rt(PagedAttnArgs a, bool ask, int* workers, hipStream_t st
 template <int D, bool FP8, bool SHARED, bool TREE>
 int paged_attn_launch_d(const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
   const int R = a.S * (a.H / a.c.heads);
+  if constexpr (TREE)
+    if (paged_few(a)) return paged_attn_launch_rt<D, FP8, SHARED, 1, 1, TREE>(a, ask, workers, stream);
   if (R <= 16) return paged_attn_launch_rt<D, FP8, SHARED, 1, 1, TREE>(a, ask, workers, stream);
   if (R <= 32) return paged_attn_launch_rt<D, FP8, SHARED, 2, 1, TREE>(a, ask, workers, stream);
   return paged_attn_launch_rt<D, FP8, SHARED, 2, 2, TREE>(a, ask, workers, stream);

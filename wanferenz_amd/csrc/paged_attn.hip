@@ -26,8 +26,10 @@ static PagedAttnSizes paged_attn_sizes(const wz_paged_kv* c, int64_t B, int64_t 
   a.c.heads = c->kv_heads;
   a.c.shared = c->v == nullptr;
   a.c.dtype = c->dtype;
+  a.B = int(B);
   a.S = int(S);
   a.H = int(H);
+  a.capacity = width * c->page_size;
   int workers = 0;
   const int64_t rows = paged_attn_any(c->head_dim, tree, a, true, &workers, nullptr);
   z.part = 2 * workers * paged_slot(int(rows), c->head_dim);

@@ -527,7 +527,7 @@ int paged_wide(const PagedAttnArgs& a, bool ask, int* workers, hipStream_t strea
 
 template <bool FP8>
 int paged_tree_launch(int D, const PagedAttnArgs& a, bool ask, int* workers, hipStream_t stream) {
-  if (a.S * (a.H / a.c.heads) > 64) {
+  if (a.S * (a.H / a.c.heads) > 64 && !paged_few(a)) {
     if (D == 64 && !a.c.shared) return paged_wide<64, FP8, false>(a, ask, workers, stream);
     if (D == 128 && a.c.shared) return paged_wide<128, FP8, true>(a, ask, workers, stream);
     if (D == 128) return paged_wide<128, FP8, false>(a, ask, workers, stream);
