@@ -24,7 +24,7 @@ constexpr int kSampleThreads = 1024;
 constexpr int64_t kSampleMaxV = 1 << 21;  // 2^21 weights of 2^42 fit 64 bits
 constexpr int kSampleHead = 1024;         // top-k up to here: the first bins are gathered, and only their tokens get weights
 
-constexpr int kSampleSteps = 64;          // of the table of 2^(42 - j / 64)
+constexpr int kSampleSteps = 256;         // of the table of 2^(42 - j / 256)
 constexpr int kSampleChunk = 4096;        // logits that a workgroup takes at least where several share a row
 
 constexpr int kSampleShare = 512;         // threads of a workgroup there
@@ -87,7 +87,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int64_t row
   return r;
 }
 
-// 2^(42 - j / 64), by Taylor's polynomial of e^y.
+// 2^(42 - j / 256), by Taylor's polynomial of e^y.
 struct SampleTable {
   double step[kSampleSteps];
   constexpr SampleTable() : step() {
@@ -101,19 +101,19 @@ struct SampleTable {
 };
 __constant__ constexpr SampleTable kSampleTable;
 
-// 2^-(x / 64) for 0 <= x < 64 * 44 in multiples of 2^-42: 2^-n from the exponent, 2^-(j / 64) from the table and e^y for what is
-// left, |y| <= ln(2) / 128, by Taylor's polynomial (the next term is 4e-14); then rounded by an addition that
-// leaves no place for the fraction.
+// 2^-(x / 256) for 0 <= x < 256 * 44 in multiples of 2^-42: 2^-n from the exponent, 2^-(j / 256) from the table and e^(r c) for
+// what is left, c = ln(2) / 256 and |r| <= 1 / 2, by Taylor's polynomial (the next term is 1.4e-13); then rounded by an
+// addition that leaves no place for the fraction.
 __device__ __forceinline__ uint64_t sample_weight(double x, const double* table) {
+  constexpr double c = 0.69314718055994530942 / kSampleSteps;
   const double t = x + 0x1.8p52;  // the nearest whole number stands in its low bits
   const int k = __double2loint(t);
-  const double y = ((t - 0x1.8p52) - x) * (0.69314718055994530942 / kSampleSteps);
+  const double r = (t - 0x1.8p52) - x;
   const double step = table[k & (kSampleSteps - 1)];
-  const double scaled = __hiloint2double(__double2hiint(step) - ((k >> 6) << 20), __double2loint(step));
-  double e = fma(y, 1.0 / 24.0, 1.0 / 6.0);
-  e = fma(e, y, 0.5);
-  e = fma(e, y, 1.0);
-  e = fma(e, y, 1.0);
+  const double scaled = __hiloint2double(__double2hiint(step) - ((k >> 8) << 20), __double2loint(step));
+  double e = fma(r, c * c * c / 6.0, c * c / 2.0);
+  e = fma(e, r, c);
+  e = fma(e, r, 1.0);
   return uint64_t(__double_as_longlong(fma(e, scaled, 0x1p52)) & ((1ll << 52) - 1));
 }
 
@@ -121,7 +121,7 @@ __device__ __forceinline__ uint64_t sample_weight(double x, const double* table)
 struct SampleScale {
   float top;     // the largest logit
   float step;    // bins a logit
-  double steps;  // steps of 2^(-1 / 64) a logit
+  double steps;  // steps of 2^(-1 / 256) a logit
   uint64_t least;  // the smallest weight that min-p keeps
   const double* table;
   __device__ SampleScale(float top, const SampleRow& r, const double* table) : top(top), table(table) {
@@ -157,31 +157,26 @@ __device__ __forceinline__ float sample_unkey(uint32_t k) {
 // what stands outside is -inf.
 template <bool BF16, typename F>
 __device__ __forceinline__ void sample_each(const SampleArgs& a, int64_t row, int begin, int end, F&& f) {
-  constexpr int ESZ = BF16 ? 2 : 4, N = 16 / ESZ, DEEP = 2;
+  constexpr int ESZ = BF16 ? 2 : 4, N = 16 / ESZ;
   const char* const base = static_cast<const char*>(a.logits) + row * a.stride * ESZ;
   const int skew = int((reinterpret_cast<uintptr_t>(base) + int64_t(begin) * ESZ) & 15) / ESZ;
   const int first = begin - skew;  // index of the first 16-byte piece's first element
   const int pieces = (end - first + N - 1) / N;
-  auto whole = [&](int c) {
-    const int i = first + c * N;
-    return c < pieces && i >= begin && i + N <= end;
-  };
-  // the body stands here once: unrolled over the pieces it did not fit the instruction cache
-  v4i x[DEEP];
-#pragma unroll
-  for (int d = 0; d < DEEP; ++d) {
-    const int c = threadIdx.x + d * int(blockDim.x);
-    if (whole(c)) x[d] = load16(base + int64_t(first + c * N) * ESZ);
-  }
+  // pieces [w0, w0 + whole) lie inside: the first and the last need not
+  const int w0 = skew ? 1 : 0, whole = (end - first) / N - w0;
+  auto load = [&](int c) { return load16(base + int64_t(begin) * ESZ + (uint32_t(c) * 16u - uint32_t(skew * ESZ))); };
+  // the body stands here once: unrolled over the pieces it did not fit the instruction cache; the next piece is on its way
+  int c = threadIdx.x;
+  v4i next = v4i{0, 0, 0, 0};
+  if (uint32_t(c - w0) < uint32_t(max(whole, 0))) next = load(c);
 #pragma unroll 1
-  for (int c = threadIdx.x; c < pieces; c += blockDim.x) {
-    const v4i now = x[0];
-#pragma unroll
-    for (int d = 1; d < DEEP; ++d) x[d - 1] = x[d];
-    const int later = c + DEEP * int(blockDim.x), i = first + c * N;
-    if (whole(later)) x[DEEP - 1] = load16(base + int64_t(first + later * N) * ESZ);
+  for (; c < pieces; c += blockDim.x) {
+    const v4i now = next;
+    const int later = c + int(blockDim.x), i = first + c * N;
+    const bool inside = uint32_t(c - w0) < uint32_t(max(whole, 0));
+    if (uint32_t(later - w0) < uint32_t(max(whole, 0))) next = load(later);
     float l[N];
-    if (whole(c)) {
+    if (inside) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if constexpr (BF16) {
@@ -493,7 +488,7 @@ __device__ __forceinline__ void sample_clear(SampleShared& s) {
     s.count[i] = 0;
     s.mass[i] = 0;
   }
-  if (threadIdx.x < kSampleSteps) s.table[threadIdx.x] = kSampleTable.step[threadIdx.x];
+  if (int(threadIdx.x) < kSampleSteps) s.table[threadIdx.x] = kSampleTable.step[threadIdx.x];
   __syncthreads();
 }
 
@@ -864,7 +859,7 @@ __global__ __launch_bounds__(kSampleShare, 4) void sample_pick_kernel(SampleArgs
     return;
   }
   const SampleScale sc(top, r, s.table);
-  if (threadIdx.x < kSampleSteps) s.table[threadIdx.x] = kSampleTable.step[threadIdx.x];
+  if (int(threadIdx.x) < kSampleSteps) s.table[threadIdx.x] = kSampleTable.step[threadIdx.x];
   if (top == INFINITY) {
     __syncthreads();
     if (blockIdx.x == 0) sample_dense<BF16>(a, row, r, sc, s);
