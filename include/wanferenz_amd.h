@@ -479,7 +479,7 @@ int wz_paged_evict(const wz_paged_kv* cache, const int32_t* table, int64_t table
  * probs[row] = w over that sum.  temperature <= 0 takes the first token, probability 1.  NaN and -inf are never
  * taken (a row of nothing else: token -1, probability 0), +inf takes all the weight.  A
  * weight below 2^-42 of the row's largest counts as nothing.  temperature, top_k, top_p and
- * min_p are device arrays [n], or NULL for the value beside them.  Few rows are shared by several workgroups each, with
+ * min_p are device arrays [n], or NULL for the value beside them; outputs overlap no input.  Few rows are shared by several workgroups each, with
  * a workspace (its size is that of the current device; 0: none is needed; one call at a time uses it). */
 int64_t wz_sample_workspace_bytes(int64_t n, int64_t V);
 int wz_sample(const void* logits, int logits_bf16, int64_t row_stride, const float* uniform, const float* temperature,

@@ -131,6 +131,21 @@ def test_long_rows_that_are_not_finite(gpu, dtype):
     assert got[0].tolist()[4:6] == [0, 0]
 
 
+@pytest.mark.parametrize("V", [1000, 40001])
+def test_temperatures_and_logits_below_the_normal_range(gpu, V):
+    """Differences of logits that are a normal number of temperatures, and far more of them than a weight has, at the
+    smallest temperatures."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.stack([-1e-36 * torch.rand(V, generator=g), -1e-37 * torch.rand(V, generator=g),
+                     -1e-43 * torch.rand(V, generator=g), -torch.rand(V, generator=g)])
+    x[:, V // 2] = 0
+    u = torch.rand(4, generator=g)
+    for t in (1e-44, 1e-40, 1e-38, 1e-37, 3e-37, 1e-36, 1e-30):
+        for k, p, m in ((0, 1.0, 0.0), (50, 1.0, 0.0), (0, 0.9, 0.0), (2000, 0.9, 0.1)):
+            got = kernels.sample(x.to(gpu), u.to(gpu), temperature=t, top_k=k, top_p=p, min_p=m)
+            check(x, u, got, t, k, p, m)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_parameters_of_each_row(gpu, dtype):
     n, V = 70, 2003

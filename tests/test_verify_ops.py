@@ -114,6 +114,21 @@ def test_sample_refusals():
         kernels.sample(torch.zeros(1, 5), torch.zeros(1))
 
 
+def test_sample_outputs_over_inputs_are_refused():
+    places = dict(logits=1 << 20, u=16, t=32, k=48, p=64, m=80, tokens=96, probs=112)
+
+    def call(**over):
+        a = {**places, **over}
+        return N.lib().wz_sample(a["logits"], 0, 100, a["u"], a["t"], 1.0, a["k"], 0, a["p"], 1.0, a["m"], 0.0, a["tokens"],
+                                 a["probs"], 3, 100, None, 0, None)
+
+    for out in ("tokens", "probs"):
+        for name in ("u", "t", "k", "p", "m"):
+            assert call(**{out: places[name] + 8}) == -1 and "an output overlaps an input" in err(), (out, name)
+        assert call(**{out: (1 << 20) + 296 * 4}) == -1 and "an output overlaps an input" in err()
+    assert call(tokens=104) == -1 and "outputs overlap" in err()
+
+
 def test_plain_tree_of_a_chain_is_causal_attention():
     rng = np.random.default_rng(0)
     c = {"k": rng.standard_normal((5, 2, 16, 8)), "v": rng.standard_normal((5, 2, 16, 8))}
@@ -223,6 +238,7 @@ def test_tables_of_few_slots_take_units_of_16_rows(tmp_path, width, rows):
     (64, 131072, True, ["sample_top_kernel", "sample_pick_kernel"]), (512, 100003, True, ["sample_kernel"]),
     (129, 100003, False, ["sample_kernel", "sample_dense_kernel"])])
 def test_sample_routes(tmp_path, n, V, greedy, names):
-    got = launches(tmp_path, "wz_sample", P, 0, V, P, None, 0.0 if greedy else 1.0, None, 0, None, 1.0, None, 0.0, P, P, n, V, P, BIG,
-                   None)
+    u, tokens, probs = (P + (1 << 40) + i * 4096 for i in range(3))
+    got = launches(tmp_path, "wz_sample", P, 0, V, u, None, 0.0 if greedy else 1.0, None, 0, None, 1.0, None, 0.0, tokens, probs, n,
+                   V, P, BIG, None)
     assert [x[0].split("<")[0] for x in got] == names

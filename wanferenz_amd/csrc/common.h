@@ -286,6 +286,13 @@ __device__ __forceinline__ int xcd_runs(int b, int d0, int n) {
 // Error reporting (errors.hip) and optional launch timing (prof.hip).
 namespace wz {
 int set_error(int code, const char* fmt, ...);
+
+// Whether [p, p + n) and [q, q + m) bytes share any.
+inline bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return n > 0 && m > 0 && a < b + uintptr_t(m) && b < a + uintptr_t(n);
+}
+
 int check_launch(const char* what);
 int cu_count();
 constexpr int kMaxDevices = 64;  // devices of a process that per-device state is kept for

@@ -238,12 +238,6 @@ __global__ __launch_bounds__(256) void paged_accept_kernel(PagedView c, AcceptAr
   }
 }
 
-// Whether [p, p + n) and [q, q + m) bytes share any.
-static bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return n > 0 && m > 0 && a < b + uintptr_t(m) && b < a + uintptr_t(n);
-}
-
 }  // namespace wz
 
 extern "C" int wz_paged_append(const wz_paged_kv* cache, const void* q_bf16, const int64_t* q_strides, const void* k_bf16,

@@ -8,8 +8,12 @@
 // counted digit by digit instead.
 //
 // Weights are whole multiples of 2^-42 of the largest, so sums have no order and the same call gives the same token: a
-// cumulated weight is off by 2^-43 a token at most, and an exponential's own error, 2e-13 of the weight, comes from double
-// precision.  32 bits would misplace the borders of 1e5 tokens so far that one row in a thousand got a neighbour.
+// cumulated weight is off by 2^-43 a token at most, and an exponential is within 1.5e-13 of its weight, which takes
+// double precision.  32 bits would misplace the borders of 1e5 tokens so far that one row in a thousand got a neighbour.
+//
+// Its bound is the histogram: some 26 vector instructions and a 64-bit addition in LDS an element, on one of 2048 places
+// that a wave's lanes often share.  512 rows of 100003 float32 by mass (205 MB, read three times, the second and third time
+// mostly from beyond L2) take 104 to 107 us: 5.8 TB/s, the vector units three quarters busy.  One row is three launches' chains, 21 us.
 #include <algorithm>
 
 #include "common.h"
@@ -130,6 +134,8 @@ struct SampleScale {
     step = float(fmin(log2t * (double(kSampleBins) / double(kSampleRange)), 3e38));
     least = uint64_t(fmin(fmax(rint(double(r.m) * kSampleOne), 0.0), kSampleOne));
   }
+  // A temperature below 2e-37 or so, of which a bin's width has no 32-bit inverse: such rows are counted by their keys.
+  __device__ bool cold() const { return step >= 3e38f; }
   // Bin of a logit, kSampleBins for one whose weight is nothing (a NaN's among them); lower logits have higher bins.
   __device__ int bin(float l) const {
     const float x = l == top ? 0.0f : (top - l) * step;
@@ -139,7 +145,8 @@ struct SampleScale {
   __device__ int bin_finite(float l) const { return int(fminf((top - l) * step, float(kSampleBins))); }
   __device__ uint64_t weight_finite(float l) const { return sample_weight((double(top) - double(l)) * steps, table); }
   __device__ uint64_t weight(float l) const {  // of a logit with a bin
-    return l == top ? uint64_t(kSampleOne) : sample_weight((double(top) - double(l)) * steps, table);
+    return l == top ? uint64_t(kSampleOne)
+                    : sample_weight(fmin((double(top) - double(l)) * steps, double(kSampleRange + 1) * kSampleSteps), table);
   }
 };
 
@@ -248,7 +255,8 @@ __device__ __forceinline__ T sample_scan(T x, T* s_wave, T* total) {
   return sample_over_waves(x, in, s_wave, total);
 }
 
-constexpr int kSampleRanked = 512;  // tokens of a list that are sorted by counting; no more than a workgroup's threads
+constexpr int kSampleRanked = 512;  // tokens of a list that are sorted by counting
+static_assert(kSampleRanked <= kSampleShare && kSampleSteps <= kSampleShare, "a thread each");
 
 struct SampleShared {
   uint32_t count[kSampleBins];  // of each bin, then of the bins before it
@@ -710,7 +718,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_kernel(SampleArgs a)
   if (sample_plain(a, row, r, top, first)) return;
   const SampleScale sc(top, r, s.table);
   sample_clear(s);
-  if (top != INFINITY) {
+  if (top != INFINITY && !sc.cold()) {
     sample_histogram<BF16>(a, row, 0, a.V, r, sc, s);
     uint32_t tokens;
     u64 total;
@@ -814,6 +822,7 @@ __global__ __launch_bounds__(kSampleShare, 8) void sample_histogram_kernel(Sampl
   }
   if (!is_finite_f32(top) || !(r.t > 0.0f)) return;
   const SampleScale sc(top, r, s.table);
+  if (sc.cold()) return;
   sample_clear(s);
   sample_histogram<BF16>(a, row, begin, end, r, sc, s);
   for (int i = threadIdx.x; i < kSampleBins; i += blockDim.x) {
@@ -860,7 +869,7 @@ __global__ __launch_bounds__(kSampleShare, 4) void sample_pick_kernel(SampleArgs
   }
   const SampleScale sc(top, r, s.table);
   if (int(threadIdx.x) < kSampleSteps) s.table[threadIdx.x] = kSampleTable.step[threadIdx.x];
-  if (top == INFINITY) {
+  if (top == INFINITY || sc.cold()) {
     __syncthreads();
     if (blockIdx.x == 0) sample_dense<BF16>(a, row, r, sc, s);
     return;
@@ -948,6 +957,14 @@ extern "C" int wz_sample(const void* logits, int logits_bf16, int64_t row_stride
                      (long long)(workspace ? workspace_bytes : 0), (long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return set_error(WZ_EINVAL, "sample: the workspace must be 16-byte aligned");
+  const int64_t bytes = n * 4;
+  const struct { const void* p; int64_t n; } in[] = {{logits, ((n - 1) * row_stride + V) * (logits_bf16 ? 2 : 4)},
+                                                     {uniform, bytes}, {temperature, bytes}, {top_k, bytes},
+                                                     {top_p, bytes}, {min_p, bytes}};
+  for (const auto& x : in)
+    if (x.p && (overlap(tokens, bytes, x.p, x.n) || overlap(probs, bytes, x.p, x.n)))
+      return set_error(WZ_EINVAL, "sample: an output overlaps an input");
+  if (overlap(tokens, bytes, probs, bytes)) return set_error(WZ_EINVAL, "sample: the outputs overlap");
   int64_t chunk;
   a.chunks = sample_chunks(n, V, &chunk);
   a.chunk = int(chunk);

@@ -577,7 +577,7 @@ def sparse_attn_workspace_bytes(b, s, h, d, topk) -> int:
 
 def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, workspace=None):
     """One token a row: logits [n, V] float32 or bf16 (rows dense, any stride between them), ``uniform`` [n] float32 in
-    [0, 1), one random number a row -> (tokens int32 [n], probs float32 [n]), in ``out`` if given.
+    [0, 1), one random number a row -> (tokens int32 [n], probs float32 [n]), in ``out`` if given (over no input).
 
     A row's tokens stand in order of their logits, the highest first, equal ones by index, and w = exp((logit -
     highest) / temperature).  Kept are those with w >= ``min_p``, of them the ``top_k`` first (0: all), and of those the
