@@ -1,5 +1,5 @@
-"""A paged key-value cache: the write of new tokens, the attention that reads it, and the
-eviction of what attention has weighed least.
+"""A paged key-value cache: the write of new tokens, the attention that reads it, the eviction of
+what attention has weighed least, and a step that verifies drafted tokens.
 
 The reference keeps one contiguous row of KV latents per sequence
 (wanferenz/model/architecture.py:596-600) and attends to selected rows of it
@@ -15,6 +15,13 @@ A decode loop::
     cache.write(k, v, table, lens, position=pos)        # the step's new tokens
     o = cache.attend(q, table, lens + 1, scale, accumulate=True)
     lens = cache.evict(table, lens + 1, keep=4096, first=4, recent=1024)
+
+A step that verifies a tree of s drafted tokens a sequence, node 0 the last known one::
+
+    q = cache.append(q, k, v, table, lens, freqs_cis, position=lens[:, None] + depth)
+    o = cache.attend_tree(q, table, lens + s, parent, scale)
+    sampled, _ = kernels.sample(logits, uniform, temperature=0.8, top_p=0.95)    # a row a node
+    lens, tokens, path = cache.accept(drafted, parent, sampled.view(b, s), table, lens)
 
 Every call runs on the current stream of the cache's device, allocates only its outputs, (unless
 given) its workspace and copies of tables and lengths that are not contiguous and of rows that are not
@@ -310,7 +317,8 @@ class PagedKV:
         s + i`` and sees the slots before the tree, itself and the nodes above it.  ``parent`` [b, s] int32: each node's
         parent, in any order; one outside [0, s) is none, and the node hangs on the prefix.  ``count`` [b] int32: the
         nodes of each sequence of a padded batch (its tree begins at ``lens[b] - count[b]``); the rows behind them are
-        0.  ``out`` may not overlap q; ``workspace``: of ``attend_tree_workspace_bytes``."""
+        0.  The kernel is chosen by the table's width, so the same tree over a wider table may round otherwise.  ``out``
+        may not overlap q; ``workspace``: of ``attend_tree_workspace_bytes``."""
         what = "PagedKV.attend_tree"
         if q.dim() != 4 or q.shape[3] != self.head_dim:
             raise ValueError(f"{what}: q must be [b, s, h, {self.head_dim}], got {list(q.shape)}")
