@@ -10,8 +10,8 @@
 //   * one barrier a tile: a tile that a wave's loads have brought is there for all behind it, and the tile before it is free;
 //   * p = 2^(y - m) as in paged_attn_kernel, m moved only when a tile's maximum exceeds it by more than 8.
 // Units, shares, partials and the join are paged_attn_kernel's, but that units without a row of a sequence's own nodes are none.
-// 8 trees of 64 nodes over 8191 tokens, 64 heads on 8 of 128 (268 MB, 137 GF) 164 us, 840 TFLOP/s, the matrix units busy
-// two fifths of it, the vector units as long; a product of 8192^3 by the library does 1218.
+// 8 trees of 64 nodes over 8191 tokens, 64 heads on 8 of 128 (268 MB, 137 GF) 157 to 195 us by card, mostly 161: 850 TFLOP/s,
+// the matrix units busy two fifths of it, the vector units as long; a product of 8192^3 by the library does 1218.
 #pragma once
 
 #include <cfloat>
